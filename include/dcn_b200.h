@@ -341,6 +341,72 @@ DCN_API int dcn_deform_conv2d_backward_overlap(const dcn_conv_desc *desc, const 
                                                dcn_params_ready_fn params_ready, void *user_data);
 
 /* ---------------------------------------------------------------------
+ * AdamW step over many tensors (no reference counterpart: the reference
+ * leaves the optimizer to its caller).  With t = steps taken + 1 and
+ * g = grad * grad_scale, for every element of every tensor:
+ *   m' = b1 m + (1 - b1) g,   v' = b2 v + (1 - b2) g^2
+ *   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+ * in fp32.  `param` is rounded once to its dtype; with `master` (fp32, numel
+ * elements) the fp32 value is read from and kept there.
+ * state_bits 32: exp_avg (m) and exp_avg_sq (v) are fp32 arrays.
+ * state_bits 8: they are float8 e4m3 codes of m and of sqrt(v), one byte per
+ * element, with one fp32 scale per 256 elements (ceil(numel / 256) each) in
+ * exp_avg_scale / exp_avg_sq_scale; a state of zeros starts from codes 0.
+ * Codes are rounded stochastically from a hash of the element's index, the
+ * step and `seed`: the same call on the same state gives the same bits.
+ * `step` points at two int32 on the device: the steps taken, and a ticket
+ * that is 0 between calls; tensors may share one.  The call advances each
+ * counter by one.  All tensors of one call are stepped together; calls that
+ * share tensors or counters must not overlap on the GPU.
+ * grad_scale (one fp32 on the device, or NULL for 1) multiplies the
+ * gradients; when it is not finite the whole step is skipped and nothing is
+ * written, counters included.  lr_device (one fp32 on the device), when not
+ * NULL, replaces lr, so that a captured call follows a schedule.
+ * Gradients are not written.  No workspace; one launch per dtype, presence of
+ * a master copy and 384 tensors.
+ */
+typedef struct dcn_adamw_tensor {
+  void *param;
+  const void *grad;         /* same dtype as param */
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale; /* state_bits 8, else NULL */
+  float *master;            /* fp32 copy of the parameter, or NULL */
+  int32_t *step;            /* two int32: steps taken, ticket (0) */
+  int64_t numel;
+  int32_t dtype;            /* DCN_FLOAT32 / DCN_FLOAT16 / DCN_BFLOAT16 */
+  int32_t reserved;         /* 0 */
+} dcn_adamw_tensor;
+typedef struct dcn_adamw_options {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float *lr_device;   /* or NULL */
+  const float *grad_scale;  /* or NULL */
+  int32_t state_bits;       /* 32 or 8 */
+  uint32_t seed;            /* of the 8-bit states' rounding */
+} dcn_adamw_options;
+DCN_API int dcn_adamw_step(const dcn_adamw_options *opt, const dcn_adamw_tensor *tensors, int64_t n,
+                           void *stream);
+
+/* ---------------------------------------------------------------------
+ * Global gradient norm and clipping factor (no reference counterpart):
+ *   norm   = sqrt(sum of the squares of all elements) / loss_scale
+ *   factor = min(1, max_norm / (norm + 1e-6)) / loss_scale
+ * two fp32 on the device.  A negative max_norm clips nothing.  When the norm
+ * is not finite the factor is NaN, which makes dcn_adamw_step skip its step:
+ * `factor` is meant as its grad_scale.  Sums are fp64 in a fixed order (the
+ * result is reproducible bit for bit).
+ */
+typedef struct dcn_tensor_ref {
+  const void *data;
+  int64_t numel;
+  int32_t dtype;
+  int32_t reserved; /* 0 */
+} dcn_tensor_ref;
+DCN_API size_t dcn_grad_norm_workspace_size(const dcn_tensor_ref *grads, int64_t n);
+DCN_API int dcn_grad_norm(const dcn_tensor_ref *grads, int64_t n, double max_norm, double loss_scale,
+                          float *norm, float *factor, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
+/* ---------------------------------------------------------------------
  * Device status.  Kernels with bounded waits record an expired wait in a
  * device-side status word instead of hanging.  This call copies and clears
  * it (it synchronises `stream`): DCN_OK, or DCN_ERR_DEVICE_TIMEOUT.

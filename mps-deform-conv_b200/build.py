@@ -92,10 +92,10 @@ def build_ext(force: bool = False) -> str:
     """Build the torch extension _C (C++ only; links libdcn_b200.so)."""
     import torch.utils.cpp_extension as ce
 
-    src = os.path.join(CSRC, "ext_C.cpp")
+    srcs = sorted(glob.glob(os.path.join(CSRC, "ext_*.cpp")))
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     out = os.path.join(PKG, "_C" + suffix)
-    if not force and not _stale(out, [src, LIB, os.path.join(INCLUDE, "dcn_b200.h")]):
+    if not force and not _stale(out, [*srcs, *glob.glob(os.path.join(CSRC, "ext_*.h")), LIB, os.path.join(INCLUDE, "dcn_b200.h")]):
         return out
     import torch
 
@@ -105,7 +105,7 @@ def build_ext(force: bool = False) -> str:
     incs = [INCLUDE, sysconfig.get_paths()["include"], *ce.include_paths(device_type="cuda")]
     libs = ce.library_paths(device_type="cuda")
     tmp = os.path.join(bdir, "_C" + suffix)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", tmp,
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *srcs, "-o", tmp,
            "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-fvisibility=hidden",
            *[f"-I{p}" for p in incs], *[f"-L{p}" for p in libs],

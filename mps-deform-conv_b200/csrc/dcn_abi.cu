@@ -69,8 +69,7 @@ KernelScope::~KernelScope() {
   g_prof.push_back({name_, start_, stop});
 }
 
-static int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -80,11 +79,11 @@ static int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-static int cuda_fail(cudaError_t e, const char* where) {
+int cuda_fail(cudaError_t e, const char* where) {
   return fail(DCN_ERR_CUDA, "%s: CUDA error %d (%s)", where, (int)e, cudaGetErrorString(e));
 }
 
-static int ok() {
+int ok() {
   g_last_error.clear();
   return DCN_OK;
 }

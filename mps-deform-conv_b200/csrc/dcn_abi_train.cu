@@ -1,0 +1,139 @@
+// dcn_abi_train.cu -- the extern "C" entry points of the training-block
+// operators of include/dcn_b200.h: argument checks and dispatch.
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
+#include "dcn_optim.h"
+
+namespace dcn {
+
+static bool dtype_ok(int32_t d) { return d == DCN_FLOAT32 || d == DCN_FLOAT16 || d == DCN_BFLOAT16; }
+static int64_t elem_bytes(int32_t d) { return d == DCN_FLOAT32 ? 4 : 2; }
+
+// No C++ exception leaves a C entry: the host-side tables are std::vectors.
+template <typename F>
+static int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(DCN_ERR_CUDA, "out of host memory");
+  } catch (...) {
+    return fail(DCN_ERR_CUDA, "unexpected host error");
+  }
+}
+
+constexpr int64_t kMaxNumel = int64_t(1) << 40;  // keeps every chunk count and byte offset in range
+
+static int check_adamw(const dcn_adamw_options* o, const dcn_adamw_tensor* t, int64_t n) {
+  if (!o) return fail(DCN_ERR_INVALID_ARGUMENT, "options are NULL");
+  if (n < 0 || (n > 0 && !t)) return fail(DCN_ERR_INVALID_ARGUMENT, "tensor list is NULL or its length negative");
+  if (o->state_bits != 32 && o->state_bits != 8)
+    return fail(DCN_ERR_UNSUPPORTED, "state_bits must be 32 or 8, got %d", o->state_bits);
+  if (!o->lr_device && !(o->lr >= 0.0 && isfinite(o->lr)))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "lr must be non-negative and finite, got %g", o->lr);
+  if (!(o->beta1 >= 0.0 && o->beta1 < 1.0) || !(o->beta2 >= 0.0 && o->beta2 < 1.0))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "betas must be in [0, 1), got (%g, %g)", o->beta1, o->beta2);
+  if (!(o->eps >= 0.0 && isfinite(o->eps)))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "eps must be non-negative and finite, got %g", o->eps);
+  if (!(o->weight_decay >= 0.0 && isfinite(o->weight_decay)))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "weight_decay must be non-negative and finite, got %g", o->weight_decay);
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  written.reserve((size_t)n * 4);
+  for (int64_t i = 0; i < n; ++i) {
+    const dcn_adamw_tensor& e = t[i];
+    if (!dtype_ok(e.dtype))
+      return fail(DCN_ERR_UNSUPPORTED, "tensor %lld: dtype %d is not one of float32, float16, bfloat16", (long long)i,
+                  e.dtype);
+    if (e.numel < 0 || e.numel > kMaxNumel)
+      return fail(DCN_ERR_UNSUPPORTED, "tensor %lld: %lld elements", (long long)i, (long long)e.numel);
+    if (!e.step) return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: step counter is NULL", (long long)i);
+    if (e.numel == 0) continue;
+    if (!e.param || !e.grad || !e.exp_avg || !e.exp_avg_sq)
+      return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: NULL pointer (param, grad, exp_avg, exp_avg_sq)", (long long)i);
+    if (o->state_bits == 8 && (!e.exp_avg_scale || !e.exp_avg_sq_scale))
+      return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: 8-bit states need exp_avg_scale and exp_avg_sq_scale",
+                  (long long)i);
+    const int64_t state = o->state_bits == 8 ? 1 : 4;
+    auto add = [&](const void* p, int64_t bytes) {
+      if (p) written.emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
+    };
+    add(e.param, e.numel * elem_bytes(e.dtype));
+    add(e.master, e.numel * 4);
+    add(e.exp_avg, e.numel * state);
+    add(e.exp_avg_sq, e.numel * state);
+    if (o->state_bits == 8) {
+      add(e.exp_avg_scale, (e.numel + 255) / 256 * 4);
+      add(e.exp_avg_sq_scale, (e.numel + 255) / 256 * 4);
+    }
+  }
+  // two CTAs must not update the same memory
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second)
+      return fail(DCN_ERR_INVALID_ARGUMENT,
+                  "parameters, master copies and states must not overlap one another (the same tensor twice?)");
+  return DCN_OK;
+}
+
+static int check_refs(const dcn_tensor_ref* t, int64_t n) {
+  if (n < 0 || (n > 0 && !t)) return fail(DCN_ERR_INVALID_ARGUMENT, "tensor list is NULL or its length negative");
+  for (int64_t i = 0; i < n; ++i) {
+    if (!dtype_ok(t[i].dtype))
+      return fail(DCN_ERR_UNSUPPORTED, "tensor %lld: dtype %d is not one of float32, float16, bfloat16", (long long)i,
+                  t[i].dtype);
+    if (t[i].numel < 0 || t[i].numel > kMaxNumel)
+      return fail(DCN_ERR_UNSUPPORTED, "tensor %lld: %lld elements", (long long)i, (long long)t[i].numel);
+  }
+  return DCN_OK;
+}
+
+}  // namespace dcn
+
+using namespace dcn;
+
+extern "C" {
+
+int dcn_adamw_step(const dcn_adamw_options* opt, const dcn_adamw_tensor* tensors, int64_t n, void* stream) {
+  return guarded([&] {
+    const int r = check_adamw(opt, tensors, n);
+    if (r != DCN_OK) return r;
+    const cudaError_t e = adamw_step(*opt, tensors, n, (cudaStream_t)stream);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "adamw_step");
+  });
+}
+
+size_t dcn_grad_norm_workspace_size(const dcn_tensor_ref* grads, int64_t n) {
+  size_t bytes = 0;
+  guarded([&] {
+    const int r = check_refs(grads, n);
+    if (r == DCN_OK) bytes = grad_norm_workspace(grads, n);
+    return r;
+  });
+  return bytes;
+}
+
+int dcn_grad_norm(const dcn_tensor_ref* grads, int64_t n, double max_norm, double loss_scale, float* norm,
+                  float* factor, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const int r = check_refs(grads, n);
+    if (r != DCN_OK) return r;
+    if (!(loss_scale > 0.0 && isfinite(loss_scale)))
+      return fail(DCN_ERR_INVALID_ARGUMENT, "loss_scale must be positive and finite, got %g", loss_scale);
+    if (isnan(max_norm)) return fail(DCN_ERR_INVALID_ARGUMENT, "max_norm is NaN");
+    if (!norm || !factor) return fail(DCN_ERR_INVALID_ARGUMENT, "NULL output (norm, factor)");
+    for (int64_t i = 0; i < n; ++i)
+      if (grads[i].numel && !grads[i].data)
+        return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: NULL pointer", (long long)i);
+    const size_t need = grad_norm_workspace(grads, n);
+    if (workspace_bytes < need || !workspace)
+      return fail(DCN_ERR_WORKSPACE, "grad_norm workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    const cudaError_t e = grad_norm(grads, n, max_norm, loss_scale, norm, factor, workspace, (cudaStream_t)stream);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "grad_norm");
+  });
+}
+
+}  // extern "C"

@@ -80,6 +80,12 @@ class KernelScope {
   cudaEvent_t start_ = nullptr;
 };
 
+// Status of a C ABI call (dcn_abi.cu): records the message of a failure for
+// dcn_last_error() and returns its code, or clears it and returns DCN_OK.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int cuda_fail(cudaError_t e, const char* where);
+int ok();
+
 // Round a byte count up to the 256-byte workspace alignment.
 inline size_t ws_align(size_t n) { return (n + 255) & ~size_t(255); }
 

@@ -16,33 +16,9 @@
 #include <tuple>
 #include <vector>
 
-#include "dcn_b200.h"
+#include "ext_common.h"
 
 namespace {
-
-int32_t dtype_code(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return DCN_FLOAT32;
-    case at::kHalf: return DCN_FLOAT16;
-    case at::kBFloat16: return DCN_BFLOAT16;
-    default:
-      TORCH_CHECK(false, "deform_conv2d: unsupported dtype ", t.scalar_type(),
-                  " (expected float32, float16 or bfloat16)");
-  }
-  return 0;
-}
-
-void check_cuda(const at::Tensor& t, const char* name, const at::Tensor& ref) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.device() == ref.device(), name, " must be on the same device as input (",
-              ref.device(), "), got ", t.device());
-  TORCH_CHECK(t.scalar_type() == ref.scalar_type(), name, " must have the same dtype as input (",
-              ref.scalar_type(), "), got ", t.scalar_type());
-}
-
-void check_status(int rc) {
-  TORCH_CHECK(rc == DCN_OK, dcn_last_error());
-}
 
 dcn_conv_desc make_desc(const at::Tensor& input, int64_t out_channels, int64_t kh, int64_t kw,
                         int64_t sh, int64_t sw, int64_t ph, int64_t pw, int64_t dh, int64_t dw,
@@ -79,14 +55,6 @@ void check_offset_mask(const dcn_conv_desc& d, const at::Tensor& offset, const a
                 "mask must have shape (", d.batch, ", ", T * d.n_offset_grps, ", ", out_h, ", ",
                 out_w, "), got ", mask.sizes());
   }
-}
-
-at::Tensor workspace(size_t bytes, const at::Tensor& like) {
-  return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, like.options().dtype(at::kByte));
-}
-
-void* stream_of(const at::Tensor& t) {
-  return (void*)at::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
 
 std::pair<int64_t, int64_t> out_size(const dcn_conv_desc& d) {
@@ -613,6 +581,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("stride_h"), py::arg("stride_w"), py::arg("pad_h"), py::arg("pad_w"), py::arg("dilation_h"),
         py::arg("dilation_w"), py::arg("n_weight_grps"), py::arg("n_offset_grps"),
         py::arg("output_mask") = std::vector<bool>{true, true, true, true}, py::arg("saved") = py::none());
+  bind_train(m);
   m.def("device_status", &device_status, "Raise if a kernel's bounded wait expired");
   m.def("abi_version", &dcn_abi_version);
 }

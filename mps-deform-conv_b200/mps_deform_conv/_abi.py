@@ -58,6 +58,27 @@ class DcnExOptions(ctypes.Structure):
                 ("flags", ctypes.c_int32)]
 
 
+class DcnAdamwTensor(ctypes.Structure):
+    """Mirror of ``dcn_adamw_tensor``."""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_avg_sq", ctypes.c_void_p), ("exp_avg_scale", ctypes.c_void_p),
+                ("exp_avg_sq_scale", ctypes.c_void_p), ("master", ctypes.c_void_p), ("step", ctypes.c_void_p),
+                ("numel", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class DcnAdamwOptions(ctypes.Structure):
+    """Mirror of ``dcn_adamw_options``."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("lr_device", ctypes.c_void_p),
+                ("grad_scale", ctypes.c_void_p), ("state_bits", ctypes.c_int32), ("seed", ctypes.c_uint32)]
+
+
+class DcnTensorRef(ctypes.Structure):
+    """Mirror of ``dcn_tensor_ref``."""
+    _fields_ = [("data", ctypes.c_void_p), ("numel", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 _O = ctypes.POINTER(DcnExOptions)
 # void (*dcn_params_ready_fn)(void* user_data)
 PARAMS_READY_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p)
@@ -97,6 +118,11 @@ SIGNATURES = {
     "dcn_deform_conv2d_forward_head": (ctypes.c_int, [_D, _V, _V, _V, _V, _V, _V, _SZ, _V, _SZ, _V]),
     "dcn_deform_conv2d_backward_head": (ctypes.c_int, [_D, _V, _V, _V, _V, _V, _SZ, _V, _V, _V, _V, _V, _SZ,
                                                        _V]),
+    "dcn_adamw_step": (ctypes.c_int, [ctypes.POINTER(DcnAdamwOptions), ctypes.POINTER(DcnAdamwTensor),
+                                      ctypes.c_int64, _V]),
+    "dcn_grad_norm_workspace_size": (_SZ, [ctypes.POINTER(DcnTensorRef), ctypes.c_int64]),
+    "dcn_grad_norm": (ctypes.c_int, [ctypes.POINTER(DcnTensorRef), ctypes.c_int64, ctypes.c_double, ctypes.c_double,
+                                     _V, _V, _V, _SZ, _V]),
     "dcn_device_status": (ctypes.c_int, [_V]),
     "dcn_uses_tensor_cores": (ctypes.c_int, [_D]),
     "dcn_debug_bounds_enabled": (ctypes.c_int, []),

@@ -1,0 +1,124 @@
+"""Host-side checks of the optimizer step and the gradient norm: the refusals of
+the C ABI (nothing launches) and of the Python layer."""
+import ctypes
+
+import pytest
+import torch
+
+from mps_deform_conv import _abi, optim
+
+
+def _options(**kw):
+    o = _abi.DcnAdamwOptions(1e-3, 0.9, 0.999, 1e-8, 0.01, None, None, 32, 0)
+    for k, v in kw.items():
+        setattr(o, k, v)
+    return o
+
+
+def _tensors(n=1, **kw):
+    """`n` tensors of 64 elements at made-up, disjoint addresses."""
+    t = (_abi.DcnAdamwTensor * n)()
+    for i in range(n):
+        base = 0x100000 * (i + 1)
+        t[i] = _abi.DcnAdamwTensor(base, base + 0x10000, base + 0x20000, base + 0x30000, None, None, None,
+                                   base + 0x50000, 64, _abi.DCN_FLOAT32, 0)
+        for k, v in kw.items():
+            setattr(t[i], k, v)
+    return t
+
+
+def _call(o, t, n):
+    lib = _abi.load()
+    rc = lib.dcn_adamw_step(ctypes.byref(o) if o is not None else None, t, n, None)
+    return rc, lib.dcn_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(lr=-1.0), "lr must be"), (dict(lr=float("nan")), "lr must be"),
+    (dict(beta1=1.0), "betas must be"), (dict(beta2=-0.1), "betas must be"),
+    (dict(eps=-1e-8), "eps must be"), (dict(weight_decay=float("inf")), "weight_decay must be"),
+    (dict(state_bits=16), "state_bits"),
+])
+def test_adamw_option_refusals(kw, needle):
+    rc, msg = _call(_options(**kw), _tensors(), 1)
+    assert rc != _abi.DCN_OK and needle in msg
+
+
+@pytest.mark.parametrize("kw,bits,needle", [
+    (dict(param=None), 32, "NULL"), (dict(grad=None), 32, "NULL"), (dict(exp_avg=None), 32, "NULL"),
+    (dict(exp_avg_sq=None), 32, "NULL"), (dict(step=None), 32, "step counter"), (dict(dtype=9), 32, "dtype"),
+    (dict(numel=-1), 32, "elements"), (dict(numel=1 << 41), 32, "elements"), (dict(), 8, "exp_avg_scale"),
+    (dict(exp_avg=0x100000), 32, "overlap"),                 # the state is the parameter
+    (dict(exp_avg_sq=0x120000 + 255), 32, "overlap"),        # the states overlap by one byte
+    (dict(master=0x100000 + 252), 32, "overlap"),
+])
+def test_adamw_tensor_refusals(kw, bits, needle):
+    rc, msg = _call(_options(state_bits=bits), _tensors(**kw), 1)
+    assert rc != _abi.DCN_OK and needle in msg
+
+
+def test_adamw_refuses_the_same_parameter_twice():
+    t = _tensors(3)
+    t[2].param = t[0].param
+    rc, msg = _call(_options(), t, 3)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "twice" in msg
+
+
+def test_adamw_empty_lists():
+    assert _call(_options(), None, 0)[0] == _abi.DCN_OK
+    assert _call(None, None, 0)[0] == _abi.DCN_ERR_INVALID_ARGUMENT
+    assert _call(_options(), None, 2)[0] == _abi.DCN_ERR_INVALID_ARGUMENT
+    assert _call(_options(), _tensors(), -1)[0] == _abi.DCN_ERR_INVALID_ARGUMENT
+
+
+def test_grad_norm_refusals_and_workspace():
+    lib = _abi.load()
+    ref = (_abi.DcnTensorRef * 2)(_abi.DcnTensorRef(0x1000, 100, _abi.DCN_FLOAT32, 0),
+                                  _abi.DcnTensorRef(None, 0, _abi.DCN_BFLOAT16, 0))
+    need = lib.dcn_grad_norm_workspace_size(ref, 2)
+    assert need >= 8
+
+    def call(max_norm=1.0, scale=1.0, norm=0x2000, factor=0x2004, ws=0x4000, size=need, n=2):
+        rc = lib.dcn_grad_norm(ref, n, max_norm, scale, norm, factor, ws, size, None)
+        return rc, lib.dcn_last_error().decode()
+
+    for kw, needle in ((dict(scale=0.0), "loss_scale"), (dict(scale=float("inf")), "loss_scale"),
+                       (dict(max_norm=float("nan")), "max_norm"), (dict(norm=None), "NULL output"),
+                       (dict(factor=None), "NULL output"), (dict(ws=None), "workspace"),
+                       (dict(size=need - 1), "workspace"), (dict(n=-1), "tensor list")):
+        rc, msg = call(**kw)
+        assert rc != _abi.DCN_OK and needle in msg, kw
+    ref[1] = _abi.DcnTensorRef(None, 5, _abi.DCN_BFLOAT16, 0)
+    assert "NULL pointer" in call()[1]
+    ref[1] = _abi.DcnTensorRef(0x1000, 5, 7, 0)
+    assert "dtype" in call()[1]
+    assert lib.dcn_grad_norm_workspace_size(ref, 2) == 0
+
+
+def test_python_layer_refuses_cpu_tensors_and_bad_arguments():
+    p = torch.zeros(4)
+    with pytest.raises(ValueError, match="must be on CUDA device"):
+        optim.adamw_step([p], [p], [p], [p], [optim.new_step("cpu")], lr=1e-3)
+    with pytest.raises(ValueError, match="must be on CUDA device"):
+        optim.grad_norm([p])
+    with pytest.raises(ValueError, match="holds no gradient"):
+        optim.grad_norm([None])
+    q = torch.nn.Parameter(torch.zeros(4))
+    for kw, needle in ((dict(lr=-1.0), "lr"), (dict(betas=(1.0, 0.9)), "betas"), (dict(eps=-1.0), "eps"),
+                       (dict(weight_decay=-1.0), "weight_decay"), (dict(state_bits=4), "state_bits")):
+        with pytest.raises(ValueError, match=needle):
+            optim.AdamW([q], **kw)
+    q.grad = torch.zeros(4)
+    with pytest.raises(ValueError, match="must be on CUDA device"):
+        optim.AdamW([q]).step()
+
+
+def test_state_layouts():
+    w = torch.empty(6, 5, 3, 3).to(memory_format=torch.channels_last)
+    m, s = optim.new_state(w, 32)
+    assert s is None and m.dtype == torch.float32 and m.stride() == w.stride() and not m.any()
+    c, s = optim.new_state(w, 8)
+    assert c.dtype == torch.float8_e4m3fn and c.stride() == w.stride() and s.shape == (2,)  # 270 elements
+    assert not c.float().any()
+    with pytest.raises(ValueError, match="state_bits"):
+        optim.new_state(w, 4)
