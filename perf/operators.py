@@ -332,13 +332,24 @@ def _updated(state):
     return {k: state[k] for k in keys if state.get(k) is not None}
 
 
+def _package():
+    """This repository's package (the repository's root is the working folder)."""
+    import os
+    import sys
+
+    at = os.path.abspath("mps-deform-conv_b200")
+    if at not in sys.path:
+        sys.path.insert(1, at)
+    import mps_deform_conv
+
+    return mps_deform_conv
+
+
 def run(state):
     case = state["case"]
     if case["op"] == "ffn":
         if own:
-            from mps_deform_conv import gated_feed_forward
-
-            y = gated_feed_forward(*state["args"], activation=case["activation"])
+            y = _package().gated_feed_forward(*state["args"], activation=case["activation"])
             if state["grad"] is None:
                 return [y]
             return [y.detach(), *torch.autograd.grad(y, [t for t in state["args"] if t is not None], state["grad"])]
@@ -346,17 +357,14 @@ def run(state):
             return [t.to(DTYPES[case["dtype"]]) for t in _ffn_in(state, torch.float32, case["activation"])]
     if case["op"] == "norm":
         if own:
-            from mps_deform_conv.optim import grad_norm
-
-            return list(grad_norm(state["grads"], max_norm=MAX_NORM, loss_scale=LOSS_SCALE))
+            return list(_package().optim.grad_norm(state["grads"], max_norm=MAX_NORM, loss_scale=LOSS_SCALE))
         return _norm_of(state["grads"], MAX_NORM, LOSS_SCALE)
     if own:
-        from mps_deform_conv.optim import adamw_step
-
-        adamw_step(state["params"], state["grads"], state["exp_avgs"], state["exp_avg_sqs"], state["steps"],
-                   masters=state["masters"], exp_avg_scales=state.get("exp_avg_scales"),
-                   exp_avg_sq_scales=state.get("exp_avg_sq_scales"), grad_scale=state["grad_scale"],
-                   seed=state["seed"], **state["hyper"])
+        _package().optim.adamw_step(
+            state["params"], state["grads"], state["exp_avgs"], state["exp_avg_sqs"], state["steps"],
+            masters=state["masters"], exp_avg_scales=state.get("exp_avg_scales"),
+            exp_avg_sq_scales=state.get("exp_avg_sq_scales"), grad_scale=state["grad_scale"], seed=state["seed"],
+            **state["hyper"])
         return _updated(state)
     for k in range(len(state["params"])):
         _adamw_one(state, k)
