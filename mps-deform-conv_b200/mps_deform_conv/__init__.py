@@ -19,6 +19,7 @@ import torch
 from torch import Tensor, nn
 
 from . import ops as _ops
+from . import optim
 
 __version__ = "0.2.2"
 
@@ -548,4 +549,4 @@ def is_available() -> bool:
 
 
 __all__ = ["deform_conv2d", "DeformConv2d", "ModulatedDeformConv2d", "is_available", "__version__",
-           "set_training_cache", "set_param_grad_hook", "set_head_fusion", "set_weight_image_cache"]
+           "optim", "set_training_cache", "set_param_grad_hook", "set_head_fusion", "set_weight_image_cache"]
