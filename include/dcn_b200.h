@@ -341,6 +341,58 @@ DCN_API int dcn_deform_conv2d_backward_overlap(const dcn_conv_desc *desc, const 
                                                dcn_params_ready_fn params_ready, void *user_data);
 
 /* ---------------------------------------------------------------------
+ * Gated feed-forward block, the channel mixing that follows a spatial layer
+ * (no reference counterpart).  Over the `tokens` rows (pixels) of x:
+ *   gate = x Wg^T + bg,  up = x Wu^T + bu
+ *   y    = (act(gate) * up) Wd^T + bd
+ *   x, y          [tokens][channels]   a channels-last map is [B*H*W][C]
+ *   w_gate, w_up  [hidden][channels]   b_gate, b_up  [hidden]    (NULL = none)
+ *   w_down        [channels][hidden]   b_down        [channels]  (NULL = none)
+ * b_gate and b_up go together.  All tensors are dense, of desc->dtype; x, y,
+ * the weights and their gradients start on 16-byte boundaries, workspace and
+ * saved state on 256-byte ones.  Any sizes (tokens may be 0).  Accumulation
+ * and elementwise work are fp32; the hidden values, and in the backward their
+ * two gradients, are rounded to the dtype as operands of the products that
+ * follow.  Activations: silu x / (1 + exp(-x)); gelu x Phi(x) (the exact
+ * form); relu; sigmoid.
+ *
+ * The forward leaves `saved` (dcn_ffn_saved_bytes, or NULL when no backward
+ * follows) for the backward of the same call: gate and up, and the hidden
+ * values.  y may be NULL when only the saved state is wanted (a backward that
+ * rebuilds it).  The backward takes the same x and weights; gradient pointers
+ * may be NULL; biases' gradients are not written when NULL.  Sums over tokens
+ * have a fixed order: results are reproducible bit for bit.  params_ready
+ * (may be NULL) is called as in dcn_deform_conv2d_backward_overlap once the
+ * gradients of the weights and biases are enqueued, before that of x.
+ */
+#define DCN_ACT_SILU 0
+#define DCN_ACT_GELU 1
+#define DCN_ACT_RELU 2
+#define DCN_ACT_SIGMOID 3
+typedef struct dcn_ffn_desc {
+  int32_t dtype;      /* DCN_FLOAT32 / DCN_FLOAT16 / DCN_BFLOAT16 */
+  int32_t activation; /* DCN_ACT_* */
+  int64_t tokens, channels, hidden;
+} dcn_ffn_desc;
+typedef struct dcn_ffn_tensors {
+  const void *x, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+} dcn_ffn_tensors;
+typedef struct dcn_ffn_grads {
+  void *x, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+} dcn_ffn_grads;
+DCN_API int dcn_ffn_validate(const dcn_ffn_desc *desc);
+DCN_API size_t dcn_ffn_saved_bytes(const dcn_ffn_desc *desc);
+/* save: whether the forward gets a saved state */
+DCN_API size_t dcn_ffn_forward_workspace_size(const dcn_ffn_desc *desc, int save);
+DCN_API int dcn_ffn_forward(const dcn_ffn_desc *desc, const dcn_ffn_tensors *t, void *y, void *saved,
+                            size_t saved_bytes, void *workspace, size_t workspace_bytes, void *stream);
+DCN_API size_t dcn_ffn_backward_workspace_size(const dcn_ffn_desc *desc);
+DCN_API int dcn_ffn_backward(const dcn_ffn_desc *desc, const dcn_ffn_tensors *t, const void *grad_y,
+                             const void *saved, size_t saved_bytes, const dcn_ffn_grads *grads,
+                             void *workspace, size_t workspace_bytes, void *stream,
+                             void (*params_ready)(void *user_data), void *user_data);
+
+/* ---------------------------------------------------------------------
  * AdamW step over many tensors (no reference counterpart: the reference
  * leaves the optimizer to its caller).  With t = steps taken + 1 and
  * g = grad * grad_scale, for every element of every tensor:

@@ -20,6 +20,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_ROOT = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_ROOT)
@@ -48,7 +49,16 @@ def _stale(out: str, deps) -> bool:
     if not os.path.exists(out):
         return True
     t = os.path.getmtime(out)
-    return any(os.path.getmtime(d) > t for d in deps)
+    return any(not os.path.exists(d) or os.path.getmtime(d) > t for d in deps)
+
+
+def _read_deps(path: str):
+    """Files named in a make dependency file; a missing file when it is absent (so the object is stale)."""
+    if not os.path.exists(path):
+        return [path]
+    with open(path) as f:
+        text = f.read().replace("\\\n", " ")
+    return [w for w in text.split(":", 1)[-1].split() if os.path.exists(w)]
 
 
 def build_lib(force: bool = False, verbose: bool = False, bounds: bool = False) -> str:
@@ -62,18 +72,27 @@ def build_lib(force: bool = False, verbose: bool = False, bounds: bool = False) 
         return out
     os.makedirs(bdir, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
-    objs = []
-    logs = []
-    for s in srcs:
-        o = os.path.join(bdir, os.path.basename(s) + ".o")
-        cmd = [_nvcc(), *NVCC_FLAGS, *(["-DDCN_DEBUG_BOUNDS"] if bounds else []), "-I", INCLUDE, "-I", CSRC,
-               "-c", s, "-o", o]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        logs.append(r.stdout + r.stderr)
+    nvcc = [_nvcc(), *NVCC_FLAGS, *(["-DDCN_DEBUG_BOUNDS"] if bounds else []), "-I", INCLUDE, "-I", CSRC]
+
+    def compile_one(src: str):
+        """Compile one file when it or a header it read last time is newer; returns (object, log)."""
+        obj = os.path.join(bdir, os.path.basename(src) + ".o")
+        if not force and not _stale(obj, [src, *_read_deps(obj + ".d")]) and os.path.exists(obj + ".log"):
+            with open(obj + ".log") as f:
+                return obj, f.read()
+        r = subprocess.run([*nvcc, "-MMD", "-MF", obj + ".d", "-c", src, "-o", obj], capture_output=True, text=True)
+        log = r.stdout + r.stderr
         if r.returncode != 0:
-            sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError(f"nvcc failed on {s}")
-        objs.append(o)
+            sys.stderr.write(log)
+            raise RuntimeError(f"nvcc failed on {src}")
+        with open(obj + ".log", "w") as f:
+            f.write(log)
+        return obj, log
+
+    with ThreadPoolExecutor(max_workers=max(1, min(len(srcs), os.cpu_count() or 1))) as pool:
+        done = list(pool.map(compile_one, srcs))
+    objs = [o for o, _ in done]
+    logs = [l for _, l in done]
     with open(os.path.join(bdir, "ptxas.log"), "w") as f:
         f.write("\n".join(logs))
     if verbose:

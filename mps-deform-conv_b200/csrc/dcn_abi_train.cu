@@ -7,6 +7,7 @@
 #include <utility>
 #include <vector>
 
+#include "dcn_ffn.h"
 #include "dcn_optim.h"
 
 namespace dcn {
@@ -91,6 +92,50 @@ static int check_refs(const dcn_tensor_ref* t, int64_t n) {
   return DCN_OK;
 }
 
+static int check_ffn(const dcn_ffn_desc* d) {
+  if (!d) return fail(DCN_ERR_INVALID_ARGUMENT, "descriptor is NULL");
+  if (!dtype_ok(d->dtype))
+    return fail(DCN_ERR_UNSUPPORTED, "dtype %d is not one of float32, float16, bfloat16", d->dtype);
+  if (d->activation < DCN_ACT_SILU || d->activation > DCN_ACT_SIGMOID)
+    return fail(DCN_ERR_INVALID_ARGUMENT, "unknown activation %d", d->activation);
+  if (d->tokens < 0 || d->channels <= 0 || d->hidden <= 0)
+    return fail(DCN_ERR_INVALID_ARGUMENT,
+                "sizes must be positive (tokens may be 0): tokens=%lld channels=%lld hidden=%lld", (long long)d->tokens,
+                (long long)d->channels, (long long)d->hidden);
+  // tensor-map extents, tile indices and byte strides stay in range
+  const int64_t lim = int64_t(1) << 20;
+  if (d->channels > lim || d->hidden > lim)
+    return fail(DCN_ERR_UNSUPPORTED, "channels (%lld) and hidden (%lld) may be at most %lld", (long long)d->channels,
+                (long long)d->hidden, (long long)lim);
+  const int64_t wide = d->channels > d->hidden ? d->channels : d->hidden;
+  if (d->tokens > (int64_t(1) << 30) || d->tokens > (int64_t(1) << 38) / wide)
+    return fail(DCN_ERR_UNSUPPORTED, "tokens (%lld) x %lld exceeds the size limit", (long long)d->tokens, (long long)wide);
+  return DCN_OK;
+}
+
+static FfnProblem problem(const dcn_ffn_desc* d) {
+  return {d->dtype, d->activation, d->tokens, d->channels, d->hidden};
+}
+
+static bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static int check_ffn_tensors(const dcn_ffn_tensors* t) {
+  if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down)
+    return fail(DCN_ERR_INVALID_ARGUMENT, "NULL tensor pointer (x, w_gate, w_up, w_down)");
+  if ((t->b_gate != nullptr) != (t->b_up != nullptr))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "b_gate and b_up go together");
+  if (!on16(t->x) || !on16(t->w_gate) || !on16(t->w_up) || !on16(t->w_down))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "x and the weights must be 16-byte aligned");
+  return DCN_OK;
+}
+
+static int check_buffer(const void* p, size_t have, size_t need, const char* what) {
+  if (need == 0) return DCN_OK;
+  if (!p || have < need) return fail(DCN_ERR_WORKSPACE, "%s too small: need %zu bytes, got %zu", what, need, p ? have : 0);
+  if (reinterpret_cast<uintptr_t>(p) & 255) return fail(DCN_ERR_INVALID_ARGUMENT, "%s must be 256-byte aligned", what);
+  return DCN_OK;
+}
+
 }  // namespace dcn
 
 using namespace dcn;
@@ -133,6 +178,77 @@ int dcn_grad_norm(const dcn_tensor_ref* grads, int64_t n, double max_norm, doubl
       return fail(DCN_ERR_WORKSPACE, "grad_norm workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
     const cudaError_t e = grad_norm(grads, n, max_norm, loss_scale, norm, factor, workspace, (cudaStream_t)stream);
     return e == cudaSuccess ? ok() : cuda_fail(e, "grad_norm");
+  });
+}
+
+int dcn_ffn_validate(const dcn_ffn_desc* desc) {
+  const int r = check_ffn(desc);
+  return r == DCN_OK ? ok() : r;
+}
+
+size_t dcn_ffn_saved_bytes(const dcn_ffn_desc* desc) {
+  return check_ffn(desc) == DCN_OK && desc->tokens ? ffn_saved_bytes(problem(desc)) : 0;
+}
+
+size_t dcn_ffn_forward_workspace_size(const dcn_ffn_desc* desc, int save) {
+  return check_ffn(desc) == DCN_OK && desc->tokens ? ffn_forward_workspace(problem(desc), save != 0) : 0;
+}
+
+size_t dcn_ffn_backward_workspace_size(const dcn_ffn_desc* desc) {
+  return check_ffn(desc) == DCN_OK && desc->tokens ? ffn_backward_workspace(problem(desc)) : 0;
+}
+
+int dcn_ffn_forward(const dcn_ffn_desc* desc, const dcn_ffn_tensors* t, void* y, void* saved, size_t saved_bytes,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    int r = check_ffn(desc);
+    if (r != DCN_OK) return r;
+    if (desc->tokens == 0) return ok();
+    if ((r = check_ffn_tensors(t)) != DCN_OK) return r;
+    if (!y && !saved) return fail(DCN_ERR_INVALID_ARGUMENT, "y and saved are both NULL");
+    if (y && !on16(y)) return fail(DCN_ERR_INVALID_ARGUMENT, "y must be 16-byte aligned");
+    const FfnProblem p = problem(desc);
+    if (saved && (r = check_buffer(saved, saved_bytes, ffn_saved_bytes(p), "saved state")) != DCN_OK) return r;
+    if ((r = check_buffer(workspace, workspace_bytes, ffn_forward_workspace(p, saved != nullptr), "forward workspace")) != DCN_OK)
+      return r;
+    const FfnTensors in{t->x, t->w_gate, t->w_up, t->w_down, t->b_gate, t->b_up, t->b_down};
+    const cudaError_t e = ffn_forward(p, in, y, saved, workspace, (cudaStream_t)stream);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "ffn_forward");
+  });
+}
+
+int dcn_ffn_backward(const dcn_ffn_desc* desc, const dcn_ffn_tensors* t, const void* grad_y, const void* saved,
+                     size_t saved_bytes, const dcn_ffn_grads* grads, void* workspace, size_t workspace_bytes,
+                     void* stream, void (*params_ready)(void* user_data), void* user_data) {
+  return guarded([&] {
+    int r = check_ffn(desc);
+    if (r != DCN_OK) return r;
+    if (!grads) return fail(DCN_ERR_INVALID_ARGUMENT, "grads is NULL");
+    const FfnGrads g{grads->x, grads->w_gate, grads->w_up, grads->w_down, grads->b_gate, grads->b_up, grads->b_down};
+    if (!on16(g.x) || !on16(g.w_gate) || !on16(g.w_up) || !on16(g.w_down))
+      return fail(DCN_ERR_INVALID_ARGUMENT, "gradients of x and of the weights must be 16-byte aligned");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (desc->tokens == 0) {  // sums over no rows
+      const size_t es = (size_t)elem_bytes(desc->dtype), c = (size_t)desc->channels, f = (size_t)desc->hidden;
+      const std::pair<void*, size_t> zero[6] = {{g.w_gate, c * f}, {g.w_up, c * f}, {g.w_down, c * f},
+                                                {g.b_gate, f},     {g.b_up, f},     {g.b_down, c}};
+      for (auto& z : zero)
+        if (z.first) {
+          const cudaError_t e = cudaMemsetAsync(z.first, 0, z.second * es, st);
+          if (e != cudaSuccess) return cuda_fail(e, "ffn_backward");
+        }
+      if (params_ready) params_ready(user_data);
+      return ok();
+    }
+    if ((r = check_ffn_tensors(t)) != DCN_OK) return r;
+    if (!grad_y || !on16(grad_y))
+      return fail(DCN_ERR_INVALID_ARGUMENT, "grad_y is NULL or not 16-byte aligned");
+    const FfnProblem p = problem(desc);
+    if ((r = check_buffer(saved, saved_bytes, ffn_saved_bytes(p), "saved state")) != DCN_OK) return r;
+    if ((r = check_buffer(workspace, workspace_bytes, ffn_backward_workspace(p), "backward workspace")) != DCN_OK) return r;
+    const FfnTensors in{t->x, t->w_gate, t->w_up, t->w_down, t->b_gate, t->b_up, t->b_down};
+    const cudaError_t e = ffn_backward(p, in, grad_y, saved, g, workspace, st, params_ready, user_data);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "ffn_backward");
   });
 }
 

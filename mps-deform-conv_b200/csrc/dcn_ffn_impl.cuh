@@ -1,0 +1,443 @@
+// dcn_ffn_impl.cuh -- the gated feed-forward block, forward and backward:
+//   gate = x Wg^T + bg, up = x Wu^T + bu, hidden = act(gate) * up, y = hidden Wd^T + bd
+//   dhidden = dy Wd, dgate = dhidden * up * act'(gate), dup = dhidden * act(gate)
+//   dx = dgate Wg + dup Wu, dWg = dgate^T x, dWu = dup^T x, dWd = dy^T hidden, db = column sums
+// Every product is ffn_gemm_kernel (dcn_ffn_gemm.cuh); this file plans the
+// launches, packs operands that the TMA cannot read in place, and finishes
+// sums that were split.  dcn_ffn_{bf16,fp16,fp32}.cu instantiate it.
+//
+// Work: 6 M C F flops forward, 12 M C F backward (M rows, C channels, F hidden).
+// The hidden values and the two hidden gradients are rounded to the data's
+// type, as operands of the following products; everything else stays in 32
+// bits to the final rounding.
+#pragma once
+
+#include <algorithm>
+#include <vector>
+
+#include "dcn_ffn_gemm.cuh"
+#include "dcn_ffn_layout.h"
+
+namespace dcn {
+
+using namespace ffn;
+
+namespace {
+
+// ---------------------------------------------------------------- operands
+bool make_map(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_rows) {
+  return make_tmap_3d(map, o.base, bf16, (uint64_t)o.planes, (uint64_t)o.rows, (uint64_t)o.cols, (uint64_t)o.ld,
+                      (uint64_t)o.plane, box_rows, BK);
+}
+
+// 32 x 32 blocks of a 16-bit result, staged with the 64-byte swizzle.
+bool make_store_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
+  return make_tmap_3d(map, base, bf16, 1, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint64_t)(rows * ld), 32, 32);
+}
+
+// ---------------------------------------------------------------- packing
+// Copies matrices into operand form: rows padded to 16 bytes, or fp32 values
+// as their three bf16 planes.  One launch for all matrices of a call; HBM
+// bound (a padded copy moves 4 bytes an element, the planes 10).
+struct PackJob {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, ld, plane;
+  int64_t first;  // first unit (8 columns of one row) of this job
+};
+struct PackArgs {
+  PackJob job[5];
+  int n;
+  int64_t units;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) ffn_pack_kernel(const __grid_constant__ PackArgs a) {
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.units; u += (int64_t)gridDim.x * 256) {
+    int k = 0;
+    while (k + 1 < a.n && u >= a.job[k + 1].first) ++k;
+    const PackJob& j = a.job[k];
+    const int64_t groups = j.ld / 8;
+    const int64_t row = (u - j.first) / groups, c0 = ((u - j.first) - row * groups) * 8;
+    const T* src = static_cast<const T*>(j.src) + row * j.cols + c0;
+    if constexpr (sizeof(T) == 4) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c0 + i < j.cols ? src[i] : 0.0f;
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(j.dst) + row * j.ld + c0;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        __nv_bfloat16 t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          t[i] = __float2bfloat16_rn(v[i]);
+          const float hi = __bfloat162float(t[i]);
+          // inf and NaN are the first plane's alone
+          v[i] = fabsf(hi) <= 3.4e38f ? v[i] - hi : 0.0f;
+        }
+        uint4 w;
+        memcpy(&w, t, 16);
+        *reinterpret_cast<uint4*>(dst + p * j.plane) = w;
+      }
+    } else {
+      T t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = c0 + i < j.cols ? src[i] : from_f<T>(0.0f);
+      uint4 w;
+      memcpy(&w, t, 16);
+      *reinterpret_cast<uint4*>(static_cast<T*>(j.dst) + row * j.ld + c0) = w;
+    }
+  }
+}
+
+struct Packer {
+  PackArgs a{};
+  void add(const Operand& o, const void* src) {
+    PackJob& j = a.job[a.n];
+    j = {src, const_cast<void*>(o.base), o.rows, o.cols, o.ld, o.plane, a.units};
+    a.units += o.rows * (o.ld / 8);
+    ++a.n;
+  }
+  template <typename T>
+  cudaError_t run(cudaStream_t st) const {
+    if (!a.n || !a.units) return cudaSuccess;
+    KernelScope ks("ffn_pack", st);
+    ffn_pack_kernel<T><<<(unsigned)std::min<int64_t>(div_up(a.units, 256), kSms * 8), 256, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+};
+
+// ---------------------------------------------------------------- split products
+// Adds the partials of each output tile in worker order (ffn_gemm_kernel's
+// slots) and stores T.  One warp per 32 x 32 block; reads are whole lines.
+struct ReduceArgs {
+  const float* partial;
+  void* out[2];
+  const void* bias;
+  int64_t ldo;
+  int M, N, tiles_m, tiles_n, batches, group_m, nkb, workers, vec;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__ ReduceArgs a) {
+  constexpr int BLOCKS = BN / 32 * 4;  // 32 x 32 blocks of a tile
+  const int lane = threadIdx.x & 31;
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.batches;
+  const int64_t unit = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5));
+  if (unit >= tiles * BLOCKS) return;
+  const int tile = (int)(unit / BLOCKS), blk = (int)(unit - (int64_t)tile * BLOCKS);
+  const int q = blk & 3, c = blk >> 2;
+  GemmArgs g;
+  g.tiles_m = a.tiles_m; g.tiles_n = a.tiles_n; g.group_m = a.group_m;
+  int z, mt, nt;
+  tile_at(g, tile, z, mt, nt);
+  const int64_t row = (int64_t)mt * BM + q * 32 + lane;
+  const int c0 = nt * BN + c * 32;
+  if (mt * BM + q * 32 >= a.M || c0 >= a.N) return;
+  const int64_t units = tiles * a.nkb;
+  const int64_t first = ((int64_t)tile * a.nkb + 1) * a.workers, last = (int64_t)(tile + 1) * a.nkb * a.workers;
+  const int w0 = (int)((first - 1) / units), w1 = (int)((last - 1) / units);
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+  for (int w = w0; w <= w1; ++w) {
+    const float* slot = a.partial + ((int64_t)w + tile) * (BM * BN) + q * (32 * BN) + c * 1024 + lane * 4;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 f = *reinterpret_cast<const float4*>(slot + j * 128);
+      v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+    }
+  }
+  if (row >= a.M) return;
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c0 + j < a.N) v[j] += to_f<T>(static_cast<const T*>(a.bias)[c0 + j]);
+  }
+  store_row32<T>(static_cast<T*>(a.out[z]) + row * a.ldo, c0, a.N, a.vec != 0, v);
+}
+
+// ---------------------------------------------------------------- column sums
+// Column sums of dy [M][C] (grad of the down bias): CTA (x, y) sums columns
+// 32 VEC x .. of rows y, y + gridDim.y, ... per warp; partials [gridDim.y * 8][C].
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) ffn_column_partial_kernel(const T* __restrict__ src, float* __restrict__ part,
+                                                                 int64_t M, int C) {
+  const int lane = threadIdx.x & 31;
+  const int64_t slice = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5), slices = (int64_t)gridDim.y * 8;
+  const int c0 = (blockIdx.x * 32 + lane) * VEC;
+  if (c0 >= C) return;
+  float acc[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+#pragma unroll 4
+  for (int64_t r = slice; r < M; r += slices) {
+    const T* p = src + r * C + c0;
+    if constexpr (VEC == 1) {
+      acc[0] += to_f<T>(p[0]);
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      T t[VEC];
+      memcpy(t, &w, 16);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] += to_f<T>(t[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) part[slice * C + c0 + j] = acc[j];
+}
+
+// out[k][c] = sum over the rows of part [rows][sets][N], in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(1024) ffn_column_finish_kernel(const float* __restrict__ part, T* out0, T* out1,
+                                                                 int64_t rows, int sets, int N) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane, k = blockIdx.y;
+  float acc = 0.0f;
+  if (c < N) {
+#pragma unroll 4
+    for (int64_t r = warp; r < rows; r += 32) acc += part[(r * sets + k) * N + c];
+  }
+  s[warp][lane] = acc;
+  __syncthreads();
+  if (warp == 0 && c < N) {
+    float t = 0.0f;
+    for (int w = 0; w < 32; ++w) t += s[w][lane];
+    T* out = k ? out1 : out0;
+    if (out) out[c] = from_f<T>(t);
+  }
+}
+
+template <typename T, int EPI, int BN, bool A_MN, bool B_MN>
+cudaError_t launch_gemm(const char* name, const Maps& maps, const GemmArgs& a, int workers, cudaStream_t st) {
+  auto kern = ffn_gemm_kernel<T, EPI, BN, A_MN, B_MN>;
+  const int smem = (int)(smem_bytes(BN) + kSmemSlack);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  KernelScope ks(name, st);
+  kern<<<workers, NTHREADS, smem, st>>>(maps, a);
+  return cudaGetLastError();
+}
+
+template <typename T, int EPI, bool A_MN, bool B_MN>
+cudaError_t launch_gemm(const char* name, const GemmPlan& p, const Maps& maps, const GemmArgs& a, cudaStream_t st) {
+  switch (p.bn) {
+    case 256:
+      if constexpr (sizeof(T) == 2) return launch_gemm<T, EPI, 256, A_MN, B_MN>(name, maps, a, p.workers, st);
+      return cudaErrorInvalidValue;  // fp32 plans stop at 128
+    case 128: return launch_gemm<T, EPI, 128, A_MN, B_MN>(name, maps, a, p.workers, st);
+    default: return launch_gemm<T, EPI, 64, A_MN, B_MN>(name, maps, a, p.workers, st);
+  }
+}
+
+// Segments of products of the given (a map, b map) pairs.
+template <typename T>
+int fill_segments(Seg* seg, const std::vector<std::pair<int, int>>& pairs) {
+  static const int kOrder[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
+  int n = 0;
+  if (sizeof(T) == 4) {
+    for (auto& o : kOrder)
+      for (auto& p : pairs) seg[n++] = {(uint8_t)p.first, (uint8_t)o[0], (uint8_t)p.second, (uint8_t)o[1]};
+  } else {
+    for (auto& p : pairs) seg[n++] = {(uint8_t)p.first, 0, (uint8_t)p.second, 0};
+  }
+  return n;
+}
+
+template <typename T>
+constexpr bool operand_bf16() { return !std::is_same<T, __half>::value; }
+
+// A product with plain sums as its result: out[z] = sum of the segments (+ bias).
+// a[z], z < batches: the row operands (one batch), or with one batch the row
+// operands of the pairs; b: the column operands of the pairs.
+template <typename T, bool A_MN, bool B_MN>
+cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, const std::vector<Operand>& b_ops,
+                          int64_t M, int64_t N, int64_t K, int batches, void* const* out, int64_t ldo,
+                          const void* bias, float* partial, cudaStream_t st) {
+  const int pairs = (int)b_ops.size();
+  Maps maps;
+  GemmArgs a{};
+  std::vector<std::pair<int, int>> pl;
+  const int n_a = (int)a_ops.size();
+  for (int i = 0; i < pairs; ++i) pl.push_back({i, n_a + i});
+  a.nseg = fill_segments<T>(a.seg, pl);
+  a.M = (int)M; a.N = (int)N;
+  a.nk = (int)div_up(K, BK);
+  const GemmPlan p = plan_gemm(M, N, (int64_t)a.nk * a.nseg, batches, false, true, sizeof(T) == 4);
+  for (int i = 0; i < n_a; ++i)
+    if (!make_map(&maps.m[i], a_ops[i], operand_bf16<T>(), A_MN ? BK : BM)) return cudaErrorInvalidValue;
+  for (int i = 0; i < pairs; ++i)
+    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B_MN ? BK : p.bn)) return cudaErrorInvalidValue;
+  a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n; a.batches = batches;
+  a.group_m = 8;
+  a.split = p.split;
+  a.operand_bf16 = operand_bf16<T>();
+  a.partial = partial;
+  a.out[0] = out[0];
+  a.out[1] = batches > 1 ? out[1] : nullptr;
+  a.ldo = ldo;
+  a.vec = (ldo * (int64_t)sizeof(T)) % 16 == 0;
+  for (int z = 0; z < batches; ++z) a.vec = a.vec && (reinterpret_cast<uintptr_t>(out[z]) & 15) == 0;
+  if (sizeof(T) == 2 && a.vec)
+    for (int z = 0; z < batches; ++z)
+      if (!make_store_map(&maps.out[z], out[z], operand_bf16<T>(), M, N, ldo)) return cudaErrorInvalidValue;
+  a.bias[0] = bias;
+  cudaError_t e = tc_status_ptr(&a.status);
+  if (e != cudaSuccess) return e;
+  if ((e = launch_gemm<T, EPI_STORE, A_MN, B_MN>(name, p, maps, a, st)) != cudaSuccess || !p.split) return e;
+  ReduceArgs r{};
+  r.partial = partial;
+  r.out[0] = a.out[0]; r.out[1] = a.out[1];
+  r.bias = bias;
+  r.ldo = ldo;
+  r.M = a.M; r.N = a.N; r.tiles_m = p.tiles_m; r.tiles_n = p.tiles_n; r.batches = batches; r.group_m = a.group_m;
+  r.nkb = a.nk * a.nseg; r.workers = p.workers; r.vec = a.vec;
+  const int64_t warps = (int64_t)p.tiles_m * p.tiles_n * batches * (p.bn / 32 * 4);
+  KernelScope ks("ffn_reduce", st);
+  const unsigned grid = (unsigned)div_up(warps, 8);
+  if (p.bn == 256) ffn_reduce_kernel<T, 256><<<grid, 256, 0, st>>>(r);
+  else if (p.bn == 128) ffn_reduce_kernel<T, 128><<<grid, 256, 0, st>>>(r);
+  else ffn_reduce_kernel<T, 64><<<grid, 256, 0, st>>>(r);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* saved, void* ws, cudaStream_t st) {
+  const Shape s(p);
+  void* hidden = saved ? static_cast<uint8_t*>(saved) + s.blocks_bytes() : nullptr;
+  const ForwardWs w(p, t, ws, hidden);
+  Packer pk;
+  if (w.pack_c) {
+    pk.add(w.x, t.x);
+    pk.add(w.wg, t.w_gate);
+    pk.add(w.wu, t.w_up);
+  }
+  if (w.pack_f) pk.add(w.wd, t.w_down);
+  cudaError_t e = pk.run<T>(st);
+  if (e != cudaSuccess) return e;
+
+  GemmArgs a{};
+  Maps maps;
+  a.nseg = fill_segments<T>(a.seg, {{0, 1}});
+  a.M = (int)s.M; a.N = (int)s.F;
+  a.nk = (int)div_up(s.C, BK);
+  const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, true, false, sizeof(T) == 4);
+  if (!make_map(&maps.m[0], w.x, operand_bf16<T>(), BM) || !make_map(&maps.m[1], w.wg, operand_bf16<T>(), plan.bn / 2) ||
+      !make_map(&maps.m[2], w.wu, operand_bf16<T>(), plan.bn / 2))
+    return cudaErrorInvalidValue;
+  a.tiles_m = plan.tiles_m; a.tiles_n = plan.tiles_n; a.batches = 1;
+  a.group_m = 8;
+  a.act = p.act;
+  a.operand_bf16 = operand_bf16<T>();
+  a.out[0] = const_cast<void*>(w.h.base);
+  a.ldo = w.h.ld;
+  a.plane = w.h.plane;
+  a.bias[0] = t.b_gate; a.bias[1] = t.b_up;
+  a.saved = saved;
+  if (sizeof(T) == 2 && !make_store_map(&maps.out[0], w.h.base, operand_bf16<T>(), s.M, s.F, w.h.ld))
+    return cudaErrorInvalidValue;
+  if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
+  if ((e = launch_gemm<T, EPI_GATED, false, false>("ffn_gate_up", plan, maps, a, st)) != cudaSuccess || !y) return e;
+  return store_product<T, false, false>("ffn_down", {w.h}, {w.wd}, s.M, s.C, s.F, 1, &y, s.C, t.b_down, w.partial, st);
+}
+
+template <typename T>
+cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy, const void* saved, const FfnGrads& g,
+                       void* ws, cudaStream_t st, dcn_params_ready_fn ready, void* user) {
+  const Shape s(p);
+  const BackwardWs w(p, t, dy, ws);
+  const Operand h = s.operand(static_cast<const uint8_t*>(saved) + s.blocks_bytes(), s.M, s.F);
+  Packer pk;
+  if (w.pack_c) {
+    pk.add(w.x, t.x);
+    pk.add(w.dy, dy);
+    pk.add(w.wg, t.w_gate);
+    pk.add(w.wu, t.w_up);
+  }
+  if (w.pack_f) pk.add(w.wd, t.w_down);
+  cudaError_t e = pk.run<T>(st);
+  if (e != cudaSuccess) return e;
+
+  const bool hidden_grads = g.x || g.w_gate || g.w_up || g.b_gate || g.b_up;
+  if (hidden_grads) {
+    GemmArgs a{};
+    Maps maps;
+    a.nseg = fill_segments<T>(a.seg, {{0, 1}});
+    a.M = (int)s.M; a.N = (int)s.F;
+    a.nk = (int)div_up(s.C, BK);
+    const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, false, false, sizeof(T) == 4);
+    if (!make_map(&maps.m[0], w.dy, operand_bf16<T>(), BM) || !make_map(&maps.m[1], w.wd, operand_bf16<T>(), BK))
+      return cudaErrorInvalidValue;
+    a.tiles_m = plan.tiles_m; a.tiles_n = plan.tiles_n; a.batches = 1;
+    a.group_m = 8;
+    a.act = p.act;
+    a.operand_bf16 = operand_bf16<T>();
+    a.out[0] = const_cast<void*>(w.dg.base); a.out[1] = const_cast<void*>(w.du.base);
+    a.ldo = w.dg.ld;
+    a.plane = w.dg.plane;
+    a.saved = const_cast<void*>(saved);
+    if (sizeof(T) == 2 && (!make_store_map(&maps.out[0], w.dg.base, operand_bf16<T>(), s.M, s.F, w.dg.ld) ||
+                           !make_store_map(&maps.out[1], w.du.base, operand_bf16<T>(), s.M, s.F, w.du.ld)))
+      return cudaErrorInvalidValue;
+    a.colsum = g.b_gate || g.b_up ? w.colsum : nullptr;
+    if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
+    if ((e = launch_gemm<T, EPI_DGATE, false, true>("ffn_dhidden", plan, maps, a, st)) != cudaSuccess) return e;
+    if (a.colsum) {
+      KernelScope ks("ffn_column_finish", st);
+      ffn_column_finish_kernel<T><<<dim3((unsigned)div_up(s.F, 32), 2), 1024, 0, st>>>(
+          w.colsum, static_cast<T*>(g.b_gate), static_cast<T*>(g.b_up), div_up(s.M, BM) * 4, 2, (int)s.F);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+  }
+  if (g.w_down &&
+      (e = store_product<T, true, true>("ffn_dw_down", {w.dy}, {h}, s.C, s.F, s.M, 1, &g.w_down, s.F, nullptr, w.partial, st)) !=
+          cudaSuccess)
+    return e;
+  if (g.w_gate && g.w_up) {
+    void* const out[2] = {g.w_gate, g.w_up};
+    e = store_product<T, true, true>("ffn_dw_gate_up", {w.dg, w.du}, {w.x}, s.F, s.C, s.M, 2, out, s.C, nullptr, w.partial, st);
+  } else if (g.w_gate || g.w_up) {
+    void* const out[1] = {g.w_gate ? g.w_gate : g.w_up};
+    e = store_product<T, true, true>("ffn_dw_gate_up", {g.w_gate ? w.dg : w.du}, {w.x}, s.F, s.C, s.M, 1, out, s.C, nullptr,
+                                     w.partial, st);
+  }
+  if (e != cudaSuccess) return e;
+  if (g.b_down) {
+    constexpr int kVec = 16 / sizeof(T);
+    const int64_t rows = std::min<int64_t>(div_up(s.M, 8), kSumSlices);
+    {
+      KernelScope ks("ffn_column_partial", st);
+      if (s.C % kVec == 0)
+        ffn_column_partial_kernel<T, kVec><<<dim3((unsigned)div_up(s.C, 32 * kVec), (unsigned)rows), 256, 0, st>>>(
+            static_cast<const T*>(dy), w.rowsum, s.M, (int)s.C);
+      else
+        ffn_column_partial_kernel<T, 1><<<dim3((unsigned)div_up(s.C, 32), (unsigned)rows), 256, 0, st>>>(
+            static_cast<const T*>(dy), w.rowsum, s.M, (int)s.C);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    KernelScope ks("ffn_column_finish", st);
+    ffn_column_finish_kernel<T><<<dim3((unsigned)div_up(s.C, 32), 1), 1024, 0, st>>>(
+        w.rowsum, static_cast<T*>(g.b_down), nullptr, rows * 8, 1, (int)s.C);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  if (ready) ready(user);
+  if (!g.x) return cudaSuccess;
+  return store_product<T, false, true>("ffn_dx", {w.dg, w.du}, {w.wg, w.wu}, s.M, s.C, s.F, 1, &g.x, s.C, nullptr, w.partial, st);
+}
+
+}  // namespace
+
+// The two passes of one data type, for dcn_ffn.cu.
+#define DCN_FFN_INSTANTIATE(T, name)                                                                              \
+  cudaError_t ffn_forward_##name(const FfnProblem& p, const FfnTensors& t, void* y, void* saved, void* workspace, \
+                                 cudaStream_t st) {                                                               \
+    return forward_t<T>(p, t, y, saved, workspace, st);                                                           \
+  }                                                                                                               \
+  cudaError_t ffn_backward_##name(const FfnProblem& p, const FfnTensors& t, const void* dy, const void* saved,    \
+                                  const FfnGrads& g, void* workspace, cudaStream_t st, dcn_params_ready_fn ready, \
+                                  void* user) {                                                                   \
+    return backward_t<T>(p, t, dy, saved, g, workspace, st, ready, user);                                         \
+  }
+
+}  // namespace dcn

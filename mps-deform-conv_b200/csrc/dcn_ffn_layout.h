@@ -1,0 +1,171 @@
+// dcn_ffn_layout.h -- the gated feed-forward block on the host: operand form,
+// launch plans, workspace and saved-state layouts.
+#pragma once
+
+#include <algorithm>
+
+#include "dcn_ffn.h"
+
+namespace dcn {
+namespace ffn {
+
+constexpr int kSms = 148;
+
+inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+inline int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
+
+constexpr int BM = 128;  // tile rows
+constexpr int BK = 64;   // contracted values of a stage (128 bytes)
+
+// Bytes of the saved gate and up values of a 32 x 32 block (dcn_ffn_gemm.cuh).
+constexpr size_t saved_block_bytes(bool wide) { return wide ? 8192 : 4096 + 64; }
+
+// A matrix as the products read it: 16-bit planes of [rows][ld], rows on
+// 16-byte boundaries.
+struct Operand {
+  const void* base = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0, plane = 0;
+  int planes = 1;
+};
+
+// ---------------------------------------------------------------- plans
+struct GemmPlan {
+  int bn = 256;
+  bool split = false;
+  int workers = 0;
+  int tiles_m = 0, tiles_n = 0;
+  size_t partial_bytes() const {
+    return split ? ((size_t)workers + (size_t)tiles_m * tiles_n * 2) * BM * bn * 4 : 0;
+  }
+};
+
+// Column tile: the one whose waves of tiles cost least, a tile's time being
+// its columns over the relative rate of that width (a narrower tile reads the
+// row operand more often for the same work).  splittable: the product stores
+// plain sums, so too few tiles for the SMs can be cut into equal runs.
+inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool gated, bool splittable,
+                          bool wide) {
+  GemmPlan best;
+  double best_cost = 1e300;
+  for (int bn : {256, 128, 64}) {
+    if (wide && bn == 256) continue;  // fp32 sums live in registers, half a row of them a thread
+    const int cols = gated ? bn / 2 : bn;
+    const double rate = bn == 256 ? 1.0 : bn == 128 ? 0.8 : 0.5;
+    const int64_t tm = div_up(M, BM), tn = div_up(N, cols), tiles = tm * tn * batches;
+    double cost = (double)div_up(tiles, kSms) * bn / rate * (double)nkb;
+    bool split = false;
+    if (splittable && tiles < 4 * kSms && tiles * nkb >= 8 * kSms) {
+      const double cut = (double)tiles / kSms * bn / rate * (double)nkb + 24.0 * bn;  // + writing and adding partials
+      if (cut < 0.95 * cost) {
+        split = true;
+        cost = cut;
+      }
+    }
+    if (cost < best_cost) {
+      best_cost = cost;
+      best.bn = bn;
+      best.split = split;
+      best.workers = (int)(split ? kSms : std::min<int64_t>(tiles, kSms));
+      best.tiles_m = (int)tm;
+      best.tiles_n = (int)tn;
+    }
+  }
+  return best;
+}
+
+inline size_t store_partial_bytes(int64_t M, int64_t N, int64_t K, int nseg, int batches) {
+  return ws_align(plan_gemm(M, N, div_up(K, BK) * nseg, batches, false, true, nseg >= 6).partial_bytes());
+}
+
+// ---------------------------------------------------------------- layouts
+struct Shape {
+  int64_t M, C, F;
+  bool wide;        // fp32 data: three planes
+  int planes, pair; // planes of an operand, segments of a product
+  size_t es;
+  explicit Shape(const FfnProblem& p)
+      : M(p.M), C(p.C), F(p.F), wide(p.dtype == DCN_FLOAT32), planes(wide ? 3 : 1), pair(wide ? 6 : 1), es(wide ? 4 : 2) {}
+  bool pack_rows_c() const { return wide || C % 8 != 0; }  // x, dy, w_gate, w_up: rows of C
+  bool pack_rows_f() const { return wide || F % 8 != 0; }  // w_down: rows of F
+  size_t operand_bytes(int64_t rows, int64_t cols) const {
+    return ws_align((size_t)planes * (size_t)rows * (size_t)round_up(cols, 8) * 2);
+  }
+  Operand operand(const void* base, int64_t rows, int64_t cols) const {
+    Operand o;
+    o.base = base;
+    o.rows = rows;
+    o.cols = cols;
+    o.ld = round_up(cols, 8);
+    o.plane = rows * o.ld;
+    o.planes = planes;
+    return o;
+  }
+  size_t blocks_bytes() const {
+    const int64_t m = div_up(M, BM) * 4, c = div_up(F, 32);
+    return ws_align((size_t)(m * c) * saved_block_bytes(wide));
+  }
+};
+
+// Hands out consecutive 256-byte-aligned pieces of a buffer.
+struct Carver {
+  uint8_t* base;
+  size_t at = 0;
+  void* take(size_t bytes) {
+    void* p = base ? base + at : nullptr;
+    at += ws_align(bytes);
+    return p;
+  }
+};
+
+struct ForwardWs {
+  Operand x, wg, wu, wd, h;
+  float* partial;
+  size_t total;
+  bool pack_c, pack_f;
+  ForwardWs(const FfnProblem& p, const FfnTensors& t, void* ws, void* hidden) {
+    const Shape s(p);
+    Carver c{static_cast<uint8_t*>(ws)};
+    pack_c = s.pack_rows_c();
+    pack_f = s.pack_rows_f();
+    x = s.operand(pack_c ? c.take(s.operand_bytes(s.M, s.C)) : t.x, s.M, s.C);
+    wg = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_gate, s.F, s.C);
+    wu = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_up, s.F, s.C);
+    wd = s.operand(pack_f ? c.take(s.operand_bytes(s.C, s.F)) : t.w_down, s.C, s.F);
+    h = s.operand(hidden ? hidden : c.take(s.operand_bytes(s.M, s.F)), s.M, s.F);
+    partial = static_cast<float*>(c.take(store_partial_bytes(s.M, s.C, s.F, s.pair, 1)));
+    total = c.at;
+  }
+};
+
+constexpr int kSumSlices = 64;  // CTA rows of the dy column sums
+
+struct BackwardWs {
+  Operand x, dy, wg, wu, wd, dg, du;
+  float *partial, *colsum, *rowsum;
+  size_t total;
+  bool pack_c, pack_f;
+  BackwardWs(const FfnProblem& p, const FfnTensors& t, const void* grad, void* ws) {
+    const Shape s(p);
+    Carver c{static_cast<uint8_t*>(ws)};
+    pack_c = s.pack_rows_c();
+    pack_f = s.pack_rows_f();
+    x = s.operand(pack_c ? c.take(s.operand_bytes(s.M, s.C)) : t.x, s.M, s.C);
+    dy = s.operand(pack_c ? c.take(s.operand_bytes(s.M, s.C)) : grad, s.M, s.C);
+    wg = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_gate, s.F, s.C);
+    wu = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_up, s.F, s.C);
+    wd = s.operand(pack_f ? c.take(s.operand_bytes(s.C, s.F)) : t.w_down, s.C, s.F);
+    dg = s.operand(c.take(s.operand_bytes(s.M, s.F)), s.M, s.F);
+    du = s.operand(c.take(s.operand_bytes(s.M, s.F)), s.M, s.F);
+    const size_t part = std::max({store_partial_bytes(s.C, s.F, s.M, s.pair, 1),
+                                  store_partial_bytes(s.F, s.C, s.M, s.pair, 1),
+                                  store_partial_bytes(s.F, s.C, s.M, s.pair, 2),
+                                  store_partial_bytes(s.M, s.C, s.F, 2 * s.pair, 1)});
+    partial = static_cast<float*>(c.take(part));
+    colsum = static_cast<float*>(c.take((size_t)div_up(s.M, BM) * 4 * 2 * (size_t)s.F * 4));
+    rowsum = static_cast<float*>(c.take((size_t)kSumSlices * 8 * (size_t)s.C * 4));
+    total = c.at;
+  }
+};
+
+}  // namespace ffn
+}  // namespace dcn

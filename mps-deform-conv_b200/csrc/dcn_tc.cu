@@ -29,6 +29,8 @@
 //               copy.  No multicast.
 // Every mbarrier wait is bounded (dcn_sm100.cuh): on expiry the kernel sets
 // the device status word and unwinds.
+#include <atomic>
+
 #include <mutex>
 #include <type_traits>
 
@@ -434,29 +436,51 @@ cudaError_t tc_status_ptr(int** out) {
   return e;
 }
 
-bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols,
-                  uint32_t box_rows, uint32_t box_cols) {
-  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                               CUtensorMapFloatOOBfill);
-  static EncodeFn encode = nullptr;
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn tmap_encoder() {
+  static std::atomic<EncodeFn> cached{nullptr};
+  EncodeFn encode = cached.load(std::memory_order_acquire);
   if (!encode) {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
         q != cudaDriverEntryPointSuccess || !fn)
-      return false;
+      return nullptr;
     encode = reinterpret_cast<EncodeFn>(fn);
+    cached.store(encode, std::memory_order_release);
   }
+  return encode;
+}
+
+static bool encode_tmap(CUtensorMap* map, const void* base, bool bf16, int rank, const cuuint64_t* dims,
+                        const cuuint64_t* strides, const cuuint32_t* box,
+                        CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+  const EncodeFn encode = tmap_encoder();
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return encode &&
+         encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols,
+                  uint32_t box_rows, uint32_t box_cols) {
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {cols * 2};
   const cuuint32_t box[2] = {box_cols, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tmap(map, base, bf16, 2, dims, strides, box);
+}
+
+bool make_tmap_3d(CUtensorMap* map, const void* base, bool bf16, uint64_t planes, uint64_t rows, uint64_t cols,
+                  uint64_t ld, uint64_t plane, uint32_t box_rows, uint32_t box_cols) {
+  const cuuint64_t dims[3] = {cols, rows, planes};
+  const cuuint64_t strides[2] = {ld * 2, plane * 2};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1};
+  return encode_tmap(map, base, bf16, 3, dims, strides, box,
+                     box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Forward weight image wsw of `w` (weight_images_kernel, or the per-image

@@ -1,5 +1,6 @@
 // ext_train.cpp -- the training-block operators of the Python module
 // `mps_deform_conv._C`: tensors to pointers and shapes over the C ABI.
+#include <exception>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -45,6 +46,138 @@ const float* scalar_ptr(const std::optional<at::Tensor>& t, const char* name, co
 }
 
 }  // namespace
+
+// ---------------------------------------------------------------- gated feed-forward block
+namespace {
+
+// A dense copy-free view where the tensor allows it, else a dense copy; 16-byte aligned.
+at::Tensor dense16(const at::Tensor& t) {
+  at::Tensor r = t.contiguous();
+  if ((reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) != 0) r = r.clone(at::MemoryFormat::Contiguous);
+  return r;
+}
+
+using OptTensor = std::optional<at::Tensor>;
+
+struct FfnArgs {
+  dcn_ffn_desc d;
+  at::Tensor x, w_gate, w_up, w_down, b_gate, b_up, b_down;  // dense; biases may be undefined
+  dcn_ffn_tensors t;
+  FfnArgs(const at::Tensor& input, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
+          const OptTensor& bg, const OptTensor& bu, const OptTensor& bd, int64_t activation) {
+    TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+    TORCH_CHECK(input.dim() >= 1, "input must have a channel dimension");
+    check_cuda(wg, "w_gate", input);
+    check_cuda(wu, "w_up", input);
+    check_cuda(wd, "w_down", input);
+    const int64_t c = input.size(-1);
+    TORCH_CHECK(wg.dim() == 2 && wg.size(1) == c, "w_gate must have shape (hidden, ", c, "), got ", wg.sizes());
+    const int64_t f = wg.size(0);
+    TORCH_CHECK(wu.sizes() == wg.sizes(), "w_up must have shape ", wg.sizes(), " as w_gate, got ", wu.sizes());
+    TORCH_CHECK(wd.dim() == 2 && wd.size(0) == c && wd.size(1) == f, "w_down must have shape (", c, ", ", f, "), got ",
+                wd.sizes());
+    TORCH_CHECK(bg.has_value() == bu.has_value(), "b_gate and b_up go together");
+    d.dtype = dtype_code(input);
+    d.activation = (int32_t)activation;
+    d.channels = c;
+    d.hidden = f;
+    d.tokens = c > 0 ? input.numel() / c : 0;
+    check_status(dcn_ffn_validate(&d));
+    x = dense16(input);
+    w_gate = dense16(wg);
+    w_up = dense16(wu);
+    w_down = dense16(wd);
+    auto bias = [&](const OptTensor& b, const char* name, int64_t n) {
+      if (!b.has_value()) return at::Tensor();
+      check_cuda(*b, name, input);
+      TORCH_CHECK(b->dim() == 1 && b->size(0) == n, name, " must have ", n, " elements, got ", b->sizes());
+      return b->contiguous();
+    };
+    b_gate = bias(bg, "b_gate", f);
+    b_up = bias(bu, "b_up", f);
+    b_down = bias(bd, "b_down", c);
+    auto p = [](const at::Tensor& v) -> const void* { return v.defined() ? v.data_ptr() : nullptr; };
+    t = {p(x), p(w_gate), p(w_up), p(w_down), p(b_gate), p(b_up), p(b_down)};
+  }
+};
+
+}  // namespace
+
+// (output, saved state); the state is empty unless keep_saved, the output when !want_output.
+std::tuple<at::Tensor, at::Tensor> gated_feed_forward_forward(const at::Tensor& input, const at::Tensor& w_gate,
+                                                              const at::Tensor& w_up, const at::Tensor& w_down,
+                                                              const OptTensor& b_gate, const OptTensor& b_up,
+                                                              const OptTensor& b_down, int64_t activation,
+                                                              bool keep_saved, bool want_output) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(input.device());
+  const FfnArgs a(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
+  at::Tensor out = want_output ? at::empty_like(a.x) : at::empty({0}, input.options());
+  const size_t sbytes = keep_saved ? dcn_ffn_saved_bytes(&a.d) : 0;
+  auto saved = at::empty({(int64_t)sbytes}, input.options().dtype(at::kByte));
+  auto ws = workspace(dcn_ffn_forward_workspace_size(&a.d, sbytes != 0), input);
+  check_status(dcn_ffn_forward(&a.d, &a.t, want_output ? out.data_ptr() : nullptr, sbytes ? saved.data_ptr() : nullptr,
+                               sbytes, ws.data_ptr(), (size_t)ws.numel(), stream_of(input)));
+  return {out, saved};
+}
+
+// Gradients of (input, w_gate, w_up, w_down, b_gate, b_up, b_down) by output_mask;
+// the others are undefined.  params_ready(grad_weight, grad_bias), when given, is
+// called for each of the three weights once they are enqueued.
+std::vector<at::Tensor> gated_feed_forward_backward(const at::Tensor& grad_output, const at::Tensor& input,
+                                                    const at::Tensor& w_gate, const at::Tensor& w_up,
+                                                    const at::Tensor& w_down, const OptTensor& b_gate,
+                                                    const OptTensor& b_up, const OptTensor& b_down, int64_t activation,
+                                                    const at::Tensor& saved, std::vector<bool> output_mask,
+                                                    const std::optional<py::function>& params_ready) {
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(input.device());
+  check_cuda(grad_output, "grad_output", input);
+  TORCH_CHECK(grad_output.sizes() == input.sizes(), "grad_output must have shape ", input.sizes(), ", got ",
+              grad_output.sizes());
+  TORCH_CHECK(output_mask.size() == 7, "output_mask must have 7 entries");
+  const FfnArgs a(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
+  if (a.d.tokens > 0)
+    TORCH_CHECK(saved.is_cuda() && saved.device() == input.device() && saved.scalar_type() == at::kByte &&
+                    saved.is_contiguous(),
+                "saved state must be a contiguous uint8 tensor on the input's device");
+  const at::Tensor dy = dense16(grad_output);
+  const at::Tensor like[7] = {a.x, a.w_gate, a.w_up, a.w_down, a.b_gate, a.b_up, a.b_down};
+  std::vector<at::Tensor> g(7);
+  void* ptr[7];
+  for (int i = 0; i < 7; ++i) {
+    if (output_mask[i] && like[i].defined()) g[i] = at::empty_like(like[i], at::MemoryFormat::Contiguous);
+    ptr[i] = g[i].defined() ? g[i].data_ptr() : nullptr;
+  }
+  const dcn_ffn_grads grads{ptr[0], ptr[1], ptr[2], ptr[3], ptr[4], ptr[5], ptr[6]};
+  auto ws = workspace(dcn_ffn_backward_workspace_size(&a.d), input);
+  // a Python exception of the hook is held and re-raised after the call, never thrown through the C ABI
+  struct Ready {
+    const py::function* fn;
+    const std::vector<at::Tensor>* g;
+    std::exception_ptr err;
+  } ready{nullptr, &g, nullptr};
+  const bool hook = params_ready.has_value() && !params_ready->is_none();
+  if (hook) ready.fn = &*params_ready;
+  auto tramp = [](void* u) {
+    auto* r = static_cast<Ready*>(u);
+    try {
+      auto cast = [](const at::Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+      for (int i = 1; i <= 3; ++i) {
+        const at::Tensor &w = (*r->g)[i], &b = (*r->g)[i + 3];
+        if (w.defined() || b.defined()) (*r->fn)(cast(w), cast(b));
+      }
+    } catch (...) {
+      r->err = std::current_exception();
+    }
+  };
+  const int rc = dcn_ffn_backward(&a.d, &a.t, dy.data_ptr(), a.d.tokens ? saved.data_ptr() : nullptr,
+                                  (size_t)saved.numel(), &grads, ws.data_ptr(), (size_t)ws.numel(), stream_of(input),
+                                  hook ? +tramp : nullptr, hook ? &ready : nullptr);
+  if (ready.err) std::rethrow_exception(ready.err);
+  check_status(rc);
+  return g;
+}
 
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
                 const Tensors& steps, const std::optional<Tensors>& masters,
@@ -164,6 +297,13 @@ std::tuple<at::Tensor, at::Tensor> grad_norm(const Tensors& grads, double max_no
 }
 
 void bind_train(py::module_& m) {
+  m.def("gated_feed_forward_forward", &gated_feed_forward_forward, "Gated feed-forward block: (output, saved)",
+        py::arg("input"), py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"), py::arg("b_gate"), py::arg("b_up"),
+        py::arg("b_down"), py::arg("activation"), py::arg("keep_saved") = false, py::arg("want_output") = true);
+  m.def("gated_feed_forward_backward", &gated_feed_forward_backward,
+        "Gradients of (input, w_gate, w_up, w_down, b_gate, b_up, b_down)", py::arg("grad_output"), py::arg("input"),
+        py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"), py::arg("b_gate"), py::arg("b_up"), py::arg("b_down"),
+        py::arg("activation"), py::arg("saved"), py::arg("output_mask"), py::arg("params_ready") = py::none());
   m.def("adamw_step", &adamw_step, "AdamW step over many tensors, in place", py::arg("params"), py::arg("grads"),
         py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("steps"), py::arg("masters"), py::arg("exp_avg_scales"),
         py::arg("exp_avg_sq_scales"), py::arg("lr"), py::arg("lr_tensor"), py::arg("beta1"), py::arg("beta2"),

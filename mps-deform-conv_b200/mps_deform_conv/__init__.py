@@ -543,10 +543,152 @@ class ModulatedDeformConv2d(nn.Module):
         )
 
 
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+class _GatedFeedForwardFunction(torch.autograd.Function):
+    """Autograd function of the gated feed-forward block.  With the training
+    cache the forward keeps gate, up and the hidden values; without it the
+    backward computes them again from the input."""
+
+    @staticmethod
+    def forward(ctx, input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
+        needs = any(ctx.needs_input_grad)
+        output, saved = _get_lib().gated_feed_forward_forward(
+            input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, needs and _training_cache)
+        ctx.save_for_backward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, saved if saved.numel() > 0 else None)
+        ctx.activation = activation
+        return output
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        *tensors, saved = ctx.saved_tensors
+        lib = _get_lib()
+        if saved is None:
+            _, saved = lib.gated_feed_forward_forward(*tensors, ctx.activation, True, False)
+        grads = lib.gated_feed_forward_backward(grad_output, *tensors, ctx.activation, saved,
+                                                list(ctx.needs_input_grad[:7]), _param_grad_hook)
+        return (*grads, None)
+
+
+def _validate_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation) -> int:
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    if input.dim() < 1:
+        raise ValueError("input must have a channel dimension")
+    channels = input.size(-1)
+    if w_gate.dim() != 2 or w_gate.size(1) != channels:
+        raise ValueError(f"w_gate must have shape (hidden, {channels}), got {tuple(w_gate.shape)}")
+    hidden = w_gate.size(0)
+    if w_up.shape != w_gate.shape:
+        raise ValueError(f"w_up must have shape {tuple(w_gate.shape)} as w_gate, got {tuple(w_up.shape)}")
+    if tuple(w_down.shape) != (channels, hidden):
+        raise ValueError(f"w_down must have shape ({channels}, {hidden}), got {tuple(w_down.shape)}")
+    if channels == 0 or hidden == 0:
+        raise ValueError(f"channels and hidden must be positive, got {channels} and {hidden}")
+    if (b_gate is None) != (b_up is None):
+        raise ValueError("b_gate and b_up go together")
+    for tensor, name, size in ((b_gate, "b_gate", hidden), (b_up, "b_up", hidden), (b_down, "b_down", channels)):
+        if tensor is not None and tuple(tensor.shape) != (size,):
+            raise ValueError(f"{name} must have shape ({size},), got {tuple(tensor.shape)}")
+    for tensor, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down"), (b_gate, "b_gate"), (b_up, "b_up"),
+                         (b_down, "b_down")):
+        if tensor is not None:
+            _check_tensor_device(tensor, name, input.device)
+    return _ACTIVATIONS[activation]
+
+
+def gated_feed_forward(
+    input: Tensor,
+    w_gate: Tensor,
+    w_up: Tensor,
+    w_down: Tensor,
+    b_gate: Optional[Tensor] = None,
+    b_up: Optional[Tensor] = None,
+    b_down: Optional[Tensor] = None,
+    activation: str = "silu",
+) -> Tensor:
+    """
+    Gated feed-forward block over the last dimension:
+    ``(act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd``.
+
+    The channel mixing of a backbone block; the reference has none, its users
+    compose it from torch's linear layers.
+
+    Args:
+        input: Input tensor (..., C); a channels_last map enters as
+            ``map.permute(0, 2, 3, 1)`` without a copy
+        w_gate, w_up: Weights (hidden, C)
+        w_down: Weight (C, hidden)
+        b_gate, b_up: Optional biases (hidden,), both or neither
+        b_down: Optional bias (C,)
+        activation: "silu", "gelu" (the exact form), "relu" or "sigmoid"
+
+    Returns:
+        Output tensor (..., C), contiguous
+
+    Raises:
+        ValueError: If input is not on a CUDA device or shapes do not fit.
+
+    float32, float16 or bfloat16, all tensors alike.  Sums are fp32; the hidden
+    values are rounded to the dtype between the two products.  With
+    ``set_training_cache(False)`` the forward keeps nothing for the backward,
+    which then computes gate and up again.  The parameter-gradient hook is
+    called once for each of the three weights.
+    """
+    traced = input.device.type == "meta" or torch.compiler.is_compiling()
+    if not (input.device.type == "cuda" or traced):
+        raise ValueError(f"Input must be on CUDA device, got {input.device}")
+    act = _validate_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
+    if traced:
+        return _ops.traced_gated_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+    return _GatedFeedForwardFunction.apply(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+
+
+class GatedFeedForward2d(nn.Module):
+    """Gated feed-forward block over the channels of a feature map (N, C, H, W).
+
+    Stands after a deformable layer in a backbone block: a channels_last map is
+    read and returned as it is; other maps are brought to that order and back.
+    """
+
+    def __init__(self, channels: int, hidden: int, bias: bool = True, activation: str = "silu"):
+        super().__init__()
+        if channels <= 0 or hidden <= 0:
+            raise ValueError(f"channels and hidden must be positive, got {channels} and {hidden}")
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+        self.channels = channels
+        self.hidden = hidden
+        self.activation = activation
+        self.w_gate = nn.Parameter(torch.empty(hidden, channels))
+        self.w_up = nn.Parameter(torch.empty(hidden, channels))
+        self.w_down = nn.Parameter(torch.empty(channels, hidden))
+        for name, size in (("b_gate", hidden), ("b_up", hidden), ("b_down", channels)):
+            self.register_parameter(name, nn.Parameter(torch.empty(size)) if bias else None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        for weight, bias in ((self.w_gate, self.b_gate), (self.w_up, self.b_up), (self.w_down, self.b_down)):
+            nn.init.kaiming_uniform_(weight, a=math.sqrt(5))
+            if bias is not None:
+                bound = 1 / math.sqrt(weight.size(1))
+                nn.init.uniform_(bias, -bound, bound)
+
+    def forward(self, input: Tensor) -> Tensor:
+        if input.dim() != 4:
+            raise ValueError(f"input must be 4-D (N, C, H, W), got {input.dim()}-D")
+        output = gated_feed_forward(input.permute(0, 2, 3, 1), self.w_gate, self.w_up, self.w_down, self.b_gate,
+                                    self.b_up, self.b_down, self.activation).permute(0, 3, 1, 2)
+        return output.contiguous() if input.is_contiguous() else output
+
+
 def is_available() -> bool:
     """True when a CUDA device is present (the reference checks MPS, __init__.py:514-516)."""
     return torch.cuda.is_available()
 
 
-__all__ = ["deform_conv2d", "DeformConv2d", "ModulatedDeformConv2d", "is_available", "__version__",
+__all__ = ["deform_conv2d", "DeformConv2d", "ModulatedDeformConv2d", "gated_feed_forward", "GatedFeedForward2d",
+           "is_available", "__version__",
            "optim", "set_training_cache", "set_param_grad_hook", "set_head_fusion", "set_weight_image_cache"]

@@ -58,6 +58,20 @@ class DcnExOptions(ctypes.Structure):
                 ("flags", ctypes.c_int32)]
 
 
+DCN_ACT_SILU, DCN_ACT_GELU, DCN_ACT_RELU, DCN_ACT_SIGMOID = 0, 1, 2, 3
+
+
+class DcnFfnDesc(ctypes.Structure):
+    """Mirror of ``dcn_ffn_desc``."""
+    _fields_ = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("tokens", ctypes.c_int64),
+                ("channels", ctypes.c_int64), ("hidden", ctypes.c_int64)]
+
+
+class DcnFfnTensors(ctypes.Structure):
+    """Mirror of ``dcn_ffn_tensors`` and of ``dcn_ffn_grads``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")]
+
+
 class DcnAdamwTensor(ctypes.Structure):
     """Mirror of ``dcn_adamw_tensor``."""
     _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
@@ -118,6 +132,14 @@ SIGNATURES = {
     "dcn_deform_conv2d_forward_head": (ctypes.c_int, [_D, _V, _V, _V, _V, _V, _V, _SZ, _V, _SZ, _V]),
     "dcn_deform_conv2d_backward_head": (ctypes.c_int, [_D, _V, _V, _V, _V, _V, _SZ, _V, _V, _V, _V, _V, _SZ,
                                                        _V]),
+    "dcn_ffn_validate": (ctypes.c_int, [ctypes.POINTER(DcnFfnDesc)]),
+    "dcn_ffn_saved_bytes": (_SZ, [ctypes.POINTER(DcnFfnDesc)]),
+    "dcn_ffn_forward_workspace_size": (_SZ, [ctypes.POINTER(DcnFfnDesc), ctypes.c_int]),
+    "dcn_ffn_forward": (ctypes.c_int, [ctypes.POINTER(DcnFfnDesc), ctypes.POINTER(DcnFfnTensors), _V, _V, _SZ, _V,
+                                       _SZ, _V]),
+    "dcn_ffn_backward_workspace_size": (_SZ, [ctypes.POINTER(DcnFfnDesc)]),
+    "dcn_ffn_backward": (ctypes.c_int, [ctypes.POINTER(DcnFfnDesc), ctypes.POINTER(DcnFfnTensors), _V, _V, _SZ,
+                                        ctypes.POINTER(DcnFfnTensors), _V, _SZ, _V, PARAMS_READY_FN, _V]),
     "dcn_adamw_step": (ctypes.c_int, [ctypes.POINTER(DcnAdamwOptions), ctypes.POINTER(DcnAdamwTensor),
                                       ctypes.c_int64, _V]),
     "dcn_grad_norm_workspace_size": (_SZ, [ctypes.POINTER(DcnTensorRef), ctypes.c_int64]),

@@ -19,7 +19,7 @@ tensor, as in the reference (mps_deform_conv/__init__.py:224-225).
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -100,3 +100,56 @@ def traced_deform_conv2d(input: Tensor, offset: Tensor, weight: Tensor, bias, st
         input, weight, offset, mask if mask is not None else empty, bias if bias is not None else empty,
         stride[0], stride[1], padding[0], padding[1], dilation[0], dilation[1], n_weight_grps, n_offset_grps,
         mask is not None)
+
+
+# The gated feed-forward block, as the pair above: a forward that keeps nothing
+# and a backward that computes gate and up again.  An absent bias is None; its
+# gradient is an empty tensor.
+@torch.library.custom_op(f"{_NS}::gated_feed_forward", mutates_args=())
+def gated_feed_forward(input: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor],
+                       b_up: Optional[Tensor], b_down: Optional[Tensor], activation: int) -> Tensor:
+    from mps_deform_conv import _get_lib
+    return _get_lib().gated_feed_forward_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)[0]
+
+
+@gated_feed_forward.register_fake
+def _feed_forward_fake(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
+    return input.new_empty(input.shape)
+
+
+@torch.library.custom_op(f"{_NS}::gated_feed_forward_backward", mutates_args=())
+def gated_feed_forward_backward(
+        grad: Tensor, input: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor],
+        b_up: Optional[Tensor], b_down: Optional[Tensor],
+        activation: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    from mps_deform_conv import _get_lib
+    lib = _get_lib()
+    tensors = (input, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    _, saved = lib.gated_feed_forward_forward(*tensors, activation, True, False)
+    grads = lib.gated_feed_forward_backward(grad, *tensors, activation, saved, [True] * 7)
+    return tuple(input.new_empty((0,)) if g is None else g for g in grads)
+
+
+@gated_feed_forward_backward.register_fake
+def _feed_forward_backward_fake(grad, input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation):
+    return tuple(input.new_empty((0,) if t is None else t.shape)
+                 for t in (input, w_gate, w_up, w_down, b_gate, b_up, b_down))
+
+
+def _feed_forward_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:7])
+    ctx.activation = inputs[7]
+
+
+def _feed_forward_backward(ctx, grad):
+    tensors = ctx.saved_tensors
+    grads = torch.ops.mps_deform_conv.gated_feed_forward_backward(grad, *tensors, ctx.activation)
+    return tuple(None if t is None else g for t, g in zip(tensors, grads)) + (None,)
+
+
+gated_feed_forward.register_autograd(_feed_forward_backward, setup_context=_feed_forward_setup)
+
+
+def traced_gated_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation: int) -> Tensor:
+    """gated_feed_forward through the registered operator (arguments validated by the caller)."""
+    return torch.ops.mps_deform_conv.gated_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
