@@ -22,12 +22,15 @@
 // epilogue runs under the next tile's MMAs.  Epilogue warp w reads TMEM lanes
 // 32 (w % 4) .. +31: lane i owns one row, 32 columns at a time.
 //
-// Work is dealt in whole tiles (worker w takes tiles w, w + W, ...), or, when
-// there are too few tiles for the SMs, in equal runs of (tile, K block) units:
-// worker w takes units [w U / W, (w + 1) U / W).  A run then covers pieces of
-// tiles, each written as an fp32 partial in slot w + tile (unique, since along
-// the runs either w or the tile grows by one), and a second kernel adds a
-// tile's slots in worker order: the result does not depend on timing.
+// Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
+// last wave would leave many of the W workers idle, its R tiles are cut along
+// K instead (struct Cut): S = W / R workers a tile walk S equal slices of K,
+// tile by tile side by side, so that at any time all tiles read the same rows
+// of both operands and these come from the L2 (dealt tile after tile, a
+// product with a long K reads them from memory once per tile); the W - S R
+// workers left over share the end of K in equal runs.  Each piece is an fp32
+// partial in a slot of its own, and a second kernel adds a tile's slots in a
+// fixed order: the result does not depend on timing.
 //
 // Every mbarrier wait is bounded (dcn_sm100.cuh).
 #pragma once
@@ -86,7 +89,7 @@ struct GemmArgs {
   Seg seg[12];
   int tiles_m, tiles_n, batches;  // a batch adds its index to a_map (and picks the output)
   int group_m;               // tiles are dealt in blocks of group_m row tiles x all column tiles
-  int split;                 // 1: equal runs of units, partials to `partial`
+  int split;                 // 1: the last tiles are cut along K (Cut), partials to `partial`
   int act;
   uint32_t operand_bf16;
   float* partial;
@@ -413,39 +416,75 @@ __device__ __forceinline__ float column_sum32(float (&v)[32], int lane) {
 }
 
 // ---------------------------------------------------------------- work
+// How the last R tiles of a product are cut along their nkb K blocks among W
+// workers.  Worker s R + t, s < S: slice s of tile t, K blocks [s a, s a + a).
+// The E = W - S R others: equal runs of the units (tile, K block >= S a), tile
+// after tile.  Slots: the worker's index in the first case; S R + e + t in the
+// second (unique, since along the runs either e or t grows by one).
+struct Cut {
+  int R, S, E, a, nkb;
+  __host__ __device__ Cut(int R_, int W, int nkb_) : R(R_), nkb(nkb_) {
+    S = W / R;
+    E = W - S * R;
+    a = E ? (int)((int64_t)nkb * R / W) : (nkb + S - 1) / S;
+  }
+  __host__ __device__ int rest() const { return E ? nkb - S * a : 0; }  // K blocks of the runs
+  __host__ __device__ int slots() const { return S * R + (E ? E + R : 0); }
+};
+
 struct Work {
-  int64_t at, end, step;  // tiles, or units
-  int nkb;                // K blocks of a tile
-  int tile, kb0, kb1;
-  bool split;
-  __device__ __forceinline__ Work(const GemmArgs& a, int worker, int workers) {
-    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.batches;
-    nkb = a.nk * a.nseg;
-    split = a.split != 0;
-    if (split) {
-      const int64_t units = tiles * nkb;
-      at = units * worker / workers;
-      end = units * (worker + 1) / workers;
-    } else {
-      at = worker;
-      end = tiles;
-      step = workers;
+  int worker, workers, nkb;
+  int at, whole_end;            // whole tiles: at, at + workers, ... below whole_end
+  int base;                     // first of the cut tiles; -1: none
+  int64_t unit, unit_end;       // units still to do of a run
+  bool slice;                   // the slice is still to do
+  int tile, kb0, kb1, slot;     // the current piece; slot < 0: a whole tile
+  __device__ __forceinline__ Work(const GemmArgs& a, int worker_, int workers_)
+      : worker(worker_), workers(workers_), nkb(a.nk * a.nseg), at(worker_), base(-1), unit(0), unit_end(0), slice(false) {
+    const int tiles = a.tiles_m * a.tiles_n * a.batches;
+    whole_end = tiles;
+    if (a.split) {
+      base = whole_end = tiles / workers * workers;
+      const Cut c(tiles - base, workers, nkb);
+      slice = worker < c.S * c.R;
+      if (!slice) {
+        const int e = worker - c.S * c.R;
+        const int64_t units = (int64_t)c.R * c.rest();
+        unit = units * e / c.E;
+        unit_end = units * (e + 1) / c.E;
+      }
     }
   }
-  __device__ __forceinline__ bool next() {
-    if (at >= end) return false;
-    if (split) {
-      tile = (int)(at / nkb);
-      kb0 = (int)(at - (int64_t)tile * nkb);
-      const int64_t left = end - at;
-      kb1 = left < nkb - kb0 ? kb0 + (int)left : nkb;
-      at += kb1 - kb0;
-    } else {
-      tile = (int)at;
+  __device__ __forceinline__ bool next(const GemmArgs& a) {
+    if (at < whole_end) {
+      tile = at;
+      at += workers;
       kb0 = 0;
       kb1 = nkb;
-      at += step;
+      slot = -1;
+      return true;
     }
+    if (base < 0) return false;
+    const Cut c(a.tiles_m * a.tiles_n * a.batches - base, workers, nkb);
+    if (slice) {
+      slice = false;
+      const int s = worker / c.R;
+      tile = base + worker - s * c.R;
+      kb0 = s * c.a;
+      kb1 = min(nkb, kb0 + c.a);
+      slot = worker;
+      return kb0 < kb1;
+    }
+    if (unit >= unit_end) return false;
+    const int rest = c.rest();
+    const int t = (int)(unit / rest);
+    const int k = (int)(unit - (int64_t)t * rest);
+    const int len = (int)min((int64_t)(rest - k), unit_end - unit);
+    tile = base + t;
+    kb0 = c.S * c.a + k;
+    kb1 = kb0 + len;
+    slot = c.S * c.R + (worker - c.S * c.R) + t;
+    unit += len;
     return true;
   }
 };
@@ -530,7 +569,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     if (lane == 0) {
       int issued = 0;
       bool ok = true;
-      while (ok && w.next()) {
+      while (ok && w.next(a)) {
         int z, mt, nt;
         tile_at(a, w.tile, z, mt, nt);
         const int m0 = mt * BM, n0 = nt * COLS;
@@ -578,7 +617,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       const uint32_t idesc = tcc::idesc_f16_major(BM, BN, a.operand_bf16 != 0, A_MN, B_MN);
       int used = 0, done = 0;
       bool ok = true;
-      while (ok && w.next()) {
+      while (ok && w.next(a)) {
         for (int k0 = w.kb0; ok && k0 < w.kb1; k0 += RUN) {
           const int k1 = w.kb1 - k0 > RUN ? k0 + RUN : w.kb1;
           const int b = done & 1;
@@ -658,14 +697,14 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       if (lane == 0) mbar_arrive(acc_empty(done & 1));
       ++done;
     };
-    while (ok && w.next()) {
+    while (ok && w.next(a)) {
       int z, mt, nt;
       tile_at(a, w.tile, z, mt, nt);
       const int n0 = nt * COLS;
       const int row0 = mt * BM + q * 32;
       const int64_t row = (int64_t)row0 + lane;
       const bool row_in = row < a.M;
-      const bool whole = !w.split;
+      const bool whole = w.slot < 0;
       const int64_t m_block = (int64_t)mt * 4 + q;
       auto saved_block = [&](int c) {
         return static_cast<uint8_t*>(a.saved) + saved_block_offset<T>(m_block, (n0 + c * 32) / 32, col_blocks);
@@ -676,7 +715,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         const int c0 = n0 + c * 32;
         if (!whole) {
           // an fp32 partial of this tile, 16-byte pieces of 32 rows side by side
-          float* slot = a.partial + ((int64_t)blockIdx.x + w.tile) * (BM * BN) + q * (32 * BN);
+          float* slot = a.partial + (int64_t)w.slot * (BM * BN) + q * (32 * BN);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             *reinterpret_cast<float4*>(slot + c * 1024 + j * 128 + lane * 4) =

@@ -108,83 +108,118 @@ struct Packer {
 };
 
 // ---------------------------------------------------------------- split products
-// Adds the partials of each output tile in worker order (ffn_gemm_kernel's
-// slots) and stores T.  One warp per 32 x 32 block; reads are whole lines.
+// Adds the partials of each cut tile (struct Cut) and stores T.  One CTA per
+// 32 x 32 block: warp i adds slots i, i + 8, ... of the tile's list, then the
+// eight sums are added in order; reads are whole lines.
 struct ReduceArgs {
   const float* partial;
   void* out[2];
   const void* bias;
   int64_t ldo;
-  int M, N, tiles_m, tiles_n, batches, group_m, nkb, workers, vec;
+  int M, N, tiles_m, tiles_n, group_m, nkb, workers, base, tiles, vec;
 };
 
 template <typename T, int BN>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__ ReduceArgs a) {
+  __shared__ float4 part[8][8][32];
   constexpr int BLOCKS = BN / 32 * 4;  // 32 x 32 blocks of a tile
-  const int lane = threadIdx.x & 31;
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.batches;
-  const int64_t unit = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5));
-  if (unit >= tiles * BLOCKS) return;
-  const int tile = (int)(unit / BLOCKS), blk = (int)(unit - (int64_t)tile * BLOCKS);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = blockIdx.x / BLOCKS, blk = blockIdx.x - t * BLOCKS;
   const int q = blk & 3, c = blk >> 2;
   GemmArgs g;
   g.tiles_m = a.tiles_m; g.tiles_n = a.tiles_n; g.group_m = a.group_m;
   int z, mt, nt;
-  tile_at(g, tile, z, mt, nt);
+  tile_at(g, a.base + t, z, mt, nt);
   const int64_t row = (int64_t)mt * BM + q * 32 + lane;
   const int c0 = nt * BN + c * 32;
   if (mt * BM + q * 32 >= a.M || c0 >= a.N) return;
-  const int64_t units = tiles * a.nkb;
-  const int64_t first = ((int64_t)tile * a.nkb + 1) * a.workers, last = (int64_t)(tile + 1) * a.nkb * a.workers;
-  const int w0 = (int)((first - 1) / units), w1 = (int)((last - 1) / units);
-  float v[32];
+  const Cut cut(a.tiles, a.workers, a.nkb);
+  int e0 = 0, e1 = -1;  // the runs that touch this tile
+  if (cut.rest() > 0) {
+    const int64_t rest = cut.rest(), units = rest * cut.R;
+    e0 = (int)(((t * rest + 1) * cut.E - 1) / units);
+    e1 = (int)(((t + 1) * rest * cut.E - 1) / units);
+  }
+  float4 v[8];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-  for (int w = w0; w <= w1; ++w) {
-    const float* slot = a.partial + ((int64_t)w + tile) * (BM * BN) + q * (32 * BN) + c * 1024 + lane * 4;
+  for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int slices = min(cut.S, (a.nkb + cut.a - 1) / cut.a);
+  const int n = slices + (e1 - e0 + 1);
+  for (int i = warp; i < n; i += 8) {
+    const int slot = i < slices ? i * cut.R + t : cut.S * cut.R + e0 + (i - slices) + t;
+    const float4* p = reinterpret_cast<const float4*>(a.partial + (int64_t)slot * (BM * BN) + q * (32 * BN) + c * 1024) + lane;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float4 f = *reinterpret_cast<const float4*>(slot + j * 128);
-      v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+      const float4 f = p[j * 32];
+      v[j].x += f.x; v[j].y += f.y; v[j].z += f.z; v[j].w += f.w;
     }
   }
-  if (row >= a.M) return;
-  if (a.bias) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (c0 + j < a.N) v[j] += to_f<T>(static_cast<const T*>(a.bias)[c0 + j]);
+  for (int j = 0; j < 8; ++j) part[warp][j][lane] = v[j];
+  __syncthreads();
+  // warp j finishes columns 4 j .. 4 j + 3 of every row
+  const int n0 = c0 + 4 * warp;
+  if (row >= a.M || n0 >= a.N) return;
+  float4 s = part[0][warp][lane];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    const float4 f = part[w][warp][lane];
+    s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
   }
-  store_row32<T>(static_cast<T*>(a.out[z]) + row * a.ldo, c0, a.N, a.vec != 0, v);
+  const float r[4] = {s.x, s.y, s.z, s.w};
+  T* out = static_cast<T*>(a.out[z]) + row * a.ldo + n0;
+  T o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    o[k] = from_f<T>(r[k] + (a.bias && n0 + k < a.N ? to_f<T>(static_cast<const T*>(a.bias)[n0 + k]) : 0.0f));
+  if (a.vec && n0 + 4 <= a.N) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(o[0], o[1], o[2], o[3]);
+    else memcpy(__builtin_assume_aligned(out, 8), o, 8);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n0 + k < a.N) out[k] = o[k];
+  }
 }
 
 // ---------------------------------------------------------------- column sums
-// Column sums of dy [M][C] (grad of the down bias): CTA (x, y) sums columns
-// 32 VEC x .. of rows y, y + gridDim.y, ... per warp; partials [gridDim.y * 8][C].
+// Column sums of dy [M][C] (grad of the down bias): CTA (x, y) adds columns
+// 32 VEC x .. of rows y 8 + warp, + 8 gridDim.y, ...; partials [gridDim.y][C].
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) ffn_column_partial_kernel(const T* __restrict__ src, float* __restrict__ part,
                                                                  int64_t M, int C) {
-  const int lane = threadIdx.x & 31;
-  const int64_t slice = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5), slices = (int64_t)gridDim.y * 8;
+  __shared__ float s[8][VEC][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c0 = (blockIdx.x * 32 + lane) * VEC;
-  if (c0 >= C) return;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-#pragma unroll 4
-  for (int64_t r = slice; r < M; r += slices) {
-    const T* p = src + r * C + c0;
-    if constexpr (VEC == 1) {
-      acc[0] += to_f<T>(p[0]);
-    } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      T t[VEC];
-      memcpy(t, &w, 16);
+  if (c0 < C) {
+#pragma unroll 8
+    for (int64_t r = (int64_t)blockIdx.y * 8 + warp; r < M; r += (int64_t)gridDim.y * 8) {
+      const T* p = src + r * C + c0;
+      if constexpr (VEC == 1) {
+        acc[0] += to_f<T>(p[0]);
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        T t[VEC];
+        memcpy(t, &w, 16);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += to_f<T>(t[j]);
+        for (int j = 0; j < VEC; ++j) acc[j] += to_f<T>(t[j]);
+      }
     }
   }
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) part[slice * C + c0 + j] = acc[j];
+  for (int j = 0; j < VEC; ++j) s[warp][j][lane] = acc[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+    const int l = i / VEC, j = i - l * VEC, c = blockIdx.x * 32 * VEC + i;
+    if (c >= C) break;
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += s[w][j][l];
+    part[(int64_t)blockIdx.y * C + c] = t;
+  }
 }
 
 // out[k][c] = sum over the rows of part [rows][sets][N], in a fixed order.
@@ -196,7 +231,7 @@ __global__ void __launch_bounds__(1024) ffn_column_finish_kernel(const float* __
   const int c = blockIdx.x * 32 + lane, k = blockIdx.y;
   float acc = 0.0f;
   if (c < N) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t r = warp; r < rows; r += 32) acc += part[(r * sets + k) * N + c];
   }
   s[warp][lane] = acc;
@@ -291,11 +326,13 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   r.out[0] = a.out[0]; r.out[1] = a.out[1];
   r.bias = bias;
   r.ldo = ldo;
-  r.M = a.M; r.N = a.N; r.tiles_m = p.tiles_m; r.tiles_n = p.tiles_n; r.batches = batches; r.group_m = a.group_m;
+  r.M = a.M; r.N = a.N; r.tiles_m = p.tiles_m; r.tiles_n = p.tiles_n; r.group_m = a.group_m;
   r.nkb = a.nk * a.nseg; r.workers = p.workers; r.vec = a.vec;
-  const int64_t warps = (int64_t)p.tiles_m * p.tiles_n * batches * (p.bn / 32 * 4);
+  const int tiles = p.tiles_m * p.tiles_n * batches;
+  r.base = tiles / p.workers * p.workers;
+  r.tiles = tiles - r.base;
   KernelScope ks("ffn_reduce", st);
-  const unsigned grid = (unsigned)div_up(warps, 8);
+  const unsigned grid = (unsigned)(r.tiles * (p.bn / 32 * 4));
   if (p.bn == 256) ffn_reduce_kernel<T, 256><<<grid, 256, 0, st>>>(r);
   else if (p.bn == 128) ffn_reduce_kernel<T, 128><<<grid, 256, 0, st>>>(r);
   else ffn_reduce_kernel<T, 64><<<grid, 256, 0, st>>>(r);
@@ -405,7 +442,7 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
   if (e != cudaSuccess) return e;
   if (g.b_down) {
     constexpr int kVec = 16 / sizeof(T);
-    const int64_t rows = std::min<int64_t>(div_up(s.M, 8), kSumSlices);
+    const int64_t rows = std::min<int64_t>(div_up(s.M, 64), kSumSlices);
     {
       KernelScope ks("ffn_column_partial", st);
       if (s.C % kVec == 0)
@@ -418,7 +455,7 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
     }
     KernelScope ks("ffn_column_finish", st);
     ffn_column_finish_kernel<T><<<dim3((unsigned)div_up(s.C, 32), 1), 1024, 0, st>>>(
-        w.rowsum, static_cast<T*>(g.b_down), nullptr, rows * 8, 1, (int)s.C);
+        w.rowsum, static_cast<T*>(g.b_down), nullptr, rows, 1, (int)s.C);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (ready) ready(user);

@@ -137,7 +137,7 @@ struct ForwardWs {
   }
 };
 
-constexpr int kSumSlices = 64;  // CTA rows of the dy column sums
+constexpr int kSumSlices = 4 * kSms;  // at most so many rows of partials of the dy column sums
 
 struct BackwardWs {
   Operand x, dy, wg, wu, wd, dg, du;
@@ -162,7 +162,7 @@ struct BackwardWs {
                                   store_partial_bytes(s.M, s.C, s.F, 2 * s.pair, 1)});
     partial = static_cast<float*>(c.take(part));
     colsum = static_cast<float*>(c.take((size_t)div_up(s.M, BM) * 4 * 2 * (size_t)s.F * 4));
-    rowsum = static_cast<float*>(c.take((size_t)kSumSlices * 8 * (size_t)s.C * 4));
+    rowsum = static_cast<float*>(c.take((size_t)kSumSlices * (size_t)s.C * 4));
     total = c.at;
   }
 };
