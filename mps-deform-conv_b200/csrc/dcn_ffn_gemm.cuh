@@ -16,11 +16,15 @@
 // values a stage in either form, zero-filled past the tensors' ends, so no
 // size needs to be a multiple of anything.
 //
-// Warp roles (320 threads): warps 0-7 epilogue, warp 8 issues the MMAs, warp 9
-// the TMA loads.  A CTA works through its share of the output tiles; the
-// accumulator is double-buffered in TMEM (2 x BN columns), so a tile's
-// epilogue runs under the next tile's MMAs.  Epilogue warp w reads TMEM lanes
-// 32 (w % 4) .. +31: lane i owns one row, 32 columns at a time.
+// Warp roles (576 threads): warps 0-15 epilogue, warp 16 issues the MMAs, warp
+// 17 the TMA loads.  A CTA works through its share of the output tiles; the
+// accumulator is double-buffered in TMEM, so a tile's epilogue runs under the
+// next tile's MMAs.  Epilogue warp w reads TMEM lanes 32 (w % 4) .. +31: lane i
+// owns one row, 16 columns at a time, and takes blocks w / 4, w / 4 + 4, ... of
+// the tile.  Sixteen warps of 16-column blocks and not eight of 32: the blocks'
+// chains of loads, exponentials and stores leave two warps a scheduler idle
+// more than half of the time (issue active 41 % and 53 % in the two gated
+// epilogues of 23104 x 512 -> 2048 rows in bf16).
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along
@@ -51,19 +55,28 @@ using namespace sm100;
 
 constexpr int kActSilu = DCN_ACT_SILU, kActGelu = DCN_ACT_GELU, kActRelu = DCN_ACT_RELU, kActSigmoid = DCN_ACT_SIGMOID;
 
-constexpr int EPI_WARPS = 8;
-constexpr int MMA_WARP = 8, LOAD_WARP = 9;
-constexpr int NTHREADS = 320;
+constexpr int EPI_WARPS = 16;
+constexpr int MMA_WARP = EPI_WARPS, LOAD_WARP = EPI_WARPS + 1;
+constexpr int NTHREADS = (EPI_WARPS + 2) * 32;
+constexpr int CB = 16;           // columns of an epilogue block
 constexpr uint32_t A_STAGE = BM * 128;
 constexpr int ST_FFN_LOAD = 61, ST_FFN_MMA = 62, ST_FFN_EPI = 63, ST_FFN_DRAIN = 64, ST_FFN_SMEM = 65;
 
-__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
-__host__ __device__ constexpr uint32_t stage_bytes(int bn) { return A_STAGE + (uint32_t)bn * 128u; }
-// operand stages, then two staged output blocks and 64 bias values of each
+enum Epi { EPI_GATED, EPI_DGATE, EPI_RECOMPUTE, EPI_STORE };
+
+// Accumulator columns are BN; EPI_RECOMPUTE has 3 x 64 (gate, up, dhidden) and
+// two row operands (x, dy).
+constexpr int kRecomputeCols = 64, kRecomputeBn = 3 * kRecomputeCols;
+__host__ __device__ constexpr uint32_t stage_bytes(int bn) {
+  return (bn == kRecomputeBn ? 2 : 1) * A_STAGE + (uint32_t)bn * 128u;
+}
+__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 4 : bn == kRecomputeBn ? 3 : bn == 128 ? 6 : 8; }
+// operand stages, then two staged output blocks and 32 bias values of each
 // epilogue warp, then barriers
-constexpr uint32_t kStaging = EPI_WARPS * 2 * 32 * 64;
+constexpr uint32_t kStageBlock = 32 * CB * 2;
+constexpr uint32_t kStaging = EPI_WARPS * 2 * kStageBlock;
 __host__ __device__ constexpr uint32_t smem_bytes(int bn) {
-  return (uint32_t)stages(bn) * stage_bytes(bn) + kStaging + EPI_WARPS * 64 * 4u +
+  return (uint32_t)stages(bn) * stage_bytes(bn) + kStaging + EPI_WARPS * 32 * 4u +
          (2u * (uint32_t)stages(bn) + 5u) * 8u + 16u;
 }
 // dynamic shared memory starts on 1024 bytes when a kernel has no static one;
@@ -73,14 +86,12 @@ static_assert(smem_bytes(256) + kSmemSlack <= 232448, "shared memory of one CTA"
 // fp32 data: K blocks added up in TMEM before their sum moves on to registers
 constexpr int kWideRun = 4;
 
-enum Epi { EPI_GATED, EPI_DGATE, EPI_STORE };
-
 struct Seg {
   uint8_t a_map, a_plane, b_map, b_plane;
 };
 struct Maps {
-  CUtensorMap m[4];
-  CUtensorMap out[2];  // 16-bit results, 32 x 32 blocks
+  CUtensorMap m[5];
+  CUtensorMap out[2];  // 16-bit results, 32 x 16 blocks
 };
 
 struct GemmArgs {
@@ -98,59 +109,40 @@ struct GemmArgs {
   int64_t ldo;
   int64_t plane;             // fp32: elements between the bf16 planes of hidden / dgate / dup
   int vec;                   // out rows take 16-byte stores (16-bit data: TMA stores)
-  const void* bias[2];       // STORE: [0]; GATED: gate, up
-  // saved gate and up (private layout, below), and the hidden values' other copy
-  void* saved;
+  const void* bias[2];       // STORE: [0]; GATED, RECOMPUTE: gate, up
+  void* saved;               // gate and up (private layout, below), or null
   float* colsum;             // DGATE: [32-row block][2][F] column sums of dgate and dup, or null
   int* status;
 };
 
 // ---------------------------------------------------------------- saved gate / up
-// What the backward needs of a 32-row x 32-column block (its rows being the
+// What the backward needs of a 32-row x 16-column block (its rows being the
 // lanes of one warp) lies together, each 16-byte piece of the 32 lanes side by
 // side, so both passes move whole lines:
-//   16-bit data: gate, up as fp16 times a power of two per (row, 32 columns)
+//   16-bit data: gate, up as fp16 times a power of two per (row, 16 columns)
 //     that puts the row's largest value near fp16's upper end: 11 bits, not
 //     bf16's 8, of values that the derivative multiplies, at the same size;
 //     then one int16 per lane with the two exponents;
 //   fp32 data: gate, up as fp32.
 template <typename T>
-struct SavedBlock {
-  static constexpr bool kWide = sizeof(T) == 4;
-  static constexpr size_t kGate = kWide ? 4096 : 2048;                     // bytes of one of the two
-  static constexpr size_t kBytes = saved_block_bytes(kWide);
-};
-template <typename T>
 __host__ __device__ inline size_t saved_block_offset(int64_t m_block, int64_t col_block, int64_t col_blocks) {
-  return (size_t)(m_block * col_blocks + col_block) * SavedBlock<T>::kBytes;
+  return (size_t)(m_block * col_blocks + col_block) * saved_block_bytes(sizeof(T) == 4);
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[CB]) {
+  uint32_t r[CB];
+  tmem_ld16(taddr, r);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < CB; ++i) v[i] = __uint_as_float(r[i]);
 }
-
 // Waits for this warp's TMEM loads; the values pass through, so that nothing
 // that uses them is scheduled before the wait.
-__device__ __forceinline__ void tmem_ld32_wait(float (&v)[32]) {
+__device__ __forceinline__ void tmem_wait(float (&v)[CB]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
-      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-      "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
-      "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
-      "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
-      "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
-      :
-      : "memory");
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -193,35 +185,35 @@ __device__ __forceinline__ float2 act_both(float x) {
     return make_float2(s, s * (1.0f - s));
   }
 }
-// A row's 32 columns at a time; the activation is picked once for all of them.
+// A row's block at a time; the activation is picked once for all of it.
 template <bool ACCURATE, int ACT>
-__device__ __forceinline__ void gate32(const float (&g)[32], const float (&u)[32], float (&h)[32]) {
+__device__ __forceinline__ void gate_block(const float (&g)[CB], const float (&u)[CB], float (&h)[CB]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) h[j] = act_value<ACCURATE, ACT>(g[j]) * u[j];
+  for (int j = 0; j < CB; ++j) h[j] = act_value<ACCURATE, ACT>(g[j]) * u[j];
 }
 // (gate, up) to (dgate, dup)
 template <bool ACCURATE, int ACT>
-__device__ __forceinline__ void dgate32(const float (&dh)[32], float (&g)[32], float (&u)[32]) {
+__device__ __forceinline__ void dgate_block(const float (&dh)[CB], float (&g)[CB], float (&u)[CB]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
+  for (int j = 0; j < CB; ++j) {
     const float2 s = act_both<ACCURATE, ACT>(g[j]);
     g[j] = dh[j] * u[j] * s.y;
     u[j] = dh[j] * s.x;
   }
 }
 template <bool ACCURATE>
-__device__ __forceinline__ void gate32(int act, const float (&g)[32], const float (&u)[32], float (&h)[32]) {
-  if (act == kActSilu) gate32<ACCURATE, kActSilu>(g, u, h);
-  else if (act == kActGelu) gate32<ACCURATE, kActGelu>(g, u, h);
-  else if (act == kActRelu) gate32<ACCURATE, kActRelu>(g, u, h);
-  else gate32<ACCURATE, kActSigmoid>(g, u, h);
+__device__ __forceinline__ void gate_block(int act, const float (&g)[CB], const float (&u)[CB], float (&h)[CB]) {
+  if (act == kActSilu) gate_block<ACCURATE, kActSilu>(g, u, h);
+  else if (act == kActGelu) gate_block<ACCURATE, kActGelu>(g, u, h);
+  else if (act == kActRelu) gate_block<ACCURATE, kActRelu>(g, u, h);
+  else gate_block<ACCURATE, kActSigmoid>(g, u, h);
 }
 template <bool ACCURATE>
-__device__ __forceinline__ void dgate32(int act, const float (&dh)[32], float (&g)[32], float (&u)[32]) {
-  if (act == kActSilu) dgate32<ACCURATE, kActSilu>(dh, g, u);
-  else if (act == kActGelu) dgate32<ACCURATE, kActGelu>(dh, g, u);
-  else if (act == kActRelu) dgate32<ACCURATE, kActRelu>(dh, g, u);
-  else dgate32<ACCURATE, kActSigmoid>(dh, g, u);
+__device__ __forceinline__ void dgate_block(int act, const float (&dh)[CB], float (&g)[CB], float (&u)[CB]) {
+  if (act == kActSilu) dgate_block<ACCURATE, kActSilu>(dh, g, u);
+  else if (act == kActGelu) dgate_block<ACCURATE, kActGelu>(dh, g, u);
+  else if (act == kActRelu) dgate_block<ACCURATE, kActRelu>(dh, g, u);
+  else dgate_block<ACCURATE, kActSigmoid>(dh, g, u);
 }
 
 // ---------------------------------------------------------------- stores
@@ -233,53 +225,49 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-
-// 32 columns of one row of a row-major matrix of T with `n` columns.
+// values 8 j .. 8 j + 7 of a block, times s, as 16-bit
 template <typename T>
-__device__ __forceinline__ void store_row32(T* row, int c0, int n, bool vec, const float (&v)[32]) {
+__device__ __forceinline__ uint4 pack8(const float (&v)[CB], int j, float s) {
+  uint4 p;
+  p.x = pack2(v[8 * j] * s, v[8 * j + 1] * s, (T*)nullptr);
+  p.y = pack2(v[8 * j + 2] * s, v[8 * j + 3] * s, (T*)nullptr);
+  p.z = pack2(v[8 * j + 4] * s, v[8 * j + 5] * s, (T*)nullptr);
+  p.w = pack2(v[8 * j + 6] * s, v[8 * j + 7] * s, (T*)nullptr);
+  return p;
+}
+
+// A block's columns of one row of a row-major matrix of T with `n` columns.
+template <typename T>
+__device__ __forceinline__ void store_row(T* row, int c0, int n, bool vec, const float (&v)[CB]) {
   if (vec) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < CB / 4; ++j)
         if (c0 + 4 * j < n)
           *reinterpret_cast<float4*>(row + c0 + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c0 + 8 * j < n) {
-          uint4 p;
-          p.x = pack2(v[8 * j], v[8 * j + 1], (T*)nullptr);
-          p.y = pack2(v[8 * j + 2], v[8 * j + 3], (T*)nullptr);
-          p.z = pack2(v[8 * j + 4], v[8 * j + 5], (T*)nullptr);
-          p.w = pack2(v[8 * j + 6], v[8 * j + 7], (T*)nullptr);
-          *reinterpret_cast<uint4*>(row + c0 + 8 * j) = p;
-        }
+      for (int j = 0; j < CB / 8; ++j)
+        if (c0 + 8 * j < n) *reinterpret_cast<uint4*>(row + c0 + 8 * j) = pack8<T>(v, j, 1.0f);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < CB; ++j)
       if (c0 + j < n) row[c0 + j] = from_f<T>(v[j]);
   }
 }
 
-// A 32 x 32 block of 16-bit values leaves through shared memory and one TMA
-// store per warp, whole 64-byte row pieces at a time (row-owning lanes would
-// write 16 bytes to 32 different lines an instruction).  Staged rows are 64
-// bytes with the 64-byte swizzle: 16-byte piece j of row r at j ^ (r / 2 % 4),
+// A 32 x 16 block of 16-bit values leaves through shared memory and one TMA
+// store per warp, whole 32-byte sectors at a time (row-owning lanes would
+// write 16 bytes to 32 different lines an instruction).  Staged rows are 32
+// bytes with the 32-byte swizzle: 16-byte piece j of row r at j ^ (r / 4 % 2),
 // so eight lanes cover all banks.  Rows and columns past the matrix are
 // dropped by the store.
-constexpr uint32_t kStageBlock = 32 * 64;
+__device__ __forceinline__ uint32_t staged_piece(int row, int j) { return row * 32 + ((j ^ ((row >> 2) & 1)) << 4); }
 template <typename T>
-__device__ __forceinline__ void stage_row32(uint8_t* block, int lane, const float (&v)[32]) {
+__device__ __forceinline__ void stage_row(uint8_t* block, int lane, const float (&v)[CB]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 p;
-    p.x = pack2(v[8 * j], v[8 * j + 1], (T*)nullptr);
-    p.y = pack2(v[8 * j + 2], v[8 * j + 3], (T*)nullptr);
-    p.z = pack2(v[8 * j + 4], v[8 * j + 5], (T*)nullptr);
-    p.w = pack2(v[8 * j + 6], v[8 * j + 7], (T*)nullptr);
-    *reinterpret_cast<uint4*>(block + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = p;
-  }
+  for (int j = 0; j < CB / 8; ++j) *reinterpret_cast<uint4*>(block + staged_piece(lane, j)) = pack8<T>(v, j, 1.0f);
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
@@ -288,40 +276,35 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
                : "memory");
 }
 
-// 32 columns of one row of an operand of a following product: T itself, or
-// for fp32 data three bf16 planes.  Rows are padded to 16 bytes (`ld`).
-template <typename T>
-__device__ __forceinline__ void store_operand32(void* base, int64_t plane, int64_t row, int64_t ld, int c0,
-                                                const float (&v)[32]) {
-  if constexpr (sizeof(T) == 4) {
-    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + row * ld;
-    float r[32];
+// A block's columns of one row of fp32 values that are an operand of a
+// following product: three bf16 planes.  Rows are padded to 16 bytes (`ld`).
+__device__ __forceinline__ void store_planes(void* base, int64_t plane, int64_t row, int64_t ld, int c0,
+                                             const float (&v)[CB]) {
+  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + row * ld;
+  float r[CB];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = v[j];
+  for (int j = 0; j < CB; ++j) r[j] = v[j];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      store_row32<__nv_bfloat16>(p + k * plane, c0, (int)ld, true, r);
-      // a plane that holds inf or NaN ends the expansion: the others are zero
+  for (int k = 0; k < 3; ++k) {
+    store_row<__nv_bfloat16>(p + k * plane, c0, (int)ld, true, r);
+    // a plane that holds inf or NaN ends the expansion: the others are zero
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float hi = __bfloat162float(__float2bfloat16_rn(r[j]));
-        r[j] = fabsf(hi) <= 3.4e38f ? r[j] - hi : 0.0f;
-      }
+    for (int j = 0; j < CB; ++j) {
+      const float hi = __bfloat162float(__float2bfloat16_rn(r[j]));
+      r[j] = fabsf(hi) <= 3.4e38f ? r[j] - hi : 0.0f;
     }
-  } else {
-    store_row32<T>(static_cast<T*>(base) + row * ld, c0, (int)ld, true, v);
   }
 }
 
 // ---------------------------------------------------------------- saved values
-__device__ __forceinline__ int scale_exponent(const float (&v)[32]) {
+__device__ __forceinline__ int scale_exponent(const float (&v)[CB]) {
   float top = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) top = fmaxf(top, fabsf(v[j]));
+  for (int j = 0; j < CB; ++j) top = fmaxf(top, fabsf(v[j]));
   if (!(top <= 3.4028235e38f)) {  // inf beside finite values: the scale is theirs
     top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < CB; ++j)
       if (fabsf(v[j]) <= 3.4028235e38f) top = fmaxf(top, fabsf(v[j]));
   }
   // values below 2^(e + 1) times 2^(14 - e) stay below 2^15, inside fp16's range
@@ -330,38 +313,29 @@ __device__ __forceinline__ int scale_exponent(const float (&v)[32]) {
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
 
 template <typename T>
-__device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, const float (&g)[32], const float (&u)[32]) {
+__device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, const float (&g)[CB], const float (&u)[CB]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 4; ++j) {
       *reinterpret_cast<float4*>(block + j * 512 + lane * 16) = make_float4(g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
-      *reinterpret_cast<float4*>(block + 4096 + j * 512 + lane * 16) =
+      *reinterpret_cast<float4*>(block + 2048 + j * 512 + lane * 16) =
           make_float4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
     }
   } else {
     const int eg = scale_exponent(g), eu = scale_exponent(u);
     const float sg = exp2_int(14 - eg), su = exp2_int(14 - eu);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint4 a, b;
-      a.x = pack2(g[8 * j] * sg, g[8 * j + 1] * sg, (__half*)nullptr);
-      a.y = pack2(g[8 * j + 2] * sg, g[8 * j + 3] * sg, (__half*)nullptr);
-      a.z = pack2(g[8 * j + 4] * sg, g[8 * j + 5] * sg, (__half*)nullptr);
-      a.w = pack2(g[8 * j + 6] * sg, g[8 * j + 7] * sg, (__half*)nullptr);
-      b.x = pack2(u[8 * j] * su, u[8 * j + 1] * su, (__half*)nullptr);
-      b.y = pack2(u[8 * j + 2] * su, u[8 * j + 3] * su, (__half*)nullptr);
-      b.z = pack2(u[8 * j + 4] * su, u[8 * j + 5] * su, (__half*)nullptr);
-      b.w = pack2(u[8 * j + 6] * su, u[8 * j + 7] * su, (__half*)nullptr);
-      *reinterpret_cast<uint4*>(block + j * 512 + lane * 16) = a;
-      *reinterpret_cast<uint4*>(block + 2048 + j * 512 + lane * 16) = b;
+    for (int j = 0; j < 2; ++j) {
+      *reinterpret_cast<uint4*>(block + j * 512 + lane * 16) = pack8<__half>(g, j, sg);
+      *reinterpret_cast<uint4*>(block + 1024 + j * 512 + lane * 16) = pack8<__half>(u, j, su);
     }
-    reinterpret_cast<uint16_t*>(block + 4096)[lane] = (uint16_t)((eg & 0xff) | (eu & 0xff) << 8);
+    reinterpret_cast<uint16_t*>(block + 2048)[lane] = (uint16_t)((eg & 0xff) | (eu & 0xff) << 8);
   }
 }
 // A lane's share of a saved block, fetched ahead of its use and then decoded.
 template <typename T>
 struct SavedRaw {
-  static constexpr int kPieces = sizeof(T) == 4 ? 8 : 4;
+  static constexpr int kPieces = sizeof(T) == 4 ? 4 : 2;
   uint4 a[kPieces], b[kPieces];
   uint16_t e;
   __device__ __forceinline__ void load(const uint8_t* block, int lane) {
@@ -370,12 +344,12 @@ struct SavedRaw {
       a[j] = *reinterpret_cast<const uint4*>(block + j * 512 + lane * 16);
       b[j] = *reinterpret_cast<const uint4*>(block + kPieces * 512 + j * 512 + lane * 16);
     }
-    e = sizeof(T) == 4 ? 0 : reinterpret_cast<const uint16_t*>(block + 4096)[lane];
+    e = sizeof(T) == 4 ? 0 : reinterpret_cast<const uint16_t*>(block + 2048)[lane];
   }
-  __device__ __forceinline__ void decode(float (&g)[32], float (&u)[32]) const {
+  __device__ __forceinline__ void decode(float (&g)[CB], float (&u)[CB]) const {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         g[4 * j] = __uint_as_float(a[j].x); g[4 * j + 1] = __uint_as_float(a[j].y);
         g[4 * j + 2] = __uint_as_float(a[j].z); g[4 * j + 3] = __uint_as_float(a[j].w);
         u[4 * j] = __uint_as_float(b[j].x); u[4 * j + 1] = __uint_as_float(b[j].y);
@@ -385,7 +359,7 @@ struct SavedRaw {
       // the exponents as signed bytes; -100 and up, so 2^(e - 14) is a normal number
       const float sg = exp2_int((int)(int8_t)(e & 0xff) - 14), su = exp2_int((int)(int8_t)(e >> 8) - 14);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         const uint32_t aw[4] = {a[j].x, a[j].y, a[j].z, a[j].w}, bw[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -399,11 +373,48 @@ struct SavedRaw {
   }
 };
 
-// Lane l returns the sum over the warp's lanes of v[l]: 31 shuffles, in an
-// order fixed by the lanes.
-__device__ __forceinline__ float column_sum32(float (&v)[32], int lane) {
+// ---------------------------------------------------------------- column sums of a block
+// 16-bit: of the staged (rounded) values, by the legacy matrix instruction with
+// a row operand of ones: two ldmatrix and four mma.sync a block, where a sum
+// across lanes takes some 120 instructions (a quarter of the whole epilogue).
+// Stores the sums of columns c0 .. c0 + 15 below n.
+template <typename T>
+__device__ __forceinline__ void staged_column_sums(uint32_t block, int lane, float* out, int c0, int n) {
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  const uint32_t one = BF ? 0x3f803f80u : 0x3c003c00u;
 #pragma unroll
-  for (int half = 16; half; half >>= 1) {
+  for (int j = 0; j < 2; ++j) {
+    uint32_t r[4];  // rows 8 i .. 8 i + 7 of eight columns, transposed: pairs of rows a lane
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(block + staged_piece(lane, j))
+                 : "memory");
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if constexpr (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(one), "r"(r[2 * s]), "r"(r[2 * s + 1]));
+      else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(one), "r"(r[2 * s]), "r"(r[2 * s + 1]));
+    }
+    const int c = c0 + 8 * j + 2 * lane;  // every row of the result is the sums; lanes 0-3 hold row 0
+    if (lane < 4) {
+      if (c < n) out[c] = d[0];
+      if (c + 1 < n) out[c + 1] = d[1];
+    }
+  }
+}
+// fp32: lanes 0-15 return the sums of columns 0-15 over the warp's lanes, in an
+// order fixed by the lanes.
+__device__ __forceinline__ float column_sum(float (&v)[CB], int lane) {
+#pragma unroll
+  for (int j = 0; j < CB; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], 16);
+#pragma unroll
+  for (int half = 8; half; half >>= 1) {
     const bool up = (lane & half) != 0;
 #pragma unroll
     for (int j = 0; j < half; ++j) {
@@ -509,8 +520,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs a) {
   constexpr int S = stages(BN);
   constexpr uint32_t STAGE = stage_bytes(BN);
-  constexpr bool GATED = EPI == EPI_GATED;
-  constexpr int COLS = GATED ? BN / 2 : BN;  // output columns of a tile
+  constexpr bool GATED = EPI == EPI_GATED, RECOMP = EPI == EPI_RECOMPUTE, TWO = GATED || RECOMP;
+  constexpr bool DGATE = EPI == EPI_DGATE || RECOMP;
+  constexpr int COLS = GATED ? BN / 2 : RECOMP ? BN / 3 : BN;  // output columns of a tile
+  constexpr int ACC = RECOMP ? 256 : BN;                       // TMEM columns of an accumulator buffer
+  constexpr uint32_t B_AT = (RECOMP ? 2 : 1) * A_STAGE;        // column operands in a stage
   constexpr bool WIDE = sizeof(T) == 4;
   // K blocks of one accumulation in TMEM.  The tensor cores truncate each
   // addition to the accumulator, an error that grows with the number of steps
@@ -518,12 +532,13 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   // sums rounded to nearest leave 6e-7); fp32 data therefore moves its sums to
   // registers every kWideRun blocks.  16-bit results do not see the difference.
   constexpr int RUN = WIDE ? kWideRun : 1 << 30;
-  static_assert(!WIDE || BN <= 128, "an epilogue thread holds BN / 2 sums");
+  static_assert(!WIDE || BN <= 128 || RECOMP, "an epilogue thread holds 32 to 48 sums");
+  static_assert(RECOMP == (BN == kRecomputeBn), "accumulator columns");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
   uint8_t* staging = smem + S * STAGE;
-  uint8_t* tail = staging + kStaging + EPI_WARPS * 64 * 4;
+  uint8_t* tail = staging + kStaging + EPI_WARPS * 32 * 4;
   if (smem + smem_bytes(BN) > smem_raw + smem_bytes(BN) + kSmemSlack) {  // an unexpected start: nothing is touched
     if (threadIdx.x == 0) atomicExch(a.status, ST_FFN_SMEM);
     return;
@@ -538,7 +553,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + (2 * S + 5) * 8 + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  constexpr uint32_t TMEM_COLS = 2 * ACC;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -590,9 +605,13 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           } else {
             tma_load_3d(dst, ma, k, m0, seg.a_plane, full(s));
           }
-          if (GATED) {
-            tma_load_3d(dst + A_STAGE, mb, k, n0, seg.b_plane, full(s));
-            tma_load_3d(dst + A_STAGE + COLS * 128, mb + 1, k, n0, seg.b_plane, full(s));
+          if (TWO) {
+            tma_load_3d(dst + B_AT, mb, k, n0, seg.b_plane, full(s));
+            tma_load_3d(dst + B_AT + COLS * 128, mb + 1, k, n0, seg.b_plane, full(s));
+            if (RECOMP) {  // dy beside x, w_down (MN-major) beside the other two
+              tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, full(s));
+              tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, full(s));
+            }
           } else if (B_MN) {
 #pragma unroll
             for (int q = 0; q < BN / 64; ++q)
@@ -614,7 +633,8 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------ MMA issuer
     if (lane == 0) {
-      const uint32_t idesc = tcc::idesc_f16_major(BM, BN, a.operand_bf16 != 0, A_MN, B_MN);
+      const uint32_t idesc = tcc::idesc_f16_major(BM, TWO ? 2 * COLS : BN, a.operand_bf16 != 0, A_MN, B_MN);
+      const uint32_t idesc_dh = tcc::idesc_f16_major(BM, COLS, a.operand_bf16 != 0, false, true);
       int used = 0, done = 0;
       bool ok = true;
       while (ok && w.next(a)) {
@@ -624,18 +644,22 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           ok = mbar_wait(acc_empty(b), ((done >> 1) & 1) ^ 1, abort_flag, a.status, ST_FFN_MMA);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(b * BN);
+          const uint32_t d = tmem + (uint32_t)(b * ACC);
           for (int i = k0; i < k1; ++i) {
             const int s = used % S;
             ok = mbar_wait(full(s), (used / S) & 1, abort_flag, a.status, ST_FFN_MMA);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t ab = sbase + s * STAGE, bb = ab + A_STAGE;
+            const uint32_t ab = sbase + s * STAGE, bb = ab + B_AT;
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
               const uint64_t ad = A_MN ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192) : desc_kmajor_sw128(ab + kk * 32);
               const uint64_t bd = B_MN ? tcc::desc_mnmajor_sw128(bb + kk * 2048, 8192) : desc_kmajor_sw128(bb + kk * 32);
               mma_f16(d, ad, bd, idesc, (i > k0 || kk > 0) ? 1u : 0u);
+              if (RECOMP)
+                mma_f16(d + 2 * COLS, desc_kmajor_sw128(ab + A_STAGE + kk * 32),
+                        tcc::desc_mnmajor_sw128(bb + 2 * COLS * 128 + kk * 2048, 8192), idesc_dh,
+                        (i > k0 || kk > 0) ? 1u : 0u);
             }
             mma_commit(empty(s));
             ++used;
@@ -653,34 +677,36 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     }
   } else {
     // ------------------------------------------------ epilogue
-    const int q = warp & 3, half = warp >> 2;
-    // the bias values of a 32-column block, one column a lane, read back by all
-    // lanes; each warp has its own, so the epilogue warps never meet at a barrier
-    float* colf = reinterpret_cast<float*>(staging + kStaging) + warp * 64;
-    auto bias32 = [&](int c0) {
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k < (GATED ? 2 : 1); ++k)
-        colf[k * 32 + lane] = c0 + lane < a.N ? to_f<T>(static_cast<const T*>(a.bias[k])[c0 + lane]) : 0.0f;
-      __syncwarp();
-    };
+    const int q = warp & 3, first = warp >> 2;  // lanes 32 q .., column blocks first, first + 4, ...
+    constexpr int BLOCKS = COLS / CB;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     uint8_t* stage = staging + warp * (2 * kStageBlock);
+    float* colf = reinterpret_cast<float*>(staging + kStaging) + warp * 32;
     const bool has_bias = EPI != EPI_DGATE && a.bias[0] != nullptr;
-    const int64_t col_blocks = (a.N + 31) / 32;
+    const int64_t col_blocks = (a.N + CB - 1) / CB;
+    // The bias values of a block, one a lane (RECOMPUTE, GATED: 16 of gate, 16
+    // of up), fetched ahead and read back by all lanes through the warp's own
+    // piece of shared memory.
+    auto bias_of = [&](int c0) {
+      const int k = lane >> 4, c = c0 + (lane & 15);
+      return (k == 0 || TWO) && c < a.N ? to_f<T>(static_cast<const T*>(a.bias[k])[c]) : 0.0f;
+    };
     // this warp's staged blocks, out through the TMA
-    auto store_staged = [&](int blocks, int x, int y, int first) {
-      fence_async_shared();
-      __syncwarp();
+    auto store_staged = [&](int blocks, int x, int y, int map) {
       if (lane == 0 && y < a.M) {
         for (int k = 0; k < blocks; ++k)
-          tma_store_3d(&maps.out[first + k], smem_addr(stage + k * kStageBlock), x, y, 0);
+          tma_store_3d(&maps.out[map + k], smem_addr(stage + k * kStageBlock), x, y, 0);
         bulk_commit();
       }
     };
     // staged blocks may be written again once the store has read them
     auto staging_free = [&] {
       if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+    };
+    // this lane's writes to the staged blocks reach the TMA and the other lanes
+    auto staging_done = [&] {
+      fence_async_shared();
       __syncwarp();
     };
     int done = 0;
@@ -707,111 +733,132 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       const bool whole = w.slot < 0;
       const int64_t m_block = (int64_t)mt * 4 + q;
       auto saved_block = [&](int c) {
-        return static_cast<uint8_t*>(a.saved) + saved_block_offset<T>(m_block, (n0 + c * 32) / 32, col_blocks);
+        return static_cast<uint8_t*>(a.saved) + saved_block_offset<T>(m_block, n0 / CB + c, col_blocks);
       };
 
-      // one 32-column block of this tile; v, u: the sums of its columns (GATED: gate and up)
-      auto block = [&](int c, float (&v)[32], float (&u)[32], const SavedRaw<T>& raw) {
-        const int c0 = n0 + c * 32;
+      // One block of this tile.  v: its sums (GATED, RECOMPUTE: gate); u: up (from
+      // TMEM or, DGATE, the saved state with gate in v's place); dh: dhidden.
+      auto block = [&](int c, float (&v)[CB], float (&u)[CB], float (&dh)[CB], float bias) {
+        const int c0 = n0 + c * CB;
         if (!whole) {
           // an fp32 partial of this tile, 16-byte pieces of 32 rows side by side
           float* slot = a.partial + (int64_t)w.slot * (BM * BN) + q * (32 * BN);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(slot + c * 1024 + j * 128 + lane * 4) =
+          for (int j = 0; j < CB / 4; ++j)
+            *reinterpret_cast<float4*>(slot + c * 512 + j * 128 + lane * 4) =
                 make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           return;
         }
         if (c0 >= a.N) return;
         if (has_bias) {
-          bias32(c0);
+          __syncwarp();
+          colf[lane] = bias;
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < CB; ++j) {
             v[j] += colf[j];
-            if (GATED) u[j] += colf[32 + j];
+            if (TWO) u[j] += colf[CB + j];
           }
         }
-        if constexpr (EPI == EPI_GATED) {
+        if constexpr (GATED) {
           if (a.saved) save_gate_up<T>(saved_block(c), lane, v, u);
-          float h[32];
-          gate32<WIDE>(a.act, v, u, h);
+          float h[CB];
+          gate_block<WIDE>(a.act, v, u, h);
           if constexpr (WIDE) {
-            if (row_in) store_operand32<T>(a.out[0], a.plane, row, a.ldo, c0, h);
+            if (row_in) store_planes(a.out[0], a.plane, row, a.ldo, c0, h);
           } else {
             staging_free();
-            stage_row32<T>(stage, lane, h);
+            stage_row<T>(stage, lane, h);
+            staging_done();
             store_staged(1, c0, row0, 0);
           }
-        } else if constexpr (EPI == EPI_DGATE) {
-          // rows past M: their saved values are those of zero rows, and dh is 0
-          float g[32], d[32];
-          raw.decode(g, d);
-          dgate32<WIDE>(a.act, v, g, d);
+        } else if constexpr (DGATE) {
+          dgate_block<WIDE>(a.act, dh, v, u);
+          if (!row_in) {  // rows past M count in no column sum
+#pragma unroll
+            for (int j = 0; j < CB; ++j) v[j] = u[j] = 0.0f;
+          }
+          float* sums = a.colsum ? a.colsum + (m_block * 2) * a.N : nullptr;
           if constexpr (WIDE) {
             if (row_in) {
-              store_operand32<T>(a.out[0], a.plane, row, a.ldo, c0, g);
-              store_operand32<T>(a.out[1], a.plane, row, a.ldo, c0, d);
+              store_planes(a.out[0], a.plane, row, a.ldo, c0, v);
+              store_planes(a.out[1], a.plane, row, a.ldo, c0, u);
+            }
+            if (sums) {
+              const float sg = column_sum(v, lane), su = column_sum(u, lane);
+              if (lane < CB && c0 + lane < a.N) {
+                sums[c0 + lane] = sg;
+                sums[a.N + c0 + lane] = su;
+              }
             }
           } else {
             staging_free();
-            stage_row32<T>(stage, lane, g);
-            stage_row32<T>(stage + kStageBlock, lane, d);
+            stage_row<T>(stage, lane, v);
+            stage_row<T>(stage + kStageBlock, lane, u);
+            staging_done();
             store_staged(2, c0, row0, 0);
-          }
-          if (a.colsum) {
-            if (!row_in) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) g[j] = d[j] = 0.0f;
-            }
-            const float sg = column_sum32(g, lane), su = column_sum32(d, lane);
-            if (c0 + lane < a.N) {
-              float* out = a.colsum + (m_block * 2) * a.N + c0 + lane;
-              out[0] = sg;
-              out[a.N] = su;
+            if (sums) {
+              staged_column_sums<T>(smem_addr(stage), lane, sums, c0, a.N);
+              staged_column_sums<T>(smem_addr(stage + kStageBlock), lane, sums + a.N, c0, a.N);
+              __syncwarp();
             }
           }
         } else {
           if (!WIDE && a.vec) {
             if constexpr (!WIDE) {
               staging_free();
-              stage_row32<T>(stage, lane, v);
+              stage_row<T>(stage, lane, v);
+              staging_done();
               store_staged(1, c0, row0, z);
             }
           } else if (row_in) {
-            store_row32<T>(static_cast<T*>(a.out[z]) + row * a.ldo, c0, a.N, a.vec != 0, v);
+            store_row<T>(static_cast<T*>(a.out[z]) + row * a.ldo, c0, a.N, a.vec != 0, v);
           }
         }
       };
 
+      // what the first block needs from memory is fetched while the products
+      // run, the next ones' a block ahead
+      const bool use_bias = has_bias && whole;
+      float bias = use_bias ? bias_of(n0 + first * CB) : 0.0f;
       SavedRaw<T> raw;
+      if (EPI == EPI_DGATE && first < BLOCKS && n0 + first * CB < a.N) raw.load(saved_block(first), lane);
       if constexpr (WIDE) {
-        // this thread's columns: blocks half, half + 2, ...; at most two of them (BN = 128)
-        constexpr int NB = (GATED ? COLS / 32 : BN / 32) > 2 ? 2 : 1;
-        float sum[NB][32], sum_u[GATED ? NB : 1][32];
+        // this thread's sums, added up over the runs: at most two blocks
+        constexpr int NB = BLOCKS > 4 ? 2 : 1;
+        static_assert(BLOCKS <= 8, "blocks of a warp");
+        float sum[NB][CB], sum_u[TWO ? NB : 1][CB], sum_dh[RECOMP ? NB : 1][CB];
 #pragma unroll
         for (int k = 0; k < NB; ++k)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < CB; ++j) {
             sum[k][j] = 0.0f;
-            if (GATED) sum_u[k][j] = 0.0f;
+            if (TWO) sum_u[k][j] = 0.0f;
+            if (RECOMP) sum_dh[k][j] = 0.0f;
           }
         for (int k0 = w.kb0; k0 < w.kb1; k0 += RUN) {
           if (!wait_acc()) break;
-          const uint32_t acc = lanes + (uint32_t)((done & 1) * BN);
+          const uint32_t acc = lanes + (uint32_t)((done & 1) * ACC);
 #pragma unroll
           for (int k = 0; k < NB; ++k) {
-            const int c = half + 2 * k;
-            if (c * 32 >= COLS) break;
-            float t[32];
-            tmem_ld32(acc + c * 32, t);
-            tmem_ld32_wait(t);
+            const int c = first + 4 * k;
+            if (c >= BLOCKS) break;
+            float t[CB];
+            tmem_load(acc + c * CB, t);
+            tmem_wait(t);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[k][j] += t[j];
-            if constexpr (GATED) {
-              tmem_ld32(acc + COLS + c * 32, t);
-              tmem_ld32_wait(t);
+            for (int j = 0; j < CB; ++j) sum[k][j] += t[j];
+            if constexpr (TWO) {
+              tmem_load(acc + COLS + c * CB, t);
+              tmem_wait(t);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sum_u[k][j] += t[j];
+              for (int j = 0; j < CB; ++j) sum_u[k][j] += t[j];
+            }
+            if constexpr (RECOMP) {
+              tmem_load(acc + 2 * COLS + c * CB, t);
+              tmem_wait(t);
+#pragma unroll
+              for (int j = 0; j < CB; ++j) sum_dh[k][j] += t[j];
             }
           }
           release_acc();
@@ -819,26 +866,41 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         if (!ok) break;
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-          const int c = half + 2 * k;
-          if (c * 32 >= COLS) break;
-          if (EPI == EPI_DGATE && n0 + c * 32 < a.N) raw.load(saved_block(c), lane);
-          block(c, sum[k], sum_u[GATED ? k : 0], raw);
+          const int c = first + 4 * k;
+          if (c >= BLOCKS) break;
+          if (k > 0 && use_bias) bias = bias_of(n0 + c * CB);
+          if constexpr (EPI == EPI_DGATE) {
+            if (k > 0 && n0 + c * CB < a.N) raw.load(saved_block(c), lane);
+            float g[CB], u[CB];
+            raw.decode(g, u);
+            block(c, g, u, sum[k], bias);
+          } else {
+            block(c, sum[k], sum_u[TWO ? k : 0], sum_dh[RECOMP ? k : 0], bias);
+          }
         }
       } else {
-        // the first block's saved values are fetched while the products run, the next ones' a block ahead
-        if (EPI == EPI_DGATE && n0 + half * 32 < a.N) raw.load(saved_block(half), lane);
         if (!wait_acc()) break;
-        const uint32_t acc = lanes + (uint32_t)((done & 1) * BN);
+        const uint32_t acc = lanes + (uint32_t)((done & 1) * ACC);
 #pragma unroll 1
-        for (int c = half; c < COLS / 32; c += 2) {
-          float v[32], u[32];
-          tmem_ld32(acc + c * 32, v);
-          if (GATED) tmem_ld32(acc + COLS + c * 32, u);
-          tmem_ld32_wait(v);
-          if (GATED) tmem_ld32_wait(u);
-          const SavedRaw<T> now = raw;
-          if (EPI == EPI_DGATE && c + 2 < COLS / 32 && n0 + (c + 2) * 32 < a.N) raw.load(saved_block(c + 2), lane);
-          block(c, v, u, now);
+        for (int c = first; c < BLOCKS; c += 4) {
+          float v[CB], u[CB], dh[CB];
+          const bool more = c + 4 < BLOCKS && n0 + (c + 4) * CB < a.N;
+          const float now = bias;
+          if constexpr (EPI == EPI_DGATE) {
+            tmem_load(acc + c * CB, dh);
+            raw.decode(v, u);
+            if (more) raw.load(saved_block(c + 4), lane);
+            tmem_wait(dh);
+          } else {
+            tmem_load(acc + c * CB, v);
+            if (TWO) tmem_load(acc + COLS + c * CB, u);
+            if (RECOMP) tmem_load(acc + 2 * COLS + c * CB, dh);
+            tmem_wait(v);
+            if (TWO) tmem_wait(u);
+            if (RECOMP) tmem_wait(dh);
+          }
+          if (more && use_bias) bias = bias_of(n0 + (c + 4) * CB);
+          block(c, v, u, dh, now);
         }
         release_acc();
       }

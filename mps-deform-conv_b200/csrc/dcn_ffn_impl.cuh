@@ -30,9 +30,9 @@ bool make_map(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_rows) 
                       (uint64_t)o.plane, box_rows, BK);
 }
 
-// 32 x 32 blocks of a 16-bit result, staged with the 64-byte swizzle.
+// 32 x 16 blocks of a 16-bit result, staged with the 32-byte swizzle.
 bool make_store_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
-  return make_tmap_3d(map, base, bf16, 1, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint64_t)(rows * ld), 32, 32);
+  return make_tmap_3d(map, base, bf16, 1, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint64_t)(rows * ld), 32, CB);
 }
 
 // ---------------------------------------------------------------- packing
@@ -371,7 +371,7 @@ cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* s
   a.ldo = w.h.ld;
   a.plane = w.h.plane;
   a.bias[0] = t.b_gate; a.bias[1] = t.b_up;
-  a.saved = saved;
+  a.saved = s.recompute() ? nullptr : saved;
   if (sizeof(T) == 2 && !make_store_map(&maps.out[0], w.h.base, operand_bf16<T>(), s.M, s.F, w.h.ld))
     return cudaErrorInvalidValue;
   if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
@@ -400,26 +400,39 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
   if (hidden_grads) {
     GemmArgs a{};
     Maps maps;
-    a.nseg = fill_segments<T>(a.seg, {{0, 1}});
+    const bool again = s.recompute(), bf16 = operand_bf16<T>();
+    a.nseg = fill_segments<T>(a.seg, {{0, again ? 2 : 1}});
     a.M = (int)s.M; a.N = (int)s.F;
     a.nk = (int)div_up(s.C, BK);
-    const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, false, false, sizeof(T) == 4);
-    if (!make_map(&maps.m[0], w.dy, operand_bf16<T>(), BM) || !make_map(&maps.m[1], w.wd, operand_bf16<T>(), BK))
-      return cudaErrorInvalidValue;
+    GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, false, false, sizeof(T) == 4);
+    bool ok;
+    if (again) {
+      plan.tiles_n = (int)div_up(s.F, kRecomputeCols);
+      plan.workers = (int)std::min<int64_t>((int64_t)plan.tiles_m * plan.tiles_n, kSms);
+      ok = make_map(&maps.m[0], w.x, bf16, BM) && make_map(&maps.m[1], w.dy, bf16, BM) &&
+           make_map(&maps.m[2], w.wg, bf16, kRecomputeCols) && make_map(&maps.m[3], w.wu, bf16, kRecomputeCols) &&
+           make_map(&maps.m[4], w.wd, bf16, BK);
+      a.bias[0] = t.b_gate; a.bias[1] = t.b_up;
+    } else {
+      ok = make_map(&maps.m[0], w.dy, bf16, BM) && make_map(&maps.m[1], w.wd, bf16, BK);
+      a.saved = const_cast<void*>(saved);
+    }
+    if (sizeof(T) == 2)
+      ok = ok && make_store_map(&maps.out[0], w.dg.base, bf16, s.M, s.F, w.dg.ld) &&
+           make_store_map(&maps.out[1], w.du.base, bf16, s.M, s.F, w.du.ld);
+    if (!ok) return cudaErrorInvalidValue;
     a.tiles_m = plan.tiles_m; a.tiles_n = plan.tiles_n; a.batches = 1;
     a.group_m = 8;
     a.act = p.act;
-    a.operand_bf16 = operand_bf16<T>();
+    a.operand_bf16 = bf16;
     a.out[0] = const_cast<void*>(w.dg.base); a.out[1] = const_cast<void*>(w.du.base);
     a.ldo = w.dg.ld;
     a.plane = w.dg.plane;
-    a.saved = const_cast<void*>(saved);
-    if (sizeof(T) == 2 && (!make_store_map(&maps.out[0], w.dg.base, operand_bf16<T>(), s.M, s.F, w.dg.ld) ||
-                           !make_store_map(&maps.out[1], w.du.base, operand_bf16<T>(), s.M, s.F, w.du.ld)))
-      return cudaErrorInvalidValue;
     a.colsum = g.b_gate || g.b_up ? w.colsum : nullptr;
     if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
-    if ((e = launch_gemm<T, EPI_DGATE, false, true>("ffn_dhidden", plan, maps, a, st)) != cudaSuccess) return e;
+    e = again ? launch_gemm<T, EPI_RECOMPUTE, kRecomputeBn, false, false>("ffn_dhidden", maps, a, plan.workers, st)
+              : launch_gemm<T, EPI_DGATE, false, true>("ffn_dhidden", plan, maps, a, st);
+    if (e != cudaSuccess) return e;
     if (a.colsum) {
       KernelScope ks("ffn_column_finish", st);
       ffn_column_finish_kernel<T><<<dim3((unsigned)div_up(s.F, 32), 2), 1024, 0, st>>>(

@@ -17,8 +17,16 @@ inline int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
 constexpr int BM = 128;  // tile rows
 constexpr int BK = 64;   // contracted values of a stage (128 bytes)
 
-// Bytes of the saved gate and up values of a 32 x 32 block (dcn_ffn_gemm.cuh).
-constexpr size_t saved_block_bytes(bool wide) { return wide ? 8192 : 4096 + 64; }
+// Bytes of the saved gate and up values of a 32 x 16 block (dcn_ffn_gemm.cuh).
+constexpr size_t saved_block_bytes(bool wide) { return wide ? 4096 : 2048 + 64; }
+
+// Whether the backward computes gate and up again beside dhidden instead of
+// reading what the forward saved.  Again: 4 C more operations a hidden value
+// (24 C on fp32 data, six passes) at some 1.2 PFLOP/s; saved: 8.25 (16) bytes
+// more, written and read at 6.4 TB/s, and kept in between.  The two meet near
+// 390 (125) channels; at and below the bounds the saved state is left out, and
+// gate and up enter the derivative unrounded.
+constexpr bool recompute_gate_up(int64_t channels, bool wide) { return channels <= (wide ? 128 : 256); }
 
 // A matrix as the products read it: 16-bit planes of [rows][ld], rows on
 // 16-byte boundaries.
@@ -85,6 +93,7 @@ struct Shape {
   size_t es;
   explicit Shape(const FfnProblem& p)
       : M(p.M), C(p.C), F(p.F), wide(p.dtype == DCN_FLOAT32), planes(wide ? 3 : 1), pair(wide ? 6 : 1), es(wide ? 4 : 2) {}
+  bool recompute() const { return recompute_gate_up(C, wide); }
   bool pack_rows_c() const { return wide || C % 8 != 0; }  // x, dy, w_gate, w_up: rows of C
   bool pack_rows_f() const { return wide || F % 8 != 0; }  // w_down: rows of F
   size_t operand_bytes(int64_t rows, int64_t cols) const {
@@ -101,7 +110,8 @@ struct Shape {
     return o;
   }
   size_t blocks_bytes() const {
-    const int64_t m = div_up(M, BM) * 4, c = div_up(F, 32);
+    if (recompute()) return 0;
+    const int64_t m = div_up(M, BM) * 4, c = div_up(F, 16);
     return ws_align((size_t)(m * c) * saved_block_bytes(wide));
   }
 };

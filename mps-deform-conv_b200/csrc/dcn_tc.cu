@@ -480,7 +480,7 @@ bool make_tmap_3d(CUtensorMap* map, const void* base, bool bf16, uint64_t planes
   const cuuint64_t strides[2] = {ld * 2, plane * 2};
   const cuuint32_t box[3] = {box_cols, box_rows, 1};
   return encode_tmap(map, base, bf16, 3, dims, strides, box,
-                     box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+                     box_cols == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Forward weight image wsw of `w` (weight_images_kernel, or the per-image

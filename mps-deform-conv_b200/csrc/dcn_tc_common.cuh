@@ -657,7 +657,7 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, 
 
 // Host: the same over `planes` matrices [rows][cols] of row stride `ld` and
 // distance `plane` (elements; ld and plane multiples of 8, base on 16 bytes).
-// A box of 32 columns (64-byte rows) has the 64-byte swizzle.
+// A box of 16 columns (32-byte rows) has the 32-byte swizzle.
 bool make_tmap_3d(CUtensorMap* map, const void* base, bool bf16, uint64_t planes, uint64_t rows, uint64_t cols,
                   uint64_t ld, uint64_t plane, uint32_t box_rows, uint32_t box_cols);
 

@@ -42,8 +42,13 @@ def test_null_descriptor_and_sizes():
             hidden = -(-planes * m * ld * 2 // 256) * 256
             assert lib.dcn_ffn_forward_workspace_size(ctypes.byref(d), 0) - \
                 lib.dcn_ffn_forward_workspace_size(ctypes.byref(d), 1) == hidden
-            assert lib.dcn_ffn_saved_bytes(ctypes.byref(d)) > hidden
+            # up to 256 (fp32: 128) channels gate and up are computed again, not saved
+            assert lib.dcn_ffn_saved_bytes(ctypes.byref(d)) == hidden
             assert lib.dcn_ffn_backward_workspace_size(ctypes.byref(d)) >= 2 * hidden
+    for dt, c in ((_abi.DCN_FLOAT32, 128), (_abi.DCN_BFLOAT16, 256)):
+        few, many = _desc(dt, 0, 1000, c, 64), _desc(dt, 0, 1000, c + 1, 64)
+        gate_up = 1000 * 64 * 2 * (4 if dt == _abi.DCN_FLOAT32 else 2)
+        assert lib.dcn_ffn_saved_bytes(ctypes.byref(many)) - lib.dcn_ffn_saved_bytes(ctypes.byref(few)) >= gate_up
 
 
 def _tensors(**kw):

@@ -6,7 +6,8 @@ Bounds are elementwise and count roundings:
     products' absolute values.  fp32 data runs six such passes, and drops terms below
     3 * 2^-24 of a product;
   * the hidden values and their gradients are rounded to the type (half of its eps) as
-    operands; saved gate and up values of 16-bit data to 11 bits;
+    operands and as summands of the bias gradients; saved gate and up values of 16-bit data
+    (more than 256 channels) to 11 bits;
   * errors of gate and up enter the activation by its largest slope, those of its derivative
     by the largest curvature (relu: a sign may change where gate is within its own error);
   * the fast exponential and quotient of 16-bit data: 2^-19 of the value; fp32: 2^-21.
@@ -77,7 +78,7 @@ def _reference(args, dy, act, dtype):
     dy = dy.double()
     dh = dy @ wd
     e_dh = _sum_err(c, dtype) * (dy.abs() @ wd.abs())
-    if not wide:  # gate and up come back from the saved state with 11 bits
+    if not wide and c > 256:  # gate and up come back from the saved state with 11 bits
         e_g = e_g + 2.0 ** -11 * (gate.abs() + e_g) + 2.0 ** -36 * gate.abs().amax(1, keepdim=True)
         e_u = e_u + 2.0 ** -11 * (up.abs() + e_u) + 2.0 ** -36 * up.abs().amax(1, keepdim=True)
         e_a = SLOPE[act] * e_g + fast * (a.abs() + e_g)
@@ -88,7 +89,6 @@ def _reference(args, dy, act, dtype):
     e_dup = e_dh * (a.abs() + e_a) + dh.abs() * e_a + 2.0 ** -23 * dup.abs()
     dgate = dh * up * da
     e_dgate = (e_dh * (up.abs() + e_u) + dh.abs() * e_u) * (da.abs() + e_da) + (dh * up).abs() * e_da + 2.0 ** -22 * dgate.abs()
-    e_bg, e_bu = e_dgate, e_dup          # bias gradients sum the unrounded values
     if not wide:
         e_dup = e_dup + u * (dup.abs() + e_dup) + floor
         e_dgate = e_dgate + u * (dgate.abs() + e_dgate) + floor
@@ -101,7 +101,7 @@ def _reference(args, dy, act, dtype):
     out.append(done(dy.t() @ h, dy.abs().t() @ e_h + sm * (dy.abs().t() @ h.abs())))
     if bg is not None:
         lin = (m / 32 + 40) * 2.0 ** -24    # running sums of fp32 values
-        out += [done(d.sum(0), e.sum(0) + lin * d.abs().sum(0)) for d, e in ((dgate, e_bg), (dup, e_bu))]
+        out += [done(d.sum(0), e.sum(0) + lin * d.abs().sum(0)) for d, e in ((dgate, e_dgate), (dup, e_dup))]
     if bd is not None:
         out.append(done(dy.sum(0), (m / 32 + 40) * 2.0 ** -24 * dy.abs().sum(0)))
     return out
@@ -130,7 +130,7 @@ def _run(args, dy, act):
 
 SIZES = [(1, 8, 8), (1, 512, 2048), (2, 1, 1), (3, 5, 7), (31, 64, 64), (127, 64, 136), (128, 64, 128), (129, 72, 200),
          (300, 100, 267), (257, 24, 40), (640, 96, 255), (1000, 256, 1024), (700, 320, 33), (4100, 64, 170),
-         (9000, 128, 512)]
+         (9000, 128, 512), (2000, 512, 300), (513, 264, 520), (90, 257, 65)]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
