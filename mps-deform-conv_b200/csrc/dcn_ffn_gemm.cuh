@@ -20,11 +20,11 @@
 // 17 the TMA loads.  A CTA works through its share of the output tiles; the
 // accumulator is double-buffered in TMEM, so a tile's epilogue runs under the
 // next tile's MMAs.  Epilogue warp w reads TMEM lanes 32 (w % 4) .. +31: lane i
-// owns one row, 16 columns at a time, and takes blocks w / 4, w / 4 + 4, ... of
-// the tile.  Sixteen warps of 16-column blocks and not eight of 32: the blocks'
-// chains of loads, exponentials and stores leave two warps a scheduler idle
-// more than half of the time (issue active 41 % and 53 % in the two gated
-// epilogues of 23104 x 512 -> 2048 rows in bf16).
+// owns one row, 16 columns at a time.  On 16-bit data warps 0-7 take the tiles
+// of the first accumulator buffer and warps 8-15 those of the second, so that
+// one half's stores go out while the other half computes: with all warps on
+// one tile their phases (TMEM reads, stores of gate and up, arithmetic, store
+// of the results) follow one another and their times add up.
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along
@@ -35,6 +35,16 @@
 // workers left over share the end of K in equal runs.  Each piece is an fp32
 // partial in a slot of its own, and a second kernel adds a tile's slots in a
 // fixed order: the result does not depend on timing.
+//
+// Pairs (template PAIR): two CTAs of a cluster share a tile of 256 rows
+// (tcgen05 cta_group::2).  Each holds its own 128 rows of the row operand, half
+// of the column operand (GATED: one gate, the other up) and the accumulator of
+// its rows; the first issues the MMAs for both.  A CTA alone reads 384 operand
+// rows for 128 x 256 results, a pair 512 for 256 x 256: the single-CTA products
+// were bound by their operand reads from the L2 (about 15 TB/s; everything an
+// epilogue wrote came on top of the products' time), and a pair reads a third
+// less.  Loads go to the CTA's own shared memory and report to the first CTA's
+// barrier; commits arrive at both.
 //
 // Every mbarrier wait is bounded (dcn_sm100.cuh).
 #pragma once
@@ -67,22 +77,27 @@ enum Epi { EPI_GATED, EPI_DGATE, EPI_RECOMPUTE, EPI_STORE };
 // Accumulator columns are BN; EPI_RECOMPUTE has 3 x 64 (gate, up, dhidden) and
 // two row operands (x, dy).
 constexpr int kRecomputeCols = 64, kRecomputeBn = 3 * kRecomputeCols;
-__host__ __device__ constexpr uint32_t stage_bytes(int bn) {
-  return (bn == kRecomputeBn ? 2 : 1) * A_STAGE + (uint32_t)bn * 128u;
+__host__ __device__ constexpr uint32_t stage_bytes(int bn, bool pair) {
+  return (bn == kRecomputeBn ? 2 : 1) * A_STAGE + (uint32_t)bn * 128u / (pair ? 2u : 1u);
 }
-__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 4 : bn == kRecomputeBn ? 3 : bn == 128 ? 6 : 8; }
+// as many stages as 192 KB hold, at most eight
+__host__ __device__ constexpr int stages(int bn, bool pair) {
+  return 196608 / stage_bytes(bn, pair) < 8 ? (int)(196608 / stage_bytes(bn, pair)) : 8;
+}
 // operand stages, then two staged output blocks and 32 bias values of each
 // epilogue warp, then barriers
 constexpr uint32_t kStageBlock = 32 * CB * 2;
 constexpr uint32_t kStaging = EPI_WARPS * 2 * kStageBlock;
-__host__ __device__ constexpr uint32_t smem_bytes(int bn) {
-  return (uint32_t)stages(bn) * stage_bytes(bn) + kStaging + EPI_WARPS * 32 * 4u +
-         (2u * (uint32_t)stages(bn) + 5u) * 8u + 16u;
+__host__ __device__ constexpr uint32_t smem_bytes(int bn, bool pair) {
+  return (uint32_t)stages(bn, pair) * stage_bytes(bn, pair) + kStaging + EPI_WARPS * 32 * 4u +
+         (2u * (uint32_t)stages(bn, pair) + 5u) * 8u + 16u;
 }
 // dynamic shared memory starts on 1024 bytes when a kernel has no static one;
 // this much is left over for a start that does not (checked by the kernel)
 constexpr uint32_t kSmemSlack = 768;
-static_assert(smem_bytes(256) + kSmemSlack <= 232448, "shared memory of one CTA");
+static_assert(smem_bytes(256, false) + kSmemSlack <= 232448 && smem_bytes(256, true) + kSmemSlack <= 232448 &&
+                  smem_bytes(128, true) + kSmemSlack <= 232448,
+              "shared memory of one CTA");
 // fp32 data: K blocks added up in TMEM before their sum moves on to registers
 constexpr int kWideRun = 4;
 
@@ -151,6 +166,80 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+
+// ---------------------------------------------------------------- CTA pairs
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// All threads of both CTAs.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The cluster address of `addr` in the first CTA.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc_g(uint32_t slot, uint32_t ncols) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, ncols);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_dealloc_g(uint32_t taddr, uint32_t ncols) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+  else tmem_dealloc(taddr, ncols);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_g(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    mma_f16(d, ad, bd, idesc, accumulate);
+}
+// Arrives on `bar` of this CTA (PAIR and both: of both CTAs) once the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit_g(uint32_t bar, bool both) {
+  if (!PAIR) {
+    mma_commit(bar);
+  } else if (both) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  } else {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  }
+}
+// A load into this CTA's shared memory; PAIR: `bar` is a cluster address in the first CTA.
+template <bool PAIR>
+__device__ __forceinline__ void load_g(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    tma_load_3d(dst, map, x, y, z, bar);
 }
 
 // ---------------------------------------------------------------- activations
@@ -515,16 +604,17 @@ __device__ __forceinline__ void tile_at(const GemmArgs& a, int tile, int& z, int
 }
 
 // ---------------------------------------------------------------- kernel
-template <typename T, int EPI, int BN, bool A_MN, bool B_MN>
+template <typename T, int EPI, int BN, bool A_MN, bool B_MN, bool PAIR>
 __global__ void __launch_bounds__(NTHREADS, 1)
 ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs a) {
-  constexpr int S = stages(BN);
-  constexpr uint32_t STAGE = stage_bytes(BN);
+  constexpr int S = stages(BN, PAIR);
+  constexpr uint32_t STAGE = stage_bytes(BN, PAIR);
   constexpr bool GATED = EPI == EPI_GATED, RECOMP = EPI == EPI_RECOMPUTE, TWO = GATED || RECOMP;
   constexpr bool DGATE = EPI == EPI_DGATE || RECOMP;
   constexpr int COLS = GATED ? BN / 2 : RECOMP ? BN / 3 : BN;  // output columns of a tile
   constexpr int ACC = RECOMP ? 256 : BN;                       // TMEM columns of an accumulator buffer
   constexpr uint32_t B_AT = (RECOMP ? 2 : 1) * A_STAGE;        // column operands in a stage
+  constexpr int CTAS = PAIR ? 2 : 1;
   constexpr bool WIDE = sizeof(T) == 4;
   // K blocks of one accumulation in TMEM.  The tensor cores truncate each
   // addition to the accumulator, an error that grows with the number of steps
@@ -534,12 +624,16 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   constexpr int RUN = WIDE ? kWideRun : 1 << 30;
   static_assert(!WIDE || BN <= 128 || RECOMP, "an epilogue thread holds 32 to 48 sums");
   static_assert(RECOMP == (BN == kRecomputeBn), "accumulator columns");
+  static_assert(!PAIR || !RECOMP, "half of 64 dhidden columns fills no swizzled row");
+  // epilogue warps that share a tile; fp32 sums stay with their warps over the
+  // runs of a tile, which alternate between the buffers
+  constexpr int GROUP = WIDE ? EPI_WARPS : EPI_WARPS / 2, STEP = GROUP / 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
   uint8_t* staging = smem + S * STAGE;
   uint8_t* tail = staging + kStaging + EPI_WARPS * 32 * 4;
-  if (smem + smem_bytes(BN) > smem_raw + smem_bytes(BN) + kSmemSlack) {  // an unexpected start: nothing is touched
+  if (smem - smem_raw > kSmemSlack) {  // an unexpected start (the same in both CTAs): nothing is touched
     if (threadIdx.x == 0) atomicExch(a.status, ST_FFN_SMEM);
     return;
   }
@@ -553,6 +647,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + (2 * S + 5) * 8 + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_rank() : 0;
   constexpr uint32_t TMEM_COLS = 2 * ACC;
 
   if (threadIdx.x == 0) {
@@ -562,22 +657,20 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), EPI_WARPS);
+      mbar_init(acc_empty(b), GROUP * CTAS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == MMA_WARP) {
-    tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
-    tmem_relinquish();
-  }
+  if (warp == MMA_WARP) tmem_alloc_g<PAIR>(smem_addr(tmem_slot), TMEM_COLS);
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  Work w(a, blockIdx.x, gridDim.x);
+  Work w(a, blockIdx.x / CTAS, gridDim.x / CTAS);
 
   if (warp == LOAD_WARP) {
     // ------------------------------------------------ TMA loads
@@ -587,7 +680,8 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       while (ok && w.next(a)) {
         int z, mt, nt;
         tile_at(a, w.tile, z, mt, nt);
-        const int m0 = mt * BM, n0 = nt * COLS;
+        const int m0 = (mt * CTAS + rank) * BM, n0 = nt * COLS;
+        const int nb = PAIR && !GATED ? n0 + rank * (BN / 2) : n0;  // this CTA's part of the column operand
         int sg = w.kb0 / a.nk, kb = w.kb0 - sg * a.nk;
         for (int i = w.kb0; i < w.kb1; ++i) {
           const int s = issued % S;
@@ -596,28 +690,31 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           const Seg seg = a.seg[sg];
           const int k = kb * BK;
           const uint32_t dst = sbase + s * STAGE;
+          const uint32_t bar = PAIR ? in_first_cta(full(s)) : full(s);
           const CUtensorMap* ma = &maps.m[seg.a_map + z];
           const CUtensorMap* mb = &maps.m[seg.b_map];
-          mbar_arrive_expect_tx(full(s), STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(full(s), CTAS * STAGE);
           if (A_MN) {
-            tma_load_3d(dst, ma, m0, k, seg.a_plane, full(s));
-            tma_load_3d(dst + 8192, ma, m0 + 64, k, seg.a_plane, full(s));
+            load_g<PAIR>(dst, ma, m0, k, seg.a_plane, bar);
+            load_g<PAIR>(dst + 8192, ma, m0 + 64, k, seg.a_plane, bar);
           } else {
-            tma_load_3d(dst, ma, k, m0, seg.a_plane, full(s));
+            load_g<PAIR>(dst, ma, k, m0, seg.a_plane, bar);
           }
-          if (TWO) {
-            tma_load_3d(dst + B_AT, mb, k, n0, seg.b_plane, full(s));
-            tma_load_3d(dst + B_AT + COLS * 128, mb + 1, k, n0, seg.b_plane, full(s));
+          if (GATED && PAIR) {
+            load_g<PAIR>(dst + B_AT, mb + rank, k, n0, seg.b_plane, bar);
+          } else if (TWO) {
+            tma_load_3d(dst + B_AT, mb, k, n0, seg.b_plane, bar);
+            tma_load_3d(dst + B_AT + COLS * 128, mb + 1, k, n0, seg.b_plane, bar);
             if (RECOMP) {  // dy beside x, w_down (MN-major) beside the other two
-              tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, full(s));
-              tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, full(s));
+              tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, bar);
+              tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, bar);
             }
           } else if (B_MN) {
 #pragma unroll
-            for (int q = 0; q < BN / 64; ++q)
-              tma_load_3d(dst + A_STAGE + q * 8192, mb, n0 + 64 * q, k, seg.b_plane, full(s));
+            for (int q = 0; q < BN / 64 / CTAS; ++q)
+              load_g<PAIR>(dst + A_STAGE + q * 8192, mb, nb + 64 * q, k, seg.b_plane, bar);
           } else {
-            tma_load_3d(dst + A_STAGE, mb, k, n0, seg.b_plane, full(s));
+            load_g<PAIR>(dst + A_STAGE, mb, k, nb, seg.b_plane, bar);
           }
           ++issued;
           if (++kb == a.nk) {
@@ -626,14 +723,15 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           }
         }
       }
-      // copies in flight land before the CTA may go
-      for (int i = issued > S ? issued - S : 0; i < issued; ++i)
-        mbar_wait(full(i % S), (i / S) & 1, abort_flag, a.status, ST_FFN_DRAIN);
+      // copies in flight land before the CTA may go (a pair's report to the first CTA)
+      if (rank == 0)
+        for (int i = issued > S ? issued - S : 0; i < issued; ++i)
+          mbar_wait(full(i % S), (i / S) & 1, abort_flag, a.status, ST_FFN_DRAIN);
     }
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      const uint32_t idesc = tcc::idesc_f16_major(BM, TWO ? 2 * COLS : BN, a.operand_bf16 != 0, A_MN, B_MN);
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * COLS : BN, a.operand_bf16 != 0, A_MN, B_MN);
       const uint32_t idesc_dh = tcc::idesc_f16_major(BM, COLS, a.operand_bf16 != 0, false, true);
       int used = 0, done = 0;
       bool ok = true;
@@ -655,29 +753,30 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
             for (int kk = 0; kk < BK / 16; ++kk) {
               const uint64_t ad = A_MN ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192) : desc_kmajor_sw128(ab + kk * 32);
               const uint64_t bd = B_MN ? tcc::desc_mnmajor_sw128(bb + kk * 2048, 8192) : desc_kmajor_sw128(bb + kk * 32);
-              mma_f16(d, ad, bd, idesc, (i > k0 || kk > 0) ? 1u : 0u);
+              mma_g<PAIR>(d, ad, bd, idesc, (i > k0 || kk > 0) ? 1u : 0u);
               if (RECOMP)
                 mma_f16(d + 2 * COLS, desc_kmajor_sw128(ab + A_STAGE + kk * 32),
                         tcc::desc_mnmajor_sw128(bb + 2 * COLS * 128 + kk * 2048, 8192), idesc_dh,
                         (i > k0 || kk > 0) ? 1u : 0u);
             }
-            mma_commit(empty(s));
+            commit_g<PAIR>(empty(s), true);
             ++used;
           }
           if (!ok) break;
-          mma_commit(acc_full(b));
+          commit_g<PAIR>(acc_full(b), true);
           ++done;
         }
       }
       // MMAs still running finish before TMEM and shared memory are released
       if (used > 0) {
-        mma_commit(drain);
+        commit_g<PAIR>(drain, false);
         mbar_wait(drain, 0, abort_flag, a.status, ST_FFN_DRAIN);
       }
     }
   } else {
     // ------------------------------------------------ epilogue
-    const int q = warp & 3, first = warp >> 2;  // lanes 32 q .., column blocks first, first + 4, ...
+    // lanes 32 q .., column blocks first, first + STEP, ... of the tiles of its group
+    const int q = warp & 3, first = (warp % GROUP) >> 2, group = warp / GROUP;
     constexpr int BLOCKS = COLS / CB;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     uint8_t* stage = staging + warp * (2 * kStageBlock);
@@ -720,18 +819,25 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     auto release_acc = [&] {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(done & 1));
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(in_first_cta(acc_empty(done & 1)));
+        else mbar_arrive(acc_empty(done & 1));
+      }
       ++done;
     };
     while (ok && w.next(a)) {
+      if (!WIDE && (done & 1) != group) {  // the other warps' tile
+        ++done;
+        continue;
+      }
       int z, mt, nt;
       tile_at(a, w.tile, z, mt, nt);
       const int n0 = nt * COLS;
-      const int row0 = mt * BM + q * 32;
+      const int row0 = (mt * CTAS + rank) * BM + q * 32;
       const int64_t row = (int64_t)row0 + lane;
       const bool row_in = row < a.M;
       const bool whole = w.slot < 0;
-      const int64_t m_block = (int64_t)mt * 4 + q;
+      const int64_t m_block = row0 / 32;
       auto saved_block = [&](int c) {
         return static_cast<uint8_t*>(a.saved) + saved_block_offset<T>(m_block, n0 / CB + c, col_blocks);
       };
@@ -742,7 +848,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         const int c0 = n0 + c * CB;
         if (!whole) {
           // an fp32 partial of this tile, 16-byte pieces of 32 rows side by side
-          float* slot = a.partial + (int64_t)w.slot * (BM * BN) + q * (32 * BN);
+          float* slot = a.partial + ((int64_t)w.slot * CTAS + rank) * (BM * BN) + q * (32 * BN);
 #pragma unroll
           for (int j = 0; j < CB / 4; ++j)
             *reinterpret_cast<float4*>(slot + c * 512 + j * 128 + lane * 4) =
@@ -841,7 +947,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           const uint32_t acc = lanes + (uint32_t)((done & 1) * ACC);
 #pragma unroll
           for (int k = 0; k < NB; ++k) {
-            const int c = first + 4 * k;
+            const int c = first + STEP * k;
             if (c >= BLOCKS) break;
             float t[CB];
             tmem_load(acc + c * CB, t);
@@ -866,7 +972,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         if (!ok) break;
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-          const int c = first + 4 * k;
+          const int c = first + STEP * k;
           if (c >= BLOCKS) break;
           if (k > 0 && use_bias) bias = bias_of(n0 + c * CB);
           if constexpr (EPI == EPI_DGATE) {
@@ -882,14 +988,14 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         if (!wait_acc()) break;
         const uint32_t acc = lanes + (uint32_t)((done & 1) * ACC);
 #pragma unroll 1
-        for (int c = first; c < BLOCKS; c += 4) {
+        for (int c = first; c < BLOCKS; c += STEP) {
           float v[CB], u[CB], dh[CB];
-          const bool more = c + 4 < BLOCKS && n0 + (c + 4) * CB < a.N;
+          const bool more = c + STEP < BLOCKS && n0 + (c + STEP) * CB < a.N;
           const float now = bias;
           if constexpr (EPI == EPI_DGATE) {
             tmem_load(acc + c * CB, dh);
             raw.decode(v, u);
-            if (more) raw.load(saved_block(c + 4), lane);
+            if (more) raw.load(saved_block(c + STEP), lane);
             tmem_wait(dh);
           } else {
             tmem_load(acc + c * CB, v);
@@ -899,7 +1005,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
             if (TWO) tmem_wait(u);
             if (RECOMP) tmem_wait(dh);
           }
-          if (more && use_bias) bias = bias_of(n0 + (c + 4) * CB);
+          if (more && use_bias) bias = bias_of(n0 + (c + STEP) * CB);
           block(c, v, u, dh, now);
         }
         release_acc();
@@ -910,11 +1016,13 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   }
 
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();  // neither CTA's memory is in use by the other any more
+  else __syncthreads();
   if (warp == MMA_WARP) {
     tc_fence_after();
-    tmem_dealloc(tmem, TMEM_COLS);
+    tmem_dealloc_g<PAIR>(tmem, TMEM_COLS);
   }
+  if (PAIR) cluster_sync();
 }
 
 }  // namespace ffn

@@ -116,23 +116,23 @@ struct ReduceArgs {
   void* out[2];
   const void* bias;
   int64_t ldo;
-  int M, N, tiles_m, tiles_n, group_m, nkb, workers, base, tiles, vec;
+  int M, N, tiles_m, tiles_n, group_m, nkb, workers, base, tiles, ctas, vec;
 };
 
 template <typename T, int BN>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__ ReduceArgs a) {
   __shared__ float4 part[8][8][32];
-  constexpr int BLOCKS = BN / 32 * 4;  // 32 x 32 blocks of a tile
+  const int quarters = 4 * a.ctas, blocks = BN / 32 * quarters;  // 32 x 32 blocks of a tile
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = blockIdx.x / BLOCKS, blk = blockIdx.x - t * BLOCKS;
-  const int q = blk & 3, c = blk >> 2;
+  const int t = blockIdx.x / blocks, blk = blockIdx.x - t * blocks;
+  const int q = blk % quarters, c = blk / quarters;
   GemmArgs g;
   g.tiles_m = a.tiles_m; g.tiles_n = a.tiles_n; g.group_m = a.group_m;
   int z, mt, nt;
   tile_at(g, a.base + t, z, mt, nt);
-  const int64_t row = (int64_t)mt * BM + q * 32 + lane;
+  const int64_t row = (int64_t)mt * BM * a.ctas + q * 32 + lane;
   const int c0 = nt * BN + c * 32;
-  if (mt * BM + q * 32 >= a.M || c0 >= a.N) return;
+  if (row - lane >= a.M || c0 >= a.N) return;
   const Cut cut(a.tiles, a.workers, a.nkb);
   int e0 = 0, e1 = -1;  // the runs that touch this tile
   if (cut.rest() > 0) {
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__
   const int n = slices + (e1 - e0 + 1);
   for (int i = warp; i < n; i += 8) {
     const int slot = i < slices ? i * cut.R + t : cut.S * cut.R + e0 + (i - slices) + t;
-    const float4* p = reinterpret_cast<const float4*>(a.partial + (int64_t)slot * (BM * BN) + q * (32 * BN) + c * 1024) + lane;
+    const float4* p = reinterpret_cast<const float4*>(a.partial + (int64_t)slot * a.ctas * (BM * BN) + q * (32 * BN) + c * 1024) + lane;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float4 f = p[j * 32];
@@ -244,25 +244,38 @@ __global__ void __launch_bounds__(1024) ffn_column_finish_kernel(const float* __
   }
 }
 
-template <typename T, int EPI, int BN, bool A_MN, bool B_MN>
+template <typename T, int EPI, int BN, bool A_MN, bool B_MN, bool PAIR>
 cudaError_t launch_gemm(const char* name, const Maps& maps, const GemmArgs& a, int workers, cudaStream_t st) {
-  auto kern = ffn_gemm_kernel<T, EPI, BN, A_MN, B_MN>;
-  const int smem = (int)(smem_bytes(BN) + kSmemSlack);
+  auto kern = ffn_gemm_kernel<T, EPI, BN, A_MN, B_MN, PAIR>;
+  const int smem = (int)(smem_bytes(BN, PAIR) + kSmemSlack);
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(workers * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(NTHREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
   KernelScope ks(name, st);
-  kern<<<workers, NTHREADS, smem, st>>>(maps, a);
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 
 template <typename T, int EPI, bool A_MN, bool B_MN>
 cudaError_t launch_gemm(const char* name, const GemmPlan& p, const Maps& maps, const GemmArgs& a, cudaStream_t st) {
+  // pairs have the widest tile of their type, 256 columns or 128 (fp32)
+  if (p.pair) return launch_gemm<T, EPI, sizeof(T) == 4 ? 128 : 256, A_MN, B_MN, true>(name, maps, a, p.workers, st);
   switch (p.bn) {
     case 256:
-      if constexpr (sizeof(T) == 2) return launch_gemm<T, EPI, 256, A_MN, B_MN>(name, maps, a, p.workers, st);
+      if constexpr (sizeof(T) == 2) return launch_gemm<T, EPI, 256, A_MN, B_MN, false>(name, maps, a, p.workers, st);
       return cudaErrorInvalidValue;  // fp32 plans stop at 128
-    case 128: return launch_gemm<T, EPI, 128, A_MN, B_MN>(name, maps, a, p.workers, st);
-    default: return launch_gemm<T, EPI, 64, A_MN, B_MN>(name, maps, a, p.workers, st);
+    case 128: return launch_gemm<T, EPI, 128, A_MN, B_MN, false>(name, maps, a, p.workers, st);
+    default: return launch_gemm<T, EPI, 64, A_MN, B_MN, false>(name, maps, a, p.workers, st);
   }
 }
 
@@ -303,7 +316,7 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   for (int i = 0; i < n_a; ++i)
     if (!make_map(&maps.m[i], a_ops[i], operand_bf16<T>(), A_MN ? BK : BM)) return cudaErrorInvalidValue;
   for (int i = 0; i < pairs; ++i)
-    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B_MN ? BK : p.bn)) return cudaErrorInvalidValue;
+    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B_MN ? BK : p.pair ? p.bn / 2 : p.bn)) return cudaErrorInvalidValue;
   a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n; a.batches = batches;
   a.group_m = 8;
   a.split = p.split;
@@ -332,7 +345,8 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   r.base = tiles / p.workers * p.workers;
   r.tiles = tiles - r.base;
   KernelScope ks("ffn_reduce", st);
-  const unsigned grid = (unsigned)(r.tiles * (p.bn / 32 * 4));
+  r.ctas = p.pair ? 2 : 1;
+  const unsigned grid = (unsigned)(r.tiles * (p.bn / 32 * 4 * r.ctas));
   if (p.bn == 256) ffn_reduce_kernel<T, 256><<<grid, 256, 0, st>>>(r);
   else if (p.bn == 128) ffn_reduce_kernel<T, 128><<<grid, 256, 0, st>>>(r);
   else ffn_reduce_kernel<T, 64><<<grid, 256, 0, st>>>(r);
@@ -407,6 +421,8 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
     GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, false, false, sizeof(T) == 4);
     bool ok;
     if (again) {
+      plan.pair = false;
+      plan.tiles_m = (int)div_up(s.M, BM);
       plan.tiles_n = (int)div_up(s.F, kRecomputeCols);
       plan.workers = (int)std::min<int64_t>((int64_t)plan.tiles_m * plan.tiles_n, kSms);
       ok = make_map(&maps.m[0], w.x, bf16, BM) && make_map(&maps.m[1], w.dy, bf16, BM) &&
@@ -430,13 +446,13 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
     a.plane = w.dg.plane;
     a.colsum = g.b_gate || g.b_up ? w.colsum : nullptr;
     if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
-    e = again ? launch_gemm<T, EPI_RECOMPUTE, kRecomputeBn, false, false>("ffn_dhidden", maps, a, plan.workers, st)
+    e = again ? launch_gemm<T, EPI_RECOMPUTE, kRecomputeBn, false, false, false>("ffn_dhidden", maps, a, plan.workers, st)
               : launch_gemm<T, EPI_DGATE, false, true>("ffn_dhidden", plan, maps, a, st);
     if (e != cudaSuccess) return e;
     if (a.colsum) {
       KernelScope ks("ffn_column_finish", st);
       ffn_column_finish_kernel<T><<<dim3((unsigned)div_up(s.F, 32), 2), 1024, 0, st>>>(
-          w.colsum, static_cast<T*>(g.b_gate), static_cast<T*>(g.b_up), div_up(s.M, BM) * 4, 2, (int)s.F);
+          w.colsum, static_cast<T*>(g.b_gate), static_cast<T*>(g.b_up), (int64_t)plan.tiles_m * (plan.pair ? 8 : 4), 2, (int)s.F);
       if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
   }

@@ -39,31 +39,40 @@ struct Operand {
 // ---------------------------------------------------------------- plans
 struct GemmPlan {
   int bn = 256;
-  bool split = false;
-  int workers = 0;
+  bool pair = false, split = false;
+  int workers = 0;  // CTAs, or pairs of them
   int tiles_m = 0, tiles_n = 0;
   size_t partial_bytes() const {
-    return split ? ((size_t)workers + (size_t)tiles_m * tiles_n * 2) * BM * bn * 4 : 0;
+    return split ? ((size_t)workers + (size_t)tiles_m * tiles_n * 2) * BM * (pair ? 2 : 1) * bn * 4 : 0;
   }
 };
 
-// Column tile: the one whose waves of tiles cost least, a tile's time being
-// its columns over the relative rate of that width (a narrower tile reads the
-// row operand more often for the same work).  splittable: the product stores
-// plain sums, so too few tiles for the SMs can be cut into equal runs.
+// Column tile and CTA pairing: the choice whose waves of tiles cost least, a
+// tile's time being its columns over the relative rate of that form (a narrower
+// or unpaired tile reads more operand rows for the same work).  splittable: the
+// product stores plain sums, so the tiles of a last wave that would leave many
+// SMs idle can be cut along K.
 inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool gated, bool splittable,
                           bool wide) {
+  struct Form {
+    int bn;
+    bool pair;
+    double rate;
+  };
+  static const Form kNarrow[4] = {{256, true, 1.0}, {256, false, 0.8}, {128, false, 0.65}, {64, false, 0.4}};
+  static const Form kWide[3] = {{128, true, 1.0}, {128, false, 0.8}, {64, false, 0.5}};  // fp32 sums live in registers
   GemmPlan best;
   double best_cost = 1e300;
-  for (int bn : {256, 128, 64}) {
-    if (wide && bn == 256) continue;  // fp32 sums live in registers, half a row of them a thread
-    const int cols = gated ? bn / 2 : bn;
-    const double rate = bn == 256 ? 1.0 : bn == 128 ? 0.8 : 0.5;
-    const int64_t tm = div_up(M, BM), tn = div_up(N, cols), tiles = tm * tn * batches;
-    double cost = (double)div_up(tiles, kSms) * bn / rate * (double)nkb;
+  const Form* forms = wide ? kWide : kNarrow;
+  for (int i = 0; i < (wide ? 3 : 4); ++i) {
+    const Form& f = forms[i];
+    const int cols = gated ? f.bn / 2 : f.bn, rows = f.pair ? 2 * BM : BM, all = f.pair ? kSms / 2 : kSms;
+    const int64_t tm = div_up(M, rows), tn = div_up(N, cols), tiles = tm * tn * batches;
+    const double tile = f.bn / f.rate * (double)nkb;
+    double cost = (double)div_up(tiles, all) * tile;
     bool split = false;
-    if (splittable && tiles < 4 * kSms && tiles * nkb >= 8 * kSms) {
-      const double cut = (double)tiles / kSms * bn / rate * (double)nkb + 24.0 * bn;  // + writing and adding partials
+    if (splittable && tiles < 4 * all && tiles * nkb >= 8 * all) {
+      const double cut = (double)tiles / all * tile + 24.0 * f.bn;  // + writing and adding partials
       if (cut < 0.95 * cost) {
         split = true;
         cost = cut;
@@ -71,9 +80,10 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
     }
     if (cost < best_cost) {
       best_cost = cost;
-      best.bn = bn;
+      best.bn = f.bn;
+      best.pair = f.pair;
       best.split = split;
-      best.workers = (int)(split ? kSms : std::min<int64_t>(tiles, kSms));
+      best.workers = (int)(split ? all : std::min<int64_t>(tiles, all));
       best.tiles_m = (int)tm;
       best.tiles_n = (int)tn;
     }
@@ -93,6 +103,7 @@ struct Shape {
   size_t es;
   explicit Shape(const FfnProblem& p)
       : M(p.M), C(p.C), F(p.F), wide(p.dtype == DCN_FLOAT32), planes(wide ? 3 : 1), pair(wide ? 6 : 1), es(wide ? 4 : 2) {}
+  int64_t row_blocks() const { return div_up(M, 2 * BM) * 8; }  // 32-row blocks, to whole tiles of a pair
   bool recompute() const { return recompute_gate_up(C, wide); }
   bool pack_rows_c() const { return wide || C % 8 != 0; }  // x, dy, w_gate, w_up: rows of C
   bool pack_rows_f() const { return wide || F % 8 != 0; }  // w_down: rows of F
@@ -111,7 +122,7 @@ struct Shape {
   }
   size_t blocks_bytes() const {
     if (recompute()) return 0;
-    const int64_t m = div_up(M, BM) * 4, c = div_up(F, 16);
+    const int64_t m = row_blocks(), c = div_up(F, 16);
     return ws_align((size_t)(m * c) * saved_block_bytes(wide));
   }
 };
@@ -171,7 +182,7 @@ struct BackwardWs {
                                   store_partial_bytes(s.F, s.C, s.M, s.pair, 2),
                                   store_partial_bytes(s.M, s.C, s.F, 2 * s.pair, 1)});
     partial = static_cast<float*>(c.take(part));
-    colsum = static_cast<float*>(c.take((size_t)div_up(s.M, BM) * 4 * 2 * (size_t)s.F * 4));
+    colsum = static_cast<float*>(c.take((size_t)s.row_blocks() * 2 * (size_t)s.F * 4));
     rowsum = static_cast<float*>(c.take((size_t)kSumSlices * (size_t)s.C * 4));
     total = c.at;
   }
