@@ -19,7 +19,7 @@ size_t ffn_forward_workspace(const FfnProblem& p, bool save) {
 }
 size_t ffn_saved_bytes(const FfnProblem& p) {
   const ffn::Shape s(p);
-  return s.blocks_bytes() + s.operand_bytes(s.M, s.F);
+  return s.blocks_bytes() + s.panels_bytes();
 }
 size_t ffn_backward_workspace(const FfnProblem& p) {
   return ffn::BackwardWs(p, FfnTensors{}, nullptr, nullptr).total;

@@ -16,15 +16,26 @@
 // values a stage in either form, zero-filled past the tensors' ends, so no
 // size needs to be a multiple of anything.
 //
-// Warp roles (576 threads): warps 0-15 epilogue, warp 16 issues the MMAs, warp
+// The caller's matrices are row-major (128-byte-swizzled tiles).  The block's
+// own operands (hidden, dgate, dup) lie in panels of 8 columns: panel p holds
+// columns 8 p .. 8 p + 7 of all rows, 16 bytes a row.  The lanes of an epilogue
+// warp are rows, so they store 512 contiguous bytes an instruction from their
+// registers, where a row-major matrix needs staging and a TMA store whose rows
+// are 32 bytes (these row requests, beside the operands', held the TMA up: the
+// dhidden pass of 92416 x 2048 in bf16 took 440 us).  Eight rows
+// of a panel are 128 contiguous bytes, the matrix unit's 8 x 16-byte core
+// matrix without swizzle, read K-major or MN-major as a product needs it.
+//
+// Warp roles (640 threads): warps 0-15 epilogue, warp 16 issues the MMAs, warp
 // 17 the TMA loads.  A CTA works through its share of the output tiles; the
 // accumulator is double-buffered in TMEM, so a tile's epilogue runs under the
 // next tile's MMAs.  Epilogue warp w reads TMEM lanes 32 (w % 4) .. +31: lane i
-// owns one row, 16 columns at a time.  On 16-bit data warps 0-7 take the tiles
-// of the first accumulator buffer and warps 8-15 those of the second, so that
-// one half's stores go out while the other half computes: with all warps on
-// one tile their phases (TMEM reads, stores of gate and up, arithmetic, store
-// of the results) follow one another and their times add up.
+// owns one row, 16 columns at a time, and takes blocks w / 4, w / 4 + 4, ... of
+// the tile.  A block's sums are read while the one before is worked on, and the
+// buffer goes back to the MMAs once the last has been read: held to the end of
+// the epilogue, a buffer's products and its epilogue exclude each other, and a
+// tile takes half of their sum (8460 cycles where the products take 4100 and
+// the gated epilogue 5500, 23104 x 512 -> 2048 rows in bf16).
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along
@@ -67,7 +78,10 @@ constexpr int kActSilu = DCN_ACT_SILU, kActGelu = DCN_ACT_GELU, kActRelu = DCN_A
 
 constexpr int EPI_WARPS = 16;
 constexpr int MMA_WARP = EPI_WARPS, LOAD_WARP = EPI_WARPS + 1;
-constexpr int NTHREADS = (EPI_WARPS + 2) * 32;
+constexpr int NTHREADS = (EPI_WARPS + 4) * 32;  // whole warpgroups: two warps of the last idle
+// Registers: 640 threads start with 96 each (61,440); the epilogue warps take
+// what the last warpgroup gives up: 512 x 112 + 128 x 32 = 61,440.
+constexpr int kEpiRegs = 112, kOtherRegs = 32;
 constexpr int CB = 16;           // columns of an epilogue block
 constexpr uint32_t A_STAGE = BM * 128;
 constexpr int ST_FFN_LOAD = 61, ST_FFN_MMA = 62, ST_FFN_EPI = 63, ST_FFN_DRAIN = 64, ST_FFN_SMEM = 65;
@@ -77,36 +91,58 @@ enum Epi { EPI_GATED, EPI_DGATE, EPI_RECOMPUTE, EPI_STORE };
 // Accumulator columns are BN; EPI_RECOMPUTE has 3 x 64 (gate, up, dhidden) and
 // two row operands (x, dy).
 constexpr int kRecomputeCols = 64, kRecomputeBn = 3 * kRecomputeCols;
+// Output staging of an epilogue warp: STORE (16-bit) its columns of a tile for
+// one TMA store, DGATE and RECOMPUTE two blocks whose columns are summed.
+constexpr uint32_t kSumBlock = 32 * CB * 2;
+__host__ __device__ constexpr uint32_t staging_bytes(int epi, int bn, bool wide) {
+  return wide || epi == EPI_GATED ? 0u : epi == EPI_STORE ? 32u * (uint32_t)(bn / 4) * 2u : 2u * kSumBlock;
+}
 __host__ __device__ constexpr uint32_t stage_bytes(int bn, bool pair) {
   return (bn == kRecomputeBn ? 2 : 1) * A_STAGE + (uint32_t)bn * 128u / (pair ? 2u : 1u);
 }
-// as many stages as 192 KB hold, at most eight
-__host__ __device__ constexpr int stages(int bn, bool pair) {
-  return 196608 / stage_bytes(bn, pair) < 8 ? (int)(196608 / stage_bytes(bn, pair)) : 8;
-}
-// operand stages, then two staged output blocks and 32 bias values of each
-// epilogue warp, then barriers
-constexpr uint32_t kStageBlock = 32 * CB * 2;
-constexpr uint32_t kStaging = EPI_WARPS * 2 * kStageBlock;
-__host__ __device__ constexpr uint32_t smem_bytes(int bn, bool pair) {
-  return (uint32_t)stages(bn, pair) * stage_bytes(bn, pair) + kStaging + EPI_WARPS * 32 * 4u +
-         (2u * (uint32_t)stages(bn, pair) + 5u) * 8u + 16u;
-}
+constexpr uint32_t kBiasBytes = EPI_WARPS * 32 * 4u, kBarBytes = 256;
 // dynamic shared memory starts on 1024 bytes when a kernel has no static one;
 // this much is left over for a start that does not (checked by the kernel)
-constexpr uint32_t kSmemSlack = 768;
-static_assert(smem_bytes(256, false) + kSmemSlack <= 232448 && smem_bytes(256, true) + kSmemSlack <= 232448 &&
-                  smem_bytes(128, true) + kSmemSlack <= 232448,
-              "shared memory of one CTA");
+constexpr uint32_t kSmemSlack = 512;
+// as many stages as fit, at most eight
+__host__ __device__ constexpr int stages(int epi, int bn, bool pair, bool wide) {
+  const uint32_t n = (232448u - kSmemSlack - kBiasBytes - kBarBytes - EPI_WARPS * staging_bytes(epi, bn, wide)) /
+                     stage_bytes(bn, pair);
+  return n < 8 ? (int)n : 8;
+}
+__host__ __device__ constexpr uint32_t smem_bytes(int epi, int bn, bool pair, bool wide) {
+  return (uint32_t)stages(epi, bn, pair, wide) * stage_bytes(bn, pair) + EPI_WARPS * staging_bytes(epi, bn, wide) +
+         kBiasBytes + kBarBytes;
+}
 // fp32 data: K blocks added up in TMEM before their sum moves on to registers
 constexpr int kWideRun = 4;
+
+// n / d for 0 <= n < 2^31 by a multiplication: mul = ceil(2^(31 + s) / d) with
+// 2^s >= d, so the rounding adds less than n / 2^31 to the quotient times 2^s / d.
+struct FastDiv {
+  uint32_t mul, shift, d;
+  __host__ __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+#ifdef __CUDA_ARCH__
+    return d == 1 ? n : __umulhi(n, mul) >> shift;
+#else
+    return n / d;
+#endif
+  }
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  const uint64_t p = uint64_t(1) << (31 + s);
+  return {(uint32_t)((p + d - 1) / d), s ? s - 1 : 0, d};
+}
+constexpr int kGroupM = 8;
 
 struct Seg {
   uint8_t a_map, a_plane, b_map, b_plane;
 };
 struct Maps {
   CUtensorMap m[5];
-  CUtensorMap out[2];  // 16-bit results, 32 x 16 blocks
+  CUtensorMap out[2];  // STORE, 16-bit: 32 rows x a warp's columns
 };
 
 struct GemmArgs {
@@ -114,15 +150,16 @@ struct GemmArgs {
   int nk, nseg;              // K blocks of a segment, segments
   Seg seg[12];
   int tiles_m, tiles_n, batches;  // a batch adds its index to a_map (and picks the output)
-  int group_m;               // tiles are dealt in blocks of group_m row tiles x all column tiles
+  // tiles are dealt in blocks of kGroupM row tiles x all column tiles; divisors of tile_at
+  FastDiv per_batch, per_block, last_rows;
   int split;                 // 1: the last tiles are cut along K (Cut), partials to `partial`
   int act;
   uint32_t operand_bf16;
   float* partial;
-  // outputs: STORE: out[batch] [M][ldo] of T (+ bias); GATED: hidden; DGATE: dgate, dup.
+  // outputs: STORE: out[batch] [M][ldo] of T (+ bias); else panels of hidden, or dgate and dup:
+  // ldo rows a panel (M rounded up to 32), `plane` bytes between the bf16 planes of fp32 data
   void* out[2];
-  int64_t ldo;
-  int64_t plane;             // fp32: elements between the bf16 planes of hidden / dgate / dup
+  int64_t ldo, plane;
   int vec;                   // out rows take 16-byte stores (16-bit data: TMA stores)
   const void* bias[2];       // STORE: [0]; GATED, RECOMPUTE: gate, up
   void* saved;               // gate and up (private layout, below), or null
@@ -134,10 +171,11 @@ struct GemmArgs {
 // What the backward needs of a 32-row x 16-column block (its rows being the
 // lanes of one warp) lies together, each 16-byte piece of the 32 lanes side by
 // side, so both passes move whole lines:
-//   16-bit data: gate, up as fp16 times a power of two per (row, 16 columns)
-//     that puts the row's largest value near fp16's upper end: 11 bits, not
-//     bf16's 8, of values that the derivative multiplies, at the same size;
-//     then one int16 per lane with the two exponents;
+//   16-bit data: gate, up as fp16: 11 bits, not bf16's 8, of values that the
+//     derivative multiplies, at the same size.  Where a warp has a row whose
+//     largest value is outside [2^-4, 2^15), its values are multiplied by powers
+//     of two per (row, 16 columns) that bring the largest below 2^15.  One int16
+//     per lane holds the two exponents (14: as they are);
 //   fp32 data: gate, up as fp32.
 template <typename T>
 __host__ __device__ inline size_t saved_block_offset(int64_t m_block, int64_t col_block, int64_t col_blocks) {
@@ -168,6 +206,17 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Descriptor of an operand in panels: core matrices of 8 rows x 16 bytes without
+// swizzle; lbo, sbo as the operand's major asks (bytes).
+__device__ __forceinline__ uint64_t desc_panels(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
+  d |= (uint64_t)1 << 46;
+  return d;
+}
+
 // ---------------------------------------------------------------- CTA pairs
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -185,8 +234,14 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
+// Relaxed: what the arrival publishes is that TMEM has been read (tcgen05 fence
+// before it); a release would wait for all of the thread's stores to global
+// memory (2100 cycles a tile).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc_g(uint32_t slot, uint32_t ncols) {
@@ -242,18 +297,69 @@ __device__ __forceinline__ void load_g(uint32_t dst, const CUtensorMap* map, int
     tma_load_3d(dst, map, x, y, z, bar);
 }
 
+// The same for panels: boxes of 512-byte pieces (32 rows of a panel).
+template <bool PAIR>
+__device__ __forceinline__ void load_panels(uint32_t dst, const CUtensorMap* map, int row, int panel, int plane,
+                                            uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row >> 5), "r"(panel), "r"(plane), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row >> 5), "r"(panel), "r"(plane), "r"(bar)
+        : "memory");
+}
+
 // ---------------------------------------------------------------- activations
-// ACCURATE (fp32 data): CUDA's expf and IEEE division; else the fast forms,
-// whose few ulp are far below a 16-bit result's rounding.
+// ACCURATE (fp32 data): CUDA's expf, erff and IEEE division.  Else the matching
+// hardware approximations, whose few ulp are far below a 16-bit result's
+// rounding, with subnormals flushed (an exponential below 2^-126 is 0 here;
+// the forms that keep them cost four instructions more each).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
 template <bool ACCURATE>
 __device__ __forceinline__ float sigmoid(float x) {
-  // for x below -88 the exponential overflows to inf and the quotient is 0, as it should be
-  return ACCURATE ? 1.0f / (1.0f + expf(-x)) : __fdividef(1.0f, 1.0f + __expf(-x));
+  // far below zero the exponential overflows to inf and the quotient is 0, as it should be
+  return ACCURATE ? 1.0f / (1.0f + expf(-x)) : rcp_fast(1.0f + exp2_fast(-kLog2e * x));
+}
+// The normal distribution function and exp(-x^2 / 2).  Fast form: with z = |x|,
+// Phi(-z) = exp(-z^2 / 2) R(z), where R(z) = erfcx(z / sqrt 2) / 2 is smooth and
+// R ~ t (c0 + c1 t + ... + c5 t^5), t = 1 / (1 + 0.308 z): coefficients fitted
+// here for the least largest relative error, 4e-6 over z in [0, 14] (past that
+// the exponential is 0).  Both tails keep that relative error, and the
+// derivative needs the same exponential.
+template <bool ACCURATE>
+__device__ __forceinline__ float2 normal_cdf(float x) {
+  if (ACCURATE) return make_float2(0.5f * (1.0f + erff(x * 0.70710678118654752f)), expf(-0.5f * x * x));
+  const float z = fabsf(x);
+  const float t = rcp_fast(fmaf(0.308f, z, 1.0f));
+  const float e = exp2_fast((-0.5f * kLog2e) * (z * z));
+  float r = fmaf(t, -0.0754310913f, 0.189621131f);
+  r = fmaf(t, r, 0.00726954421f);
+  r = fmaf(t, r, 0.136535319f);
+  r = fmaf(t, r, 0.118880802f);
+  r = fmaf(t, r, 0.123122739f);
+  const float low = e * (t * r);
+  return make_float2(x > 0.0f ? 1.0f - low : low, e);
 }
 template <bool ACCURATE, int ACT>
 __device__ __forceinline__ float act_value(float x) {
   if constexpr (ACT == kActSilu) return x * sigmoid<ACCURATE>(x);
-  else if constexpr (ACT == kActGelu) return x * (0.5f * (1.0f + erff(x * 0.70710678118654752f)));
+  else if constexpr (ACT == kActGelu) return x * normal_cdf<ACCURATE>(x).x;
   else if constexpr (ACT == kActRelu) return x > 0.0f ? x : (x == x ? 0.0f : x);
   else return sigmoid<ACCURATE>(x);
 }
@@ -261,12 +367,11 @@ __device__ __forceinline__ float act_value(float x) {
 template <bool ACCURATE, int ACT>
 __device__ __forceinline__ float2 act_both(float x) {
   if constexpr (ACT == kActSilu) {
-    const float s = sigmoid<ACCURATE>(x);
-    return make_float2(x * s, s * (1.0f + x * (1.0f - s)));
+    const float s = sigmoid<ACCURATE>(x), a = x * s;
+    return make_float2(a, fmaf(a, 1.0f - s, s));
   } else if constexpr (ACT == kActGelu) {
-    const float c = 0.5f * (1.0f + erff(x * 0.70710678118654752f));
-    const float e = ACCURATE ? expf(-0.5f * x * x) : __expf(-0.5f * x * x);
-    return make_float2(x * c, c + x * (0.39894228040143268f * e));
+    const float2 c = normal_cdf<ACCURATE>(x);
+    return make_float2(x * c.x, fmaf(x, 0.39894228040143268f * c.y, c.x));
   } else if constexpr (ACT == kActRelu) {
     return x > 0.0f ? make_float2(x, 1.0f) : make_float2(x == x ? 0.0f : x, 0.0f);
   } else {
@@ -314,7 +419,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// values 8 j .. 8 j + 7 of a block, times s, as 16-bit
+// values 8 j .. 8 j + 7 of a block as 16-bit
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[CB], int j) {
+  uint4 p;
+  p.x = pack2(v[8 * j], v[8 * j + 1], (T*)nullptr);
+  p.y = pack2(v[8 * j + 2], v[8 * j + 3], (T*)nullptr);
+  p.z = pack2(v[8 * j + 4], v[8 * j + 5], (T*)nullptr);
+  p.w = pack2(v[8 * j + 6], v[8 * j + 7], (T*)nullptr);
+  return p;
+}
+// the same times s
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&v)[CB], int j, float s) {
   uint4 p;
@@ -337,7 +452,7 @@ __device__ __forceinline__ void store_row(T* row, int c0, int n, bool vec, const
     } else {
 #pragma unroll
       for (int j = 0; j < CB / 8; ++j)
-        if (c0 + 8 * j < n) *reinterpret_cast<uint4*>(row + c0 + 8 * j) = pack8<T>(v, j, 1.0f);
+        if (c0 + 8 * j < n) *reinterpret_cast<uint4*>(row + c0 + 8 * j) = pack8<T>(v, j);
     }
   } else {
 #pragma unroll
@@ -346,18 +461,21 @@ __device__ __forceinline__ void store_row(T* row, int c0, int n, bool vec, const
   }
 }
 
-// A 32 x 16 block of 16-bit values leaves through shared memory and one TMA
-// store per warp, whole 32-byte sectors at a time (row-owning lanes would
-// write 16 bytes to 32 different lines an instruction).  Staged rows are 32
-// bytes with the 32-byte swizzle: 16-byte piece j of row r at j ^ (r / 4 % 2),
-// so eight lanes cover all banks.  Rows and columns past the matrix are
-// dropped by the store.
-__device__ __forceinline__ uint32_t staged_piece(int row, int j) { return row * 32 + ((j ^ ((row >> 2) & 1)) << 4); }
-template <typename T>
-__device__ __forceinline__ void stage_row(uint8_t* block, int lane, const float (&v)[CB]) {
-#pragma unroll
-  for (int j = 0; j < CB / 8; ++j) *reinterpret_cast<uint4*>(block + staged_piece(lane, j)) = pack8<T>(v, j, 1.0f);
+// A block's two 16-byte pieces of a staged row of W bytes, with the swizzle of
+// that width (128, 64 or 32 bytes: piece j of row r at j ^ (r % 8), j ^ (r / 2 %
+// 4) or j ^ (r / 4 % 2)), so eight lanes cover all banks.
+template <int W>
+__device__ __forceinline__ uint32_t staged_piece(int row, int j) {
+  return row * W + ((W == 128 ? j ^ (row & 7) : W == 64 ? j ^ ((row >> 1) & 3) : j ^ ((row >> 2) & 1)) << 4);
 }
+template <typename T, int W>
+__device__ __forceinline__ void stage_row(uint8_t* rows, int lane, int block, const float (&v)[CB]) {
+#pragma unroll
+  for (int j = 0; j < CB / 8; ++j)
+    *reinterpret_cast<uint4*>(rows + staged_piece<W>(lane, 2 * block + j)) = pack8<T>(v, j);
+}
+// 32 rows of a warp's columns leave in one TMA store; rows and columns past the
+// matrix are dropped by it.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -365,31 +483,44 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
                : "memory");
 }
 
-// A block's columns of one row of fp32 values that are an operand of a
-// following product: three bf16 planes.  Rows are padded to 16 bytes (`ld`).
-__device__ __forceinline__ void store_planes(void* base, int64_t plane, int64_t row, int64_t ld, int c0,
+// A block's columns of one row, as an operand of a following product: two
+// panels' pieces (fp32 data: in each of three bf16 planes).  `at`: this row in
+// the first panel; columns at and past `left` are not in the matrix, their
+// panel is skipped (values inside a last panel are zero).
+template <typename T>
+__device__ __forceinline__ void store_panels(uint8_t* at, int64_t panel_bytes, int64_t plane, int left,
                                              const float (&v)[CB]) {
-  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + row * ld;
-  float r[CB];
+  if constexpr (sizeof(T) == 4) {
+    float r[CB];
 #pragma unroll
-  for (int j = 0; j < CB; ++j) r[j] = v[j];
+    for (int j = 0; j < CB; ++j) r[j] = v[j];
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    store_row<__nv_bfloat16>(p + k * plane, c0, (int)ld, true, r);
-    // a plane that holds inf or NaN ends the expansion: the others are zero
+    for (int k = 0; k < 3; ++k) {
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      const float hi = __bfloat162float(__float2bfloat16_rn(r[j]));
-      r[j] = fabsf(hi) <= 3.4e38f ? r[j] - hi : 0.0f;
+      for (int j = 0; j < CB / 8; ++j)
+        if (8 * j < left) *reinterpret_cast<uint4*>(at + k * plane + j * panel_bytes) = pack8<__nv_bfloat16>(r, j);
+      // a plane that holds inf or NaN ends the expansion: the others are zero
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        const float hi = __bfloat162float(__float2bfloat16_rn(r[j]));
+        r[j] = fabsf(hi) <= 3.4e38f ? r[j] - hi : 0.0f;
+      }
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CB / 8; ++j)
+      if (8 * j < left) *reinterpret_cast<uint4*>(at + j * panel_bytes) = pack8<T>(v, j);
   }
 }
 
 // ---------------------------------------------------------------- saved values
-__device__ __forceinline__ int scale_exponent(const float (&v)[CB]) {
+__device__ __forceinline__ float largest(const float (&v)[CB]) {
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < CB; ++j) top = fmaxf(top, fabsf(v[j]));
+  return top;
+}
+__device__ __forceinline__ int scale_exponent(const float (&v)[CB], float top) {
   if (!(top <= 3.4028235e38f)) {  // inf beside finite values: the scale is theirs
     top = 0.0f;
 #pragma unroll
@@ -411,12 +542,24 @@ __device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, const flo
           make_float4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
     }
   } else {
-    const int eg = scale_exponent(g), eu = scale_exponent(u);
-    const float sg = exp2_int(14 - eg), su = exp2_int(14 - eu);
+    const float tg = largest(g), tu = largest(u);
+    const bool fits = fminf(tg, tu) >= 0.0625f && fmaxf(tg, tu) < 32768.0f;
+    int eg = 14, eu = 14;
+    if (__all_sync(0xffffffffu, fits)) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      *reinterpret_cast<uint4*>(block + j * 512 + lane * 16) = pack8<__half>(g, j, sg);
-      *reinterpret_cast<uint4*>(block + 1024 + j * 512 + lane * 16) = pack8<__half>(u, j, su);
+      for (int j = 0; j < 2; ++j) {
+        *reinterpret_cast<uint4*>(block + j * 512 + lane * 16) = pack8<__half>(g, j);
+        *reinterpret_cast<uint4*>(block + 1024 + j * 512 + lane * 16) = pack8<__half>(u, j);
+      }
+    } else {
+      eg = scale_exponent(g, tg);
+      eu = scale_exponent(u, tu);
+      const float sg = exp2_int(14 - eg), su = exp2_int(14 - eu);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        *reinterpret_cast<uint4*>(block + j * 512 + lane * 16) = pack8<__half>(g, j, sg);
+        *reinterpret_cast<uint4*>(block + 1024 + j * 512 + lane * 16) = pack8<__half>(u, j, su);
+      }
     }
     reinterpret_cast<uint16_t*>(block + 2048)[lane] = (uint16_t)((eg & 0xff) | (eu & 0xff) << 8);
   }
@@ -445,8 +588,6 @@ struct SavedRaw {
         u[4 * j + 2] = __uint_as_float(b[j].z); u[4 * j + 3] = __uint_as_float(b[j].w);
       }
     } else {
-      // the exponents as signed bytes; -100 and up, so 2^(e - 14) is a normal number
-      const float sg = exp2_int((int)(int8_t)(e & 0xff) - 14), su = exp2_int((int)(int8_t)(e >> 8) - 14);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t aw[4] = {a[j].x, a[j].y, a[j].z, a[j].w}, bw[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
@@ -454,8 +595,17 @@ struct SavedRaw {
         for (int k = 0; k < 4; ++k) {
           const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&aw[k]));
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&bw[k]));
-          g[8 * j + 2 * k] = x.x * sg; g[8 * j + 2 * k + 1] = x.y * sg;
-          u[8 * j + 2 * k] = y.x * su; u[8 * j + 2 * k + 1] = y.y * su;
+          g[8 * j + 2 * k] = x.x; g[8 * j + 2 * k + 1] = x.y;
+          u[8 * j + 2 * k] = y.x; u[8 * j + 2 * k + 1] = y.y;
+        }
+      }
+      if (!__all_sync(0xffffffffu, e == (14 | 14 << 8))) {
+        // the exponents as signed bytes; -100 and up, so 2^(e - 14) is a normal number
+        const float sg = exp2_int((int)(int8_t)(e & 0xff) - 14), su = exp2_int((int)(int8_t)(e >> 8) - 14);
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          g[j] *= sg;
+          u[j] *= su;
         }
       }
     }
@@ -476,7 +626,7 @@ __device__ __forceinline__ void staged_column_sums(uint32_t block, int lane, flo
     uint32_t r[4];  // rows 8 i .. 8 i + 7 of eight columns, transposed: pairs of rows a lane
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(block + staged_piece(lane, j))
+                 : "r"(block + staged_piece<32>(lane, j))
                  : "memory");
     float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -589,25 +739,37 @@ struct Work {
   }
 };
 
-// Tile index -> (batch, row tile, column tile): blocks of group_m row tiles,
+// Tile index -> (batch, row tile, column tile): blocks of kGroupM row tiles,
 // row tiles fastest inside a block, so the CTAs of a wave share both operands
 // in the L2.
-__device__ __forceinline__ void tile_at(const GemmArgs& a, int tile, int& z, int& mt, int& nt) {
-  const int per = a.tiles_m * a.tiles_n;
-  z = tile / per;
-  int t = tile - z * per;
-  const int block = t / (a.group_m * a.tiles_n);
-  const int rows = min(a.group_m, a.tiles_m - block * a.group_m);
-  t -= block * a.group_m * a.tiles_n;
-  nt = t / rows;
-  mt = block * a.group_m + (t - nt * rows);
+__host__ __device__ __forceinline__ void tile_at(const GemmArgs& a, int tile, int& z, int& mt, int& nt) {
+  z = (int)a.per_batch((uint32_t)tile);
+  int t = tile - z * (a.tiles_m * a.tiles_n);
+  const int block = (int)a.per_block((uint32_t)t);
+  t -= block * (kGroupM * a.tiles_n);
+  const bool last = (block + 1) * kGroupM > a.tiles_m;
+  nt = last ? (int)a.last_rows((uint32_t)t) : t / kGroupM;
+  mt = block * kGroupM + t - nt * (last ? a.tiles_m - block * kGroupM : kGroupM);
+}
+inline void set_tiles(GemmArgs& a, int tiles_m, int tiles_n, int batches) {
+  a.tiles_m = tiles_m;
+  a.tiles_n = tiles_n;
+  a.batches = batches;
+  a.per_batch = fast_div((uint32_t)(tiles_m * tiles_n));
+  a.per_block = fast_div((uint32_t)(kGroupM * tiles_n));
+  a.last_rows = fast_div((uint32_t)(tiles_m % kGroupM ? tiles_m % kGroupM : kGroupM));
 }
 
 // ---------------------------------------------------------------- kernel
-template <typename T, int EPI, int BN, bool A_MN, bool B_MN, bool PAIR>
+// A, B: the operand's form.
+enum Form { ROWS_K, ROWS_MN, PANELS_K, PANELS_MN };
+
+template <typename T, int EPI, int BN, Form A, Form B, bool PAIR>
 __global__ void __launch_bounds__(NTHREADS, 1)
 ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs a) {
-  constexpr int S = stages(BN, PAIR);
+  constexpr bool A_MN = A == ROWS_MN || A == PANELS_MN, B_MN = B == ROWS_MN || B == PANELS_MN;
+  constexpr int S = stages(EPI, BN, PAIR, sizeof(T) == 4);
+  constexpr uint32_t STAGING = staging_bytes(EPI, BN, sizeof(T) == 4);  // of a warp
   constexpr uint32_t STAGE = stage_bytes(BN, PAIR);
   constexpr bool GATED = EPI == EPI_GATED, RECOMP = EPI == EPI_RECOMPUTE, TWO = GATED || RECOMP;
   constexpr bool DGATE = EPI == EPI_DGATE || RECOMP;
@@ -625,14 +787,12 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   static_assert(!WIDE || BN <= 128 || RECOMP, "an epilogue thread holds 32 to 48 sums");
   static_assert(RECOMP == (BN == kRecomputeBn), "accumulator columns");
   static_assert(!PAIR || !RECOMP, "half of 64 dhidden columns fills no swizzled row");
-  // epilogue warps that share a tile; fp32 sums stay with their warps over the
-  // runs of a tile, which alternate between the buffers
-  constexpr int GROUP = WIDE ? EPI_WARPS : EPI_WARPS / 2, STEP = GROUP / 4;
+  constexpr int STEP = EPI_WARPS / 4;  // warps that share 32 rows of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
   uint8_t* staging = smem + S * STAGE;
-  uint8_t* tail = staging + kStaging + EPI_WARPS * 32 * 4;
+  uint8_t* tail = staging + EPI_WARPS * STAGING + kBiasBytes;
   if (smem - smem_raw > kSmemSlack) {  // an unexpected start (the same in both CTAs): nothing is touched
     if (threadIdx.x == 0) atomicExch(a.status, ST_FFN_SMEM);
     return;
@@ -657,7 +817,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), GROUP * CTAS);
+      mbar_init(acc_empty(b), EPI_WARPS * CTAS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -672,6 +832,8 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
 
   Work w(a, blockIdx.x / CTAS, gridDim.x / CTAS);
 
+  if (warp >= EPI_WARPS) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == LOAD_WARP) {
     // ------------------------------------------------ TMA loads
     if (lane == 0) {
@@ -694,7 +856,11 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           const CUtensorMap* ma = &maps.m[seg.a_map + z];
           const CUtensorMap* mb = &maps.m[seg.b_map];
           if (rank == 0) mbar_arrive_expect_tx(full(s), CTAS * STAGE);
-          if (A_MN) {
+          if (A == PANELS_MN) {
+            load_panels<PAIR>(dst, ma, k, m0 >> 3, seg.a_plane, bar);
+          } else if (A == PANELS_K) {
+            load_panels<PAIR>(dst, ma, m0, k >> 3, seg.a_plane, bar);
+          } else if (A == ROWS_MN) {
             load_g<PAIR>(dst, ma, m0, k, seg.a_plane, bar);
             load_g<PAIR>(dst + 8192, ma, m0 + 64, k, seg.a_plane, bar);
           } else {
@@ -709,7 +875,9 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
               tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, bar);
               tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, bar);
             }
-          } else if (B_MN) {
+          } else if (B == PANELS_MN) {
+            load_panels<PAIR>(dst + A_STAGE, mb, k, nb >> 3, seg.b_plane, bar);
+          } else if (B == ROWS_MN) {
 #pragma unroll
             for (int q = 0; q < BN / 64 / CTAS; ++q)
               load_g<PAIR>(dst + A_STAGE + q * 8192, mb, nb + 64 * q, k, seg.b_plane, bar);
@@ -751,8 +919,16 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
             const uint32_t ab = sbase + s * STAGE, bb = ab + B_AT;
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              const uint64_t ad = A_MN ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192) : desc_kmajor_sw128(ab + kk * 32);
-              const uint64_t bd = B_MN ? tcc::desc_mnmajor_sw128(bb + kk * 2048, 8192) : desc_kmajor_sw128(bb + kk * 32);
+              // panels in shared memory: K-major [panel][128 rows][16 B] (panels along K by
+              // LBO, 8-row groups by SBO); MN-major [panel][64 rows][16 B] (8-row groups along
+              // K by LBO, panels by SBO)
+              const uint64_t ad = A == PANELS_K    ? desc_panels(ab + kk * 4096, 2048, 128)
+                                  : A == PANELS_MN ? desc_panels(ab + kk * 256, 128, 1024)
+                                  : A == ROWS_MN   ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192)
+                                                   : desc_kmajor_sw128(ab + kk * 32);
+              const uint64_t bd = B == PANELS_MN ? desc_panels(bb + kk * 256, 128, 1024)
+                                  : B == ROWS_MN ? tcc::desc_mnmajor_sw128(bb + kk * 2048, 8192)
+                                                 : desc_kmajor_sw128(bb + kk * 32);
               mma_g<PAIR>(d, ad, bd, idesc, (i > k0 || kk > 0) ? 1u : 0u);
               if (RECOMP)
                 mma_f16(d + 2 * COLS, desc_kmajor_sw128(ab + A_STAGE + kk * 32),
@@ -773,14 +949,21 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         mbar_wait(drain, 0, abort_flag, a.status, ST_FFN_DRAIN);
       }
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     // ------------------------------------------------ epilogue
-    // lanes 32 q .., column blocks first, first + STEP, ... of the tiles of its group
-    const int q = warp & 3, first = (warp % GROUP) >> 2, group = warp / GROUP;
+    const int q = warp & 3;  // lanes 32 q ..
+    // of the tile's column blocks: STORE a run of its own, else first, first + STEP, ...
     constexpr int BLOCKS = COLS / CB;
+    constexpr bool RUNS = EPI == EPI_STORE && !WIDE;
+    constexpr int MINE = BLOCKS / STEP > 0 ? BLOCKS / STEP : 1;  // blocks of a warp (BLOCKS = 2: of two warps in four)
+    const int first = RUNS ? (warp >> 2) * MINE : warp >> 2;
+    constexpr int NEXT = RUNS ? 1 : STEP;
+    const int end = RUNS ? first + MINE : BLOCKS;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-    uint8_t* stage = staging + warp * (2 * kStageBlock);
-    float* colf = reinterpret_cast<float*>(staging + kStaging) + warp * 32;
+    uint8_t* stage = staging + warp * STAGING;
+    float* colf = reinterpret_cast<float*>(staging + EPI_WARPS * STAGING) + warp * 32;
     const bool has_bias = EPI != EPI_DGATE && a.bias[0] != nullptr;
     const int64_t col_blocks = (a.N + CB - 1) / CB;
     // The bias values of a block, one a lane (RECOMPUTE, GATED: 16 of gate, 16
@@ -788,25 +971,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     // piece of shared memory.
     auto bias_of = [&](int c0) {
       const int k = lane >> 4, c = c0 + (lane & 15);
-      return (k == 0 || TWO) && c < a.N ? to_f<T>(static_cast<const T*>(a.bias[k])[c]) : 0.0f;
-    };
-    // this warp's staged blocks, out through the TMA
-    auto store_staged = [&](int blocks, int x, int y, int map) {
-      if (lane == 0 && y < a.M) {
-        for (int k = 0; k < blocks; ++k)
-          tma_store_3d(&maps.out[map + k], smem_addr(stage + k * kStageBlock), x, y, 0);
-        bulk_commit();
-      }
-    };
-    // staged blocks may be written again once the store has read them
-    auto staging_free = [&] {
-      if (lane == 0) bulk_wait_read_all();
-      __syncwarp();
-    };
-    // this lane's writes to the staged blocks reach the TMA and the other lanes
-    auto staging_done = [&] {
-      fence_async_shared();
-      __syncwarp();
+      return (k == 0 || TWO) && c < a.N ? static_cast<const T*>(a.bias[k])[c] : from_f<T>(0.0f);
     };
     int done = 0;
     bool ok = true;
@@ -821,15 +986,11 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       __syncwarp();
       if (lane == 0) {
         if (PAIR) mbar_arrive_cluster(in_first_cta(acc_empty(done & 1)));
-        else mbar_arrive(acc_empty(done & 1));
+        else mbar_arrive_relaxed(acc_empty(done & 1));
       }
       ++done;
     };
     while (ok && w.next(a)) {
-      if (!WIDE && (done & 1) != group) {  // the other warps' tile
-        ++done;
-        continue;
-      }
       int z, mt, nt;
       tile_at(a, w.tile, z, mt, nt);
       const int n0 = nt * COLS;
@@ -844,7 +1005,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
 
       // One block of this tile.  v: its sums (GATED, RECOMPUTE: gate); u: up (from
       // TMEM or, DGATE, the saved state with gate in v's place); dh: dhidden.
-      auto block = [&](int c, float (&v)[CB], float (&u)[CB], float (&dh)[CB], float bias) {
+      auto block = [&](int c, float (&v)[CB], float (&u)[CB], float (&dh)[CB], T bias) {
         const int c0 = n0 + c * CB;
         if (!whole) {
           // an fp32 partial of this tile, 16-byte pieces of 32 rows side by side
@@ -858,64 +1019,65 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         if (c0 >= a.N) return;
         if (has_bias) {
           __syncwarp();
-          colf[lane] = bias;
+          colf[lane] = to_f<T>(bias);
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < CB; ++j) {
-            v[j] += colf[j];
-            if (TWO) u[j] += colf[CB + j];
+          for (int j = 0; j < CB / 4; ++j) {
+            const float4 f = reinterpret_cast<const float4*>(colf)[j];
+            v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+            if (TWO) {
+              const float4 h = reinterpret_cast<const float4*>(colf + CB)[j];
+              u[4 * j] += h.x; u[4 * j + 1] += h.y; u[4 * j + 2] += h.z; u[4 * j + 3] += h.w;
+            }
           }
         }
+        // this row in the panels of the block's columns
+        const int64_t panel = a.ldo * 16;
+        const int64_t at = (int64_t)(c0 >> 3) * panel + row * 16;
         if constexpr (GATED) {
           if (a.saved) save_gate_up<T>(saved_block(c), lane, v, u);
-          float h[CB];
-          gate_block<WIDE>(a.act, v, u, h);
-          if constexpr (WIDE) {
-            if (row_in) store_planes(a.out[0], a.plane, row, a.ldo, c0, h);
-          } else {
-            staging_free();
-            stage_row<T>(stage, lane, h);
-            staging_done();
-            store_staged(1, c0, row0, 0);
+          gate_block<WIDE>(a.act, v, u, v);
+          if (row0 + 32 > a.M && !row_in) {  // rows past M are zero in the panels
+#pragma unroll
+            for (int j = 0; j < CB; ++j) v[j] = 0.0f;
           }
+          if (row0 < a.M) store_panels<T>(static_cast<uint8_t*>(a.out[0]) + at, panel, a.plane, a.N - c0, v);
         } else if constexpr (DGATE) {
           dgate_block<WIDE>(a.act, dh, v, u);
-          if (!row_in) {  // rows past M count in no column sum
+          if (row0 + 32 > a.M && !row_in) {
 #pragma unroll
             for (int j = 0; j < CB; ++j) v[j] = u[j] = 0.0f;
           }
-          float* sums = a.colsum ? a.colsum + (m_block * 2) * a.N : nullptr;
-          if constexpr (WIDE) {
-            if (row_in) {
-              store_planes(a.out[0], a.plane, row, a.ldo, c0, v);
-              store_planes(a.out[1], a.plane, row, a.ldo, c0, u);
-            }
-            if (sums) {
+          if (row0 < a.M) {
+            store_panels<T>(static_cast<uint8_t*>(a.out[0]) + at, panel, a.plane, a.N - c0, v);
+            store_panels<T>(static_cast<uint8_t*>(a.out[1]) + at, panel, a.plane, a.N - c0, u);
+          }
+          if (a.colsum) {
+            float* sums = a.colsum + (m_block * 2) * a.N;
+            if constexpr (WIDE) {
               const float sg = column_sum(v, lane), su = column_sum(u, lane);
               if (lane < CB && c0 + lane < a.N) {
                 sums[c0 + lane] = sg;
                 sums[a.N + c0 + lane] = su;
               }
-            }
-          } else {
-            staging_free();
-            stage_row<T>(stage, lane, v);
-            stage_row<T>(stage + kStageBlock, lane, u);
-            staging_done();
-            store_staged(2, c0, row0, 0);
-            if (sums) {
-              staged_column_sums<T>(smem_addr(stage), lane, sums, c0, a.N);
-              staged_column_sums<T>(smem_addr(stage + kStageBlock), lane, sums + a.N, c0, a.N);
+            } else {
               __syncwarp();
+              stage_row<T, 32>(stage, lane, 0, v);
+              stage_row<T, 32>(stage + kSumBlock, lane, 0, u);
+              __syncwarp();
+              staged_column_sums<T>(smem_addr(stage), lane, sums, c0, a.N);
+              staged_column_sums<T>(smem_addr(stage + kSumBlock), lane, sums + a.N, c0, a.N);
             }
           }
         } else {
           if (!WIDE && a.vec) {
             if constexpr (!WIDE) {
-              staging_free();
-              stage_row<T>(stage, lane, v);
-              staging_done();
-              store_staged(1, c0, row0, z);
+              // the last tile's store has read the staged rows
+              if (c == first) {
+                if (lane == 0) bulk_wait_read_all();
+                __syncwarp();
+              }
+              stage_row<T, BN / 2>(stage, lane, c - first, v);
             }
           } else if (row_in) {
             store_row<T>(static_cast<T*>(a.out[z]) + row * a.ldo, c0, a.N, a.vec != 0, v);
@@ -926,7 +1088,8 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       // what the first block needs from memory is fetched while the products
       // run, the next ones' a block ahead
       const bool use_bias = has_bias && whole;
-      float bias = use_bias ? bias_of(n0 + first * CB) : 0.0f;
+      T bias = from_f<T>(0.0f);
+      if (use_bias) bias = bias_of(n0 + first * CB);
       SavedRaw<T> raw;
       if (EPI == EPI_DGATE && first < BLOCKS && n0 + first * CB < a.N) raw.load(saved_block(first), lane);
       if constexpr (WIDE) {
@@ -987,28 +1150,55 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       } else {
         if (!wait_acc()) break;
         const uint32_t acc = lanes + (uint32_t)((done & 1) * ACC);
+        // v: gate or plain sums or (DGATE) dhidden; u: up; dh: RECOMPUTE's dhidden
+        auto read = [&](int c, float (&v)[CB], float (&u)[CB], float (&dh)[CB]) {
+          tmem_load(acc + c * CB, v);
+          if (TWO) tmem_load(acc + COLS + c * CB, u);
+          if (RECOMP) tmem_load(acc + 2 * COLS + c * CB, dh);
+          tmem_wait(v);
+          if (TWO) tmem_wait(u);
+          if (RECOMP) tmem_wait(dh);
+        };
+        float v[CB], u[CB], dh[CB];
+        if (first < end) read(first, v, u, dh);
+        if (first + NEXT >= end) release_acc();
 #pragma unroll 1
-        for (int c = first; c < BLOCKS; c += STEP) {
-          float v[CB], u[CB], dh[CB];
-          const bool more = c + STEP < BLOCKS && n0 + (c + STEP) * CB < a.N;
-          const float now = bias;
-          if constexpr (EPI == EPI_DGATE) {
-            tmem_load(acc + c * CB, dh);
-            raw.decode(v, u);
-            if (more) raw.load(saved_block(c + STEP), lane);
-            tmem_wait(dh);
-          } else {
-            tmem_load(acc + c * CB, v);
-            if (TWO) tmem_load(acc + COLS + c * CB, u);
-            if (RECOMP) tmem_load(acc + 2 * COLS + c * CB, dh);
-            tmem_wait(v);
-            if (TWO) tmem_wait(u);
-            if (RECOMP) tmem_wait(dh);
+        for (int c = first; c < end; c += NEXT) {
+          const bool more = c + NEXT < end;
+          const T now = bias;
+          float nv[CB], nu[CB], ndh[CB];
+          if (more) {
+            read(c + NEXT, nv, nu, ndh);
+            if (c + 2 * NEXT >= end) release_acc();
           }
-          if (more && use_bias) bias = bias_of(n0 + (c + STEP) * CB);
-          block(c, v, u, dh, now);
+          const bool inside = more && n0 + (c + NEXT) * CB < a.N;
+          if (inside && use_bias) bias = bias_of(n0 + (c + NEXT) * CB);
+          if constexpr (EPI == EPI_DGATE) {
+            float g[CB], up[CB];
+            raw.decode(g, up);
+            if (inside) raw.load(saved_block(c + NEXT), lane);
+            block(c, g, up, v, now);
+          } else {
+            block(c, v, u, dh, now);
+          }
+#pragma unroll
+          for (int j = 0; j < CB; ++j) {
+            v[j] = nv[j];
+            if (TWO) u[j] = nu[j];
+            if (RECOMP) dh[j] = ndh[j];
+          }
         }
-        release_acc();
+        if constexpr (RUNS) {
+          // the staged columns leave; the writes reach the TMA first
+          if (whole && a.vec && n0 + first * CB < a.N) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && row0 < a.M) {
+              tma_store_3d(&maps.out[z], smem_addr(stage), n0 + first * CB, row0, 0);
+              bulk_commit();
+            }
+          }
+        }
       }
     }
     // the stores have left shared memory and are done before the CTA ends

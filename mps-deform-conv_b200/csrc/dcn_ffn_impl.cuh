@@ -25,14 +25,15 @@ using namespace ffn;
 namespace {
 
 // ---------------------------------------------------------------- operands
-bool make_map(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_rows) {
-  return make_tmap_3d(map, o.base, bf16, (uint64_t)o.planes, (uint64_t)o.rows, (uint64_t)o.cols, (uint64_t)o.ld,
-                      (uint64_t)o.plane, box_rows, BK);
-}
-
-// 32 x 16 blocks of a 16-bit result, staged with the 32-byte swizzle.
-bool make_store_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
-  return make_tmap_3d(map, base, bf16, 1, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint64_t)(rows * ld), 32, CB);
+// `box`: rows (K-major) of the operand in a stage, or its columns (panels,
+// MN-major); row-major MN-major operands come in 64-column boxes.
+bool make_map(CUtensorMap* map, const Operand& o, bool bf16, Form form, uint32_t box) {
+  switch (form) {
+    case ROWS_K: return make_tmap_rows(map, o.base, bf16, o.planes, o.rows, o.cols, o.ld, o.plane, box, BK, 128);
+    case ROWS_MN: return make_tmap_rows(map, o.base, bf16, o.planes, o.rows, o.cols, o.ld, o.plane, BK, 64, 128);
+    case PANELS_K: return make_tmap_panels(map, o.base, bf16, o.planes, round_up(o.rows, 32), div_up(o.cols, 8), box, BK / 8);
+    default: return make_tmap_panels(map, o.base, bf16, o.planes, round_up(o.rows, 32), div_up(o.cols, 8), BK, box / 8);
+  }
 }
 
 // ---------------------------------------------------------------- packing
@@ -116,7 +117,8 @@ struct ReduceArgs {
   void* out[2];
   const void* bias;
   int64_t ldo;
-  int M, N, tiles_m, tiles_n, group_m, nkb, workers, base, tiles, ctas, vec;
+  int M, N, nkb, workers, base, tiles, ctas, vec;
+  GemmArgs g;  // for tile_at
 };
 
 template <typename T, int BN>
@@ -126,10 +128,8 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = blockIdx.x / blocks, blk = blockIdx.x - t * blocks;
   const int q = blk % quarters, c = blk / quarters;
-  GemmArgs g;
-  g.tiles_m = a.tiles_m; g.tiles_n = a.tiles_n; g.group_m = a.group_m;
   int z, mt, nt;
-  tile_at(g, a.base + t, z, mt, nt);
+  tile_at(a.g, a.base + t, z, mt, nt);
   const int64_t row = (int64_t)mt * BM * a.ctas + q * 32 + lane;
   const int c0 = nt * BN + c * 32;
   if (row - lane >= a.M || c0 >= a.N) return;
@@ -244,10 +244,10 @@ __global__ void __launch_bounds__(1024) ffn_column_finish_kernel(const float* __
   }
 }
 
-template <typename T, int EPI, int BN, bool A_MN, bool B_MN, bool PAIR>
+template <typename T, int EPI, int BN, Form A, Form B, bool PAIR>
 cudaError_t launch_gemm(const char* name, const Maps& maps, const GemmArgs& a, int workers, cudaStream_t st) {
-  auto kern = ffn_gemm_kernel<T, EPI, BN, A_MN, B_MN, PAIR>;
-  const int smem = (int)(smem_bytes(BN, PAIR) + kSmemSlack);
+  auto kern = ffn_gemm_kernel<T, EPI, BN, A, B, PAIR>;
+  const int smem = (int)(smem_bytes(EPI, BN, PAIR, sizeof(T) == 4) + kSmemSlack);
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -266,16 +266,16 @@ cudaError_t launch_gemm(const char* name, const Maps& maps, const GemmArgs& a, i
   return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 
-template <typename T, int EPI, bool A_MN, bool B_MN>
+template <typename T, int EPI, Form A, Form B>
 cudaError_t launch_gemm(const char* name, const GemmPlan& p, const Maps& maps, const GemmArgs& a, cudaStream_t st) {
   // pairs have the widest tile of their type, 256 columns or 128 (fp32)
-  if (p.pair) return launch_gemm<T, EPI, sizeof(T) == 4 ? 128 : 256, A_MN, B_MN, true>(name, maps, a, p.workers, st);
+  if (p.pair) return launch_gemm<T, EPI, sizeof(T) == 4 ? 128 : 256, A, B, true>(name, maps, a, p.workers, st);
   switch (p.bn) {
     case 256:
-      if constexpr (sizeof(T) == 2) return launch_gemm<T, EPI, 256, A_MN, B_MN, false>(name, maps, a, p.workers, st);
+      if constexpr (sizeof(T) == 2) return launch_gemm<T, EPI, 256, A, B, false>(name, maps, a, p.workers, st);
       return cudaErrorInvalidValue;  // fp32 plans stop at 128
-    case 128: return launch_gemm<T, EPI, 128, A_MN, B_MN, false>(name, maps, a, p.workers, st);
-    default: return launch_gemm<T, EPI, 64, A_MN, B_MN, false>(name, maps, a, p.workers, st);
+    case 128: return launch_gemm<T, EPI, 128, A, B, false>(name, maps, a, p.workers, st);
+    default: return launch_gemm<T, EPI, 64, A, B, false>(name, maps, a, p.workers, st);
   }
 }
 
@@ -299,7 +299,7 @@ constexpr bool operand_bf16() { return !std::is_same<T, __half>::value; }
 // A product with plain sums as its result: out[z] = sum of the segments (+ bias).
 // a[z], z < batches: the row operands (one batch), or with one batch the row
 // operands of the pairs; b: the column operands of the pairs.
-template <typename T, bool A_MN, bool B_MN>
+template <typename T, Form A, Form B>
 cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, const std::vector<Operand>& b_ops,
                           int64_t M, int64_t N, int64_t K, int batches, void* const* out, int64_t ldo,
                           const void* bias, float* partial, cudaStream_t st) {
@@ -314,11 +314,11 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   a.nk = (int)div_up(K, BK);
   const GemmPlan p = plan_gemm(M, N, (int64_t)a.nk * a.nseg, batches, false, true, sizeof(T) == 4);
   for (int i = 0; i < n_a; ++i)
-    if (!make_map(&maps.m[i], a_ops[i], operand_bf16<T>(), A_MN ? BK : BM)) return cudaErrorInvalidValue;
+    if (!make_map(&maps.m[i], a_ops[i], operand_bf16<T>(), A, BM)) return cudaErrorInvalidValue;
   for (int i = 0; i < pairs; ++i)
-    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B_MN ? BK : p.pair ? p.bn / 2 : p.bn)) return cudaErrorInvalidValue;
-  a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n; a.batches = batches;
-  a.group_m = 8;
+    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B, (uint32_t)(p.pair ? p.bn / 2 : p.bn)))
+      return cudaErrorInvalidValue;
+  set_tiles(a, p.tiles_m, p.tiles_n, batches);
   a.split = p.split;
   a.operand_bf16 = operand_bf16<T>();
   a.partial = partial;
@@ -329,17 +329,18 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   for (int z = 0; z < batches; ++z) a.vec = a.vec && (reinterpret_cast<uintptr_t>(out[z]) & 15) == 0;
   if (sizeof(T) == 2 && a.vec)
     for (int z = 0; z < batches; ++z)
-      if (!make_store_map(&maps.out[z], out[z], operand_bf16<T>(), M, N, ldo)) return cudaErrorInvalidValue;
+      if (!make_tmap_rows(&maps.out[z], out[z], operand_bf16<T>(), 1, M, N, ldo, M * ldo, 32, (uint32_t)(p.bn / 4), p.bn / 2))
+        return cudaErrorInvalidValue;
   a.bias[0] = bias;
   cudaError_t e = tc_status_ptr(&a.status);
   if (e != cudaSuccess) return e;
-  if ((e = launch_gemm<T, EPI_STORE, A_MN, B_MN>(name, p, maps, a, st)) != cudaSuccess || !p.split) return e;
+  if ((e = launch_gemm<T, EPI_STORE, A, B>(name, p, maps, a, st)) != cudaSuccess || !p.split) return e;
   ReduceArgs r{};
   r.partial = partial;
   r.out[0] = a.out[0]; r.out[1] = a.out[1];
   r.bias = bias;
   r.ldo = ldo;
-  r.M = a.M; r.N = a.N; r.tiles_m = p.tiles_m; r.tiles_n = p.tiles_n; r.group_m = a.group_m;
+  r.M = a.M; r.N = a.N; r.g = a;
   r.nkb = a.nk * a.nseg; r.workers = p.workers; r.vec = a.vec;
   const int tiles = p.tiles_m * p.tiles_n * batches;
   r.base = tiles / p.workers * p.workers;
@@ -374,23 +375,21 @@ cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* s
   a.M = (int)s.M; a.N = (int)s.F;
   a.nk = (int)div_up(s.C, BK);
   const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, true, false, sizeof(T) == 4);
-  if (!make_map(&maps.m[0], w.x, operand_bf16<T>(), BM) || !make_map(&maps.m[1], w.wg, operand_bf16<T>(), plan.bn / 2) ||
-      !make_map(&maps.m[2], w.wu, operand_bf16<T>(), plan.bn / 2))
+  if (!make_map(&maps.m[0], w.x, operand_bf16<T>(), ROWS_K, BM) ||
+      !make_map(&maps.m[1], w.wg, operand_bf16<T>(), ROWS_K, (uint32_t)plan.bn / 2) ||
+      !make_map(&maps.m[2], w.wu, operand_bf16<T>(), ROWS_K, (uint32_t)plan.bn / 2))
     return cudaErrorInvalidValue;
-  a.tiles_m = plan.tiles_m; a.tiles_n = plan.tiles_n; a.batches = 1;
-  a.group_m = 8;
+  set_tiles(a, plan.tiles_m, plan.tiles_n, 1);
   a.act = p.act;
   a.operand_bf16 = operand_bf16<T>();
   a.out[0] = const_cast<void*>(w.h.base);
-  a.ldo = w.h.ld;
-  a.plane = w.h.plane;
+  a.ldo = round_up(s.M, 32);
+  a.plane = s.panel_plane_bytes();
   a.bias[0] = t.b_gate; a.bias[1] = t.b_up;
   a.saved = s.recompute() ? nullptr : saved;
-  if (sizeof(T) == 2 && !make_store_map(&maps.out[0], w.h.base, operand_bf16<T>(), s.M, s.F, w.h.ld))
-    return cudaErrorInvalidValue;
   if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
-  if ((e = launch_gemm<T, EPI_GATED, false, false>("ffn_gate_up", plan, maps, a, st)) != cudaSuccess || !y) return e;
-  return store_product<T, false, false>("ffn_down", {w.h}, {w.wd}, s.M, s.C, s.F, 1, &y, s.C, t.b_down, w.partial, st);
+  if ((e = launch_gemm<T, EPI_GATED, ROWS_K, ROWS_K>("ffn_gate_up", plan, maps, a, st)) != cudaSuccess || !y) return e;
+  return store_product<T, PANELS_K, ROWS_K>("ffn_down", {w.h}, {w.wd}, s.M, s.C, s.F, 1, &y, s.C, t.b_down, w.partial, st);
 }
 
 template <typename T>
@@ -398,7 +397,7 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
                        void* ws, cudaStream_t st, dcn_params_ready_fn ready, void* user) {
   const Shape s(p);
   const BackwardWs w(p, t, dy, ws);
-  const Operand h = s.operand(static_cast<const uint8_t*>(saved) + s.blocks_bytes(), s.M, s.F);
+  const Operand h = s.operand(static_cast<const uint8_t*>(saved) + s.blocks_bytes(), s.M, s.F);  // panels
   Packer pk;
   if (w.pack_c) {
     pk.add(w.x, t.x);
@@ -425,29 +424,25 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
       plan.tiles_m = (int)div_up(s.M, BM);
       plan.tiles_n = (int)div_up(s.F, kRecomputeCols);
       plan.workers = (int)std::min<int64_t>((int64_t)plan.tiles_m * plan.tiles_n, kSms);
-      ok = make_map(&maps.m[0], w.x, bf16, BM) && make_map(&maps.m[1], w.dy, bf16, BM) &&
-           make_map(&maps.m[2], w.wg, bf16, kRecomputeCols) && make_map(&maps.m[3], w.wu, bf16, kRecomputeCols) &&
-           make_map(&maps.m[4], w.wd, bf16, BK);
+      ok = make_map(&maps.m[0], w.x, bf16, ROWS_K, BM) && make_map(&maps.m[1], w.dy, bf16, ROWS_K, BM) &&
+           make_map(&maps.m[2], w.wg, bf16, ROWS_K, kRecomputeCols) &&
+           make_map(&maps.m[3], w.wu, bf16, ROWS_K, kRecomputeCols) && make_map(&maps.m[4], w.wd, bf16, ROWS_MN, BK);
       a.bias[0] = t.b_gate; a.bias[1] = t.b_up;
     } else {
-      ok = make_map(&maps.m[0], w.dy, bf16, BM) && make_map(&maps.m[1], w.wd, bf16, BK);
+      ok = make_map(&maps.m[0], w.dy, bf16, ROWS_K, BM) && make_map(&maps.m[1], w.wd, bf16, ROWS_MN, BK);
       a.saved = const_cast<void*>(saved);
     }
-    if (sizeof(T) == 2)
-      ok = ok && make_store_map(&maps.out[0], w.dg.base, bf16, s.M, s.F, w.dg.ld) &&
-           make_store_map(&maps.out[1], w.du.base, bf16, s.M, s.F, w.du.ld);
     if (!ok) return cudaErrorInvalidValue;
-    a.tiles_m = plan.tiles_m; a.tiles_n = plan.tiles_n; a.batches = 1;
-    a.group_m = 8;
+    set_tiles(a, plan.tiles_m, plan.tiles_n, 1);
     a.act = p.act;
     a.operand_bf16 = bf16;
     a.out[0] = const_cast<void*>(w.dg.base); a.out[1] = const_cast<void*>(w.du.base);
-    a.ldo = w.dg.ld;
-    a.plane = w.dg.plane;
+    a.ldo = round_up(s.M, 32);
+    a.plane = s.panel_plane_bytes();
     a.colsum = g.b_gate || g.b_up ? w.colsum : nullptr;
     if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;
-    e = again ? launch_gemm<T, EPI_RECOMPUTE, kRecomputeBn, false, false, false>("ffn_dhidden", maps, a, plan.workers, st)
-              : launch_gemm<T, EPI_DGATE, false, true>("ffn_dhidden", plan, maps, a, st);
+    e = again ? launch_gemm<T, EPI_RECOMPUTE, kRecomputeBn, ROWS_K, ROWS_K, false>("ffn_dhidden", maps, a, plan.workers, st)
+              : launch_gemm<T, EPI_DGATE, ROWS_K, ROWS_MN>("ffn_dhidden", plan, maps, a, st);
     if (e != cudaSuccess) return e;
     if (a.colsum) {
       KernelScope ks("ffn_column_finish", st);
@@ -457,15 +452,15 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
     }
   }
   if (g.w_down &&
-      (e = store_product<T, true, true>("ffn_dw_down", {w.dy}, {h}, s.C, s.F, s.M, 1, &g.w_down, s.F, nullptr, w.partial, st)) !=
+      (e = store_product<T, ROWS_MN, PANELS_MN>("ffn_dw_down", {w.dy}, {h}, s.C, s.F, s.M, 1, &g.w_down, s.F, nullptr, w.partial, st)) !=
           cudaSuccess)
     return e;
   if (g.w_gate && g.w_up) {
     void* const out[2] = {g.w_gate, g.w_up};
-    e = store_product<T, true, true>("ffn_dw_gate_up", {w.dg, w.du}, {w.x}, s.F, s.C, s.M, 2, out, s.C, nullptr, w.partial, st);
+    e = store_product<T, PANELS_MN, ROWS_MN>("ffn_dw_gate_up", {w.dg, w.du}, {w.x}, s.F, s.C, s.M, 2, out, s.C, nullptr, w.partial, st);
   } else if (g.w_gate || g.w_up) {
     void* const out[1] = {g.w_gate ? g.w_gate : g.w_up};
-    e = store_product<T, true, true>("ffn_dw_gate_up", {g.w_gate ? w.dg : w.du}, {w.x}, s.F, s.C, s.M, 1, out, s.C, nullptr,
+    e = store_product<T, PANELS_MN, ROWS_MN>("ffn_dw_gate_up", {g.w_gate ? w.dg : w.du}, {w.x}, s.F, s.C, s.M, 1, out, s.C, nullptr,
                                      w.partial, st);
   }
   if (e != cudaSuccess) return e;
@@ -489,7 +484,7 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
   }
   if (ready) ready(user);
   if (!g.x) return cudaSuccess;
-  return store_product<T, false, true>("ffn_dx", {w.dg, w.du}, {w.wg, w.wu}, s.M, s.C, s.F, 1, &g.x, s.C, nullptr, w.partial, st);
+  return store_product<T, PANELS_K, ROWS_MN>("ffn_dx", {w.dg, w.du}, {w.wg, w.wu}, s.M, s.C, s.F, 1, &g.x, s.C, nullptr, w.partial, st);
 }
 
 }  // namespace

@@ -28,8 +28,9 @@ constexpr size_t saved_block_bytes(bool wide) { return wide ? 4096 : 2048 + 64; 
 // gate and up enter the derivative unrounded.
 constexpr bool recompute_gate_up(int64_t channels, bool wide) { return channels <= (wide ? 128 : 256); }
 
-// A matrix as the products read it: 16-bit planes of [rows][ld], rows on
-// 16-byte boundaries.
+// A matrix as the products read it, in 16-bit planes: row-major [rows][ld], rows
+// on 16-byte boundaries; or, for the block's own operands, panels of 8 columns
+// (dcn_ffn_gemm.cuh; ld and plane do not apply).
 struct Operand {
   const void* base = nullptr;
   int64_t rows = 0, cols = 0, ld = 0, plane = 0;
@@ -110,6 +111,9 @@ struct Shape {
   size_t operand_bytes(int64_t rows, int64_t cols) const {
     return ws_align((size_t)planes * (size_t)rows * (size_t)round_up(cols, 8) * 2);
   }
+  // the block's own operands: [cols / 8][rows to 32][8] a plane
+  size_t panel_plane_bytes() const { return (size_t)round_up(M, 32) * (size_t)round_up(F, 8) * 2; }
+  size_t panels_bytes() const { return ws_align((size_t)planes * panel_plane_bytes()); }
   Operand operand(const void* base, int64_t rows, int64_t cols) const {
     Operand o;
     o.base = base;
@@ -152,7 +156,7 @@ struct ForwardWs {
     wg = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_gate, s.F, s.C);
     wu = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_up, s.F, s.C);
     wd = s.operand(pack_f ? c.take(s.operand_bytes(s.C, s.F)) : t.w_down, s.C, s.F);
-    h = s.operand(hidden ? hidden : c.take(s.operand_bytes(s.M, s.F)), s.M, s.F);
+    h = s.operand(hidden ? hidden : c.take(s.panels_bytes()), s.M, s.F);
     partial = static_cast<float*>(c.take(store_partial_bytes(s.M, s.C, s.F, s.pair, 1)));
     total = c.at;
   }
@@ -175,8 +179,8 @@ struct BackwardWs {
     wg = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_gate, s.F, s.C);
     wu = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_up, s.F, s.C);
     wd = s.operand(pack_f ? c.take(s.operand_bytes(s.C, s.F)) : t.w_down, s.C, s.F);
-    dg = s.operand(c.take(s.operand_bytes(s.M, s.F)), s.M, s.F);
-    du = s.operand(c.take(s.operand_bytes(s.M, s.F)), s.M, s.F);
+    dg = s.operand(c.take(s.panels_bytes()), s.M, s.F);
+    du = s.operand(c.take(s.panels_bytes()), s.M, s.F);
     const size_t part = std::max({store_partial_bytes(s.C, s.F, s.M, s.pair, 1),
                                   store_partial_bytes(s.F, s.C, s.M, s.pair, 1),
                                   store_partial_bytes(s.F, s.C, s.M, s.pair, 2),

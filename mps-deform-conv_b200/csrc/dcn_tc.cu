@@ -459,7 +459,7 @@ static bool encode_tmap(CUtensorMap* map, const void* base, bool bf16, int rank,
                         const cuuint64_t* strides, const cuuint32_t* box,
                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   const EncodeFn encode = tmap_encoder();
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
   return encode &&
          encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
                 const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -474,13 +474,23 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, 
   return encode_tmap(map, base, bf16, 2, dims, strides, box);
 }
 
-bool make_tmap_3d(CUtensorMap* map, const void* base, bool bf16, uint64_t planes, uint64_t rows, uint64_t cols,
-                  uint64_t ld, uint64_t plane, uint32_t box_rows, uint32_t box_cols) {
-  const cuuint64_t dims[3] = {cols, rows, planes};
-  const cuuint64_t strides[2] = {ld * 2, plane * 2};
+bool make_tmap_rows(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t cols,
+                    int64_t ld, int64_t plane, uint32_t box_rows, uint32_t box_cols, int swizzle) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
   const cuuint32_t box[3] = {box_cols, box_rows, 1};
   return encode_tmap(map, base, bf16, 3, dims, strides, box,
-                     box_cols == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_128B);
+                     swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                     : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                     : CU_TENSOR_MAP_SWIZZLE_32B);
+}
+
+bool make_tmap_panels(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t panels,
+                      uint32_t box_rows, uint32_t box_panels) {
+  const cuuint64_t dims[4] = {256, (cuuint64_t)rows / 32, (cuuint64_t)panels, (cuuint64_t)planes};
+  const cuuint64_t strides[3] = {512, (cuuint64_t)rows * 16, (cuuint64_t)(rows * panels) * 16};
+  const cuuint32_t box[4] = {256, box_rows / 32, box_panels, 1};
+  return encode_tmap(map, base, bf16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // Forward weight image wsw of `w` (weight_images_kernel, or the per-image

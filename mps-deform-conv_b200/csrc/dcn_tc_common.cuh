@@ -656,10 +656,15 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, 
                   uint32_t box_rows, uint32_t box_cols);
 
 // Host: the same over `planes` matrices [rows][cols] of row stride `ld` and
-// distance `plane` (elements; ld and plane multiples of 8, base on 16 bytes).
-// A box of 16 columns (32-byte rows) has the 32-byte swizzle.
-bool make_tmap_3d(CUtensorMap* map, const void* base, bool bf16, uint64_t planes, uint64_t rows, uint64_t cols,
-                  uint64_t ld, uint64_t plane, uint32_t box_rows, uint32_t box_cols);
+// distance `plane` (elements; ld and plane multiples of 8, base on 16 bytes),
+// with the swizzle of the box's rows: 128, 64 or 32 bytes.
+bool make_tmap_rows(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t cols,
+                    int64_t ld, int64_t plane, uint32_t box_rows, uint32_t box_cols, int swizzle);
+// Host: a matrix in panels of 8 columns, [planes][panels][rows][8] with rows a
+// multiple of 32: boxes of box_rows (a multiple of 32) x box_panels panels, no
+// swizzle; coordinates (0, row / 32, panel, plane).
+bool make_tmap_panels(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t panels,
+                      uint32_t box_rows, uint32_t box_panels);
 
 // Host: device address of the status word on the current device.
 cudaError_t tc_status_ptr(int** out);

@@ -10,7 +10,8 @@ Bounds are elementwise and count roundings:
     (more than 256 channels) to 11 bits;
   * errors of gate and up enter the activation by its largest slope, those of its derivative
     by the largest curvature (relu: a sign may change where gate is within its own error);
-  * the fast exponential and quotient of 16-bit data: 2^-19 of the value; fp32: 2^-21.
+  * 16-bit data: the fast exponential and quotient leave 2^-19 of an activation's value, the
+    fitted normal distribution function 2^-17; fp32: 2^-21.
 """
 import math
 
@@ -58,7 +59,7 @@ def _reference(args, dy, act, dtype):
     u = torch.finfo(dtype).eps / 2
     wide = dtype == torch.float32
     floor = 2.0 ** -25 if dtype == torch.float16 else 1e-38
-    fast = 2.0 ** (-21 if wide else -19)
+    fast = 2.0 ** (-21 if wide else -17 if act == "gelu" else -19)
     z = lambda t: 0.0 if t is None else t  # noqa: E731
     ab = lambda t: 0.0 if t is None else t.abs()  # noqa: E731
     gate, up = x @ wg.t() + z(bg), x @ wu.t() + z(bu)
@@ -79,8 +80,9 @@ def _reference(args, dy, act, dtype):
     dh = dy @ wd
     e_dh = _sum_err(c, dtype) * (dy.abs() @ wd.abs())
     if not wide and c > 256:  # gate and up come back from the saved state with 11 bits
-        e_g = e_g + 2.0 ** -11 * (gate.abs() + e_g) + 2.0 ** -36 * gate.abs().amax(1, keepdim=True)
-        e_u = e_u + 2.0 ** -11 * (up.abs() + e_u) + 2.0 ** -36 * up.abs().amax(1, keepdim=True)
+        # (a subnormal's step where the largest of 16 columns is at least 2^-4, else relative to that)
+        e_g = e_g + 2.0 ** -11 * (gate.abs() + e_g) + (2.0 ** -36 * gate.abs()).amax(1, keepdim=True).clamp(min=2.0 ** -25)
+        e_u = e_u + 2.0 ** -11 * (up.abs() + e_u) + (2.0 ** -36 * up.abs()).amax(1, keepdim=True).clamp(min=2.0 ** -25)
         e_a = SLOPE[act] * e_g + fast * (a.abs() + e_g)
     e_da = CURVE[act] * e_g + fast * 2
     if act == "relu":
