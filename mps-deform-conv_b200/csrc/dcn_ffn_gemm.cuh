@@ -331,6 +331,33 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+// Two fp32 operations an instruction (each rounded as the scalar one).
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 parts(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pair_of(a, a); }
 template <bool ACCURATE>
 __device__ __forceinline__ float sigmoid(float x) {
   // far below zero the exponential overflows to inf and the quotient is 0, as it should be
@@ -379,20 +406,99 @@ __device__ __forceinline__ float2 act_both(float x) {
     return make_float2(s, s * (1.0f - s));
   }
 }
+// The fast forms on two values.
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t x) {
+  const float2 e = parts(mul2(x, twice(-kLog2e)));
+  const float2 d = parts(add2(pair_of(exp2_fast(e.x), exp2_fast(e.y)), twice(1.0f)));
+  return pair_of(rcp_fast(d.x), rcp_fast(d.y));
+}
+struct Cdf2 {
+  uint64_t cdf, e;
+};
+__device__ __forceinline__ Cdf2 normal_cdf2(uint64_t x) {
+  const float2 xs = parts(x);
+  const uint64_t z = pair_of(fabsf(xs.x), fabsf(xs.y));
+  const float2 d = parts(fma2(twice(0.308f), z, twice(1.0f)));
+  const uint64_t t = pair_of(rcp_fast(d.x), rcp_fast(d.y));
+  const float2 q = parts(mul2(mul2(x, x), twice(-0.5f * kLog2e)));
+  const uint64_t e = pair_of(exp2_fast(q.x), exp2_fast(q.y));
+  uint64_t r = fma2(t, twice(-0.0754310913f), twice(0.189621131f));
+  r = fma2(t, r, twice(0.00726954421f));
+  r = fma2(t, r, twice(0.136535319f));
+  r = fma2(t, r, twice(0.118880802f));
+  r = fma2(t, r, twice(0.123122739f));
+  const uint64_t low2 = mul2(e, mul2(t, r));
+  const float2 low = parts(low2), high = parts(fma2(low2, twice(-1.0f), twice(1.0f)));
+  return {pair_of(xs.x > 0.0f ? high.x : low.x, xs.y > 0.0f ? high.y : low.y), e};
+}
+template <int ACT>
+__device__ __forceinline__ uint64_t act_value2(uint64_t x) {
+  if constexpr (ACT == kActSilu) return mul2(x, sigmoid2(x));
+  else if constexpr (ACT == kActGelu) return mul2(x, normal_cdf2(x).cdf);
+  else if constexpr (ACT == kActSigmoid) return sigmoid2(x);
+  else {
+    const float2 f = parts(x);
+    return pair_of(act_value<false, kActRelu>(f.x), act_value<false, kActRelu>(f.y));
+  }
+}
+template <int ACT>
+__device__ __forceinline__ void act_both2(uint64_t x, uint64_t& a, uint64_t& da) {
+  if constexpr (ACT == kActSilu) {
+    const uint64_t s = sigmoid2(x);
+    a = mul2(x, s);
+    da = fma2(a, fma2(s, twice(-1.0f), twice(1.0f)), s);
+  } else if constexpr (ACT == kActGelu) {
+    const Cdf2 c = normal_cdf2(x);
+    a = mul2(x, c.cdf);
+    da = fma2(x, mul2(twice(0.39894228040143268f), c.e), c.cdf);
+  } else if constexpr (ACT == kActSigmoid) {
+    a = sigmoid2(x);
+    da = mul2(a, fma2(a, twice(-1.0f), twice(1.0f)));
+  } else {
+    const float2 f = parts(x);
+    const float2 p = act_both<false, kActRelu>(f.x), q = act_both<false, kActRelu>(f.y);
+    a = pair_of(p.x, q.x);
+    da = pair_of(p.y, q.y);
+  }
+}
+
 // A row's block at a time; the activation is picked once for all of it.
 template <bool ACCURATE, int ACT>
 __device__ __forceinline__ void gate_block(const float (&g)[CB], const float (&u)[CB], float (&h)[CB]) {
 #pragma unroll
-  for (int j = 0; j < CB; ++j) h[j] = act_value<ACCURATE, ACT>(g[j]) * u[j];
+  for (int j = 0; j < CB; j += 2) {
+    if constexpr (ACCURATE) {
+      h[j] = act_value<true, ACT>(g[j]) * u[j];
+      h[j + 1] = act_value<true, ACT>(g[j + 1]) * u[j + 1];
+    } else {
+      const float2 r = parts(mul2(act_value2<ACT>(pair_of(g[j], g[j + 1])), pair_of(u[j], u[j + 1])));
+      h[j] = r.x;
+      h[j + 1] = r.y;
+    }
+  }
 }
 // (gate, up) to (dgate, dup)
 template <bool ACCURATE, int ACT>
 __device__ __forceinline__ void dgate_block(const float (&dh)[CB], float (&g)[CB], float (&u)[CB]) {
 #pragma unroll
-  for (int j = 0; j < CB; ++j) {
-    const float2 s = act_both<ACCURATE, ACT>(g[j]);
-    g[j] = dh[j] * u[j] * s.y;
-    u[j] = dh[j] * s.x;
+  for (int j = 0; j < CB; j += 2) {
+    if constexpr (ACCURATE) {
+#pragma unroll
+      for (int k = j; k < j + 2; ++k) {
+        const float2 s = act_both<true, ACT>(g[k]);
+        g[k] = dh[k] * u[k] * s.y;
+        u[k] = dh[k] * s.x;
+      }
+    } else {
+      uint64_t a, da;
+      act_both2<ACT>(pair_of(g[j], g[j + 1]), a, da);
+      const uint64_t d = pair_of(dh[j], dh[j + 1]);
+      const float2 x = parts(mul2(mul2(d, pair_of(u[j], u[j + 1])), da)), y = parts(mul2(d, a));
+      g[j] = x.x;
+      g[j + 1] = x.y;
+      u[j] = y.x;
+      u[j + 1] = y.y;
+    }
   }
 }
 template <bool ACCURATE>
@@ -613,39 +719,40 @@ struct SavedRaw {
 };
 
 // ---------------------------------------------------------------- column sums of a block
-// 16-bit: of the staged (rounded) values, by the legacy matrix instruction with
-// a row operand of ones: two ldmatrix and four mma.sync a block, where a sum
-// across lanes takes some 120 instructions (a quarter of the whole epilogue).
-// Stores the sums of columns c0 .. c0 + 15 below n.
+// 16-bit: of the rounded values, staged by their lanes as [32 rows][dgate 16,
+// dup 16] (64-byte rows, their 8-byte pieces rotated by the row): lane l adds
+// four columns, piece l % 8, of rows l / 8, l / 8 + 4, ..., then the four row
+// groups meet in two shuffles.  Lanes 0-7 hold the sums of columns 4 l .. 4 l + 3
+// of the 32.  (By mma.sync with a row operand of ones: 150 us more in the
+// 92416 x 2048 pass; the legacy instruction takes the tensor cores' time.)
 template <typename T>
-__device__ __forceinline__ void staged_column_sums(uint32_t block, int lane, float* out, int c0, int n) {
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  const uint32_t one = BF ? 0x3f803f80u : 0x3c003c00u;
+__device__ __forceinline__ void stage_sums(uint8_t* rows, int lane, int at, const float (&v)[CB]) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t r[4];  // rows 8 i .. 8 i + 7 of eight columns, transposed: pairs of rows a lane
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(block + staged_piece<32>(lane, j))
-                 : "memory");
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if constexpr (BF)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(one), "r"(r[2 * s]), "r"(r[2 * s + 1]));
-      else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(one), "r"(r[2 * s]), "r"(r[2 * s + 1]));
-    }
-    const int c = c0 + 8 * j + 2 * lane;  // every row of the result is the sums; lanes 0-3 hold row 0
-    if (lane < 4) {
-      if (c < n) out[c] = d[0];
-      if (c + 1 < n) out[c + 1] = d[1];
-    }
+  for (int j = 0; j < CB / 4; ++j) {
+    uint2 p;
+    p.x = pack2(v[4 * j], v[4 * j + 1], (T*)nullptr);
+    p.y = pack2(v[4 * j + 2], v[4 * j + 3], (T*)nullptr);
+    *reinterpret_cast<uint2*>(rows + lane * 64 + (((at + j + lane) & 7) << 3)) = p;
   }
+}
+template <typename T>
+__device__ __forceinline__ void staged_column_sums(const uint8_t* rows, int lane, float (&sum)[4]) {
+  const int piece = lane & 7;
+  uint64_t lo = twice(0.0f), hi = twice(0.0f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = (lane >> 3) + 4 * i;
+    const uint2 p = *reinterpret_cast<const uint2*>(rows + r * 64 + (((piece + r) & 7) << 3));
+    const float2 x = tcc::Vec<T>::unpack(p.x), y = tcc::Vec<T>::unpack(p.y);
+    lo = add2(lo, pair_of(x.x, x.y));
+    hi = add2(hi, pair_of(y.x, y.y));
+  }
+  const float2 x = parts(lo), y = parts(hi);
+  sum[0] = x.x; sum[1] = x.y; sum[2] = y.x; sum[3] = y.y;
+#pragma unroll
+  for (int o = 8; o <= 16; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
 }
 // fp32: lanes 0-15 return the sums of columns 0-15 over the warp's lanes, in an
 // order fixed by the lanes.
@@ -1024,11 +1131,13 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
 #pragma unroll
           for (int j = 0; j < CB / 4; ++j) {
             const float4 f = reinterpret_cast<const float4*>(colf)[j];
-            v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
-            if (TWO) {
-              const float4 h = reinterpret_cast<const float4*>(colf + CB)[j];
-              u[4 * j] += h.x; u[4 * j + 1] += h.y; u[4 * j + 2] += h.z; u[4 * j + 3] += h.w;
-            }
+            auto add4 = [&](float (&t)[CB], const float4& b) {
+              const float2 lo = parts(add2(pair_of(t[4 * j], t[4 * j + 1]), pair_of(b.x, b.y)));
+              const float2 hi = parts(add2(pair_of(t[4 * j + 2], t[4 * j + 3]), pair_of(b.z, b.w)));
+              t[4 * j] = lo.x; t[4 * j + 1] = lo.y; t[4 * j + 2] = hi.x; t[4 * j + 3] = hi.y;
+            };
+            add4(v, f);
+            if (TWO) add4(u, reinterpret_cast<const float4*>(colf + CB)[j]);
           }
         }
         // this row in the panels of the block's columns
@@ -1062,11 +1171,18 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
               }
             } else {
               __syncwarp();
-              stage_row<T, 32>(stage, lane, 0, v);
-              stage_row<T, 32>(stage + kSumBlock, lane, 0, u);
+              stage_sums<T>(stage, lane, 0, v);
+              stage_sums<T>(stage, lane, 4, u);
               __syncwarp();
-              staged_column_sums<T>(smem_addr(stage), lane, sums, c0, a.N);
-              staged_column_sums<T>(smem_addr(stage + kSumBlock), lane, sums + a.N, c0, a.N);
+              float sum[4];
+              staged_column_sums<T>(stage, lane, sum);
+              if (lane < 8) {  // dgate's columns, then dup's
+                const int c = c0 + 4 * (lane & 3);
+                float* out = sums + (lane >= 4 ? a.N : 0) + c;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (c + j < a.N) out[j] = sum[j];
+              }
             }
           }
         } else {
