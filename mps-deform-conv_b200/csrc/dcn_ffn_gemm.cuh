@@ -17,8 +17,9 @@
 // size needs to be a multiple of anything.
 //
 // The caller's matrices are row-major (128-byte-swizzled tiles).  The block's
-// own operands (hidden, dgate, dup) lie in panels of 8 columns: panel p holds
-// columns 8 p .. 8 p + 7 of all rows, 16 bytes a row.  The lanes of an epilogue
+// own operands (hidden, dgate, dup) lie in panels: of each 128 rows, panel p
+// holds columns 8 p .. 8 p + 7, 16 bytes a row, and the panels of the 128 rows
+// follow one another (a tile is one run of memory).  The lanes of an epilogue
 // warp are rows, so they store 512 contiguous bytes an instruction from their
 // registers, where a row-major matrix needs staging and a TMA store whose rows
 // are 32 bytes (these row requests, beside the operands', held the TMA up: the
@@ -157,7 +158,7 @@ struct GemmArgs {
   uint32_t operand_bf16;
   float* partial;
   // outputs: STORE: out[batch] [M][ldo] of T (+ bias); else panels of hidden, or dgate and dup:
-  // ldo rows a panel (M rounded up to 32), `plane` bytes between the bf16 planes of fp32 data
+  // ldo panels of 128 rows, `plane` bytes between the bf16 planes of fp32 data
   void* out[2];
   int64_t ldo, plane;
   int vec;                   // out rows take 16-byte stores (16-bit data: TMA stores)
@@ -301,17 +302,18 @@ __device__ __forceinline__ void load_g(uint32_t dst, const CUtensorMap* map, int
 template <bool PAIR>
 __device__ __forceinline__ void load_panels(uint32_t dst, const CUtensorMap* map, int row, int panel, int plane,
                                             uint32_t bar) {
+  const int piece = (row >> 5) & 3, rows = row >> 7;
   if (PAIR)
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row >> 5), "r"(panel), "r"(plane), "r"(bar)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(piece), "r"(panel), "r"(rows), "r"(plane), "r"(bar)
         : "memory");
   else
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row >> 5), "r"(panel), "r"(plane), "r"(bar)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(piece), "r"(panel), "r"(rows), "r"(plane), "r"(bar)
         : "memory");
 }
 
@@ -591,11 +593,11 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
 
 // A block's columns of one row, as an operand of a following product: two
 // panels' pieces (fp32 data: in each of three bf16 planes).  `at`: this row in
-// the first panel; columns at and past `left` are not in the matrix, their
+// the first panel, 2048 bytes before the next; columns at and past `left` are not in the matrix, their
 // panel is skipped (values inside a last panel are zero).
 template <typename T>
-__device__ __forceinline__ void store_panels(uint8_t* at, int64_t panel_bytes, int64_t plane, int left,
-                                             const float (&v)[CB]) {
+__device__ __forceinline__ void store_panels(uint8_t* at, int64_t plane, int left, const float (&v)[CB]) {
+  constexpr int kPanel = BM * 16;
   if constexpr (sizeof(T) == 4) {
     float r[CB];
 #pragma unroll
@@ -604,7 +606,7 @@ __device__ __forceinline__ void store_panels(uint8_t* at, int64_t panel_bytes, i
     for (int k = 0; k < 3; ++k) {
 #pragma unroll
       for (int j = 0; j < CB / 8; ++j)
-        if (8 * j < left) *reinterpret_cast<uint4*>(at + k * plane + j * panel_bytes) = pack8<__nv_bfloat16>(r, j);
+        if (8 * j < left) *reinterpret_cast<uint4*>(at + k * plane + j * kPanel) = pack8<__nv_bfloat16>(r, j);
       // a plane that holds inf or NaN ends the expansion: the others are zero
 #pragma unroll
       for (int j = 0; j < CB; ++j) {
@@ -615,7 +617,7 @@ __device__ __forceinline__ void store_panels(uint8_t* at, int64_t panel_bytes, i
   } else {
 #pragma unroll
     for (int j = 0; j < CB / 8; ++j)
-      if (8 * j < left) *reinterpret_cast<uint4*>(at + j * panel_bytes) = pack8<T>(v, j);
+      if (8 * j < left) *reinterpret_cast<uint4*>(at + j * kPanel) = pack8<T>(v, j);
   }
 }
 
@@ -1140,26 +1142,27 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
             if (TWO) add4(u, reinterpret_cast<const float4*>(colf + CB)[j]);
           }
         }
-        // this row in the panels of the block's columns
-        const int64_t panel = a.ldo * 16;
-        const int64_t at = (int64_t)(c0 >> 3) * panel + row * 16;
+        // this row in the panels of the block's columns; rows past M are zero
+        // there, to the end of their 128
+        const bool rows_in = row0 - q * 32 < a.M;
+        const int64_t at = ((int64_t)(row0 >> 7) * a.ldo + (c0 >> 3)) * (BM * 16) + (q * 32 + lane) * 16;
         if constexpr (GATED) {
           if (a.saved) save_gate_up<T>(saved_block(c), lane, v, u);
           gate_block<WIDE>(a.act, v, u, v);
-          if (row0 + 32 > a.M && !row_in) {  // rows past M are zero in the panels
+          if (row0 + 32 > a.M && !row_in) {
 #pragma unroll
             for (int j = 0; j < CB; ++j) v[j] = 0.0f;
           }
-          if (row0 < a.M) store_panels<T>(static_cast<uint8_t*>(a.out[0]) + at, panel, a.plane, a.N - c0, v);
+          if (rows_in) store_panels<T>(static_cast<uint8_t*>(a.out[0]) + at, a.plane, a.N - c0, v);
         } else if constexpr (DGATE) {
           dgate_block<WIDE>(a.act, dh, v, u);
           if (row0 + 32 > a.M && !row_in) {
 #pragma unroll
             for (int j = 0; j < CB; ++j) v[j] = u[j] = 0.0f;
           }
-          if (row0 < a.M) {
-            store_panels<T>(static_cast<uint8_t*>(a.out[0]) + at, panel, a.plane, a.N - c0, v);
-            store_panels<T>(static_cast<uint8_t*>(a.out[1]) + at, panel, a.plane, a.N - c0, u);
+          if (rows_in) {
+            store_panels<T>(static_cast<uint8_t*>(a.out[0]) + at, a.plane, a.N - c0, v);
+            store_panels<T>(static_cast<uint8_t*>(a.out[1]) + at, a.plane, a.N - c0, u);
           }
           if (a.colsum) {
             float* sums = a.colsum + (m_block * 2) * a.N;

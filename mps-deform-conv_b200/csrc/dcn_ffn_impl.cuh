@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <vector>
 
+#include "dcn_ffn_few.cuh"
 #include "dcn_ffn_gemm.cuh"
 #include "dcn_ffn_layout.h"
 
@@ -31,8 +32,8 @@ bool make_map(CUtensorMap* map, const Operand& o, bool bf16, Form form, uint32_t
   switch (form) {
     case ROWS_K: return make_tmap_rows(map, o.base, bf16, o.planes, o.rows, o.cols, o.ld, o.plane, box, BK, 128);
     case ROWS_MN: return make_tmap_rows(map, o.base, bf16, o.planes, o.rows, o.cols, o.ld, o.plane, BK, 64, 128);
-    case PANELS_K: return make_tmap_panels(map, o.base, bf16, o.planes, round_up(o.rows, 32), div_up(o.cols, 8), box, BK / 8);
-    default: return make_tmap_panels(map, o.base, bf16, o.planes, round_up(o.rows, 32), div_up(o.cols, 8), BK, box / 8);
+    case PANELS_K: return make_tmap_panels(map, o.base, bf16, o.planes, div_up(o.rows, BM), div_up(o.cols, 8), box, BK / 8);
+    default: return make_tmap_panels(map, o.base, bf16, o.planes, div_up(o.rows, BM), div_up(o.cols, 8), BK, box / 8);
   }
 }
 
@@ -359,6 +360,12 @@ cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* s
   const Shape s(p);
   void* hidden = saved ? static_cast<uint8_t*>(saved) + s.blocks_bytes() : nullptr;
   const ForwardWs w(p, t, ws, hidden);
+  if (w.few) {
+    const FewArgs up{t.x, {t.w_gate, t.w_up}, {t.b_gate, t.b_up}, w.few, (int)s.M, (int)s.F, (int)s.C, p.act};
+    const FewArgs down{w.few, {t.w_down, nullptr}, {t.b_down, nullptr}, y, (int)s.M, (int)s.C, (int)s.F, p.act};
+    const cudaError_t e = launch_few<T, true>("ffn_few_gate_up", up, st);
+    return e != cudaSuccess ? e : launch_few<T, false>("ffn_few_down", down, st);
+  }
   Packer pk;
   if (w.pack_c) {
     pk.add(w.x, t.x);
@@ -383,7 +390,7 @@ cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* s
   a.act = p.act;
   a.operand_bf16 = operand_bf16<T>();
   a.out[0] = const_cast<void*>(w.h.base);
-  a.ldo = round_up(s.M, 32);
+  a.ldo = div_up(s.F, 8);
   a.plane = s.panel_plane_bytes();
   a.bias[0] = t.b_gate; a.bias[1] = t.b_up;
   a.saved = s.recompute() ? nullptr : saved;
@@ -437,7 +444,7 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
     a.act = p.act;
     a.operand_bf16 = bf16;
     a.out[0] = const_cast<void*>(w.dg.base); a.out[1] = const_cast<void*>(w.du.base);
-    a.ldo = round_up(s.M, 32);
+    a.ldo = div_up(s.F, 8);
     a.plane = s.panel_plane_bytes();
     a.colsum = g.b_gate || g.b_up ? w.colsum : nullptr;
     if ((e = tc_status_ptr(&a.status)) != cudaSuccess) return e;

@@ -111,8 +111,8 @@ struct Shape {
   size_t operand_bytes(int64_t rows, int64_t cols) const {
     return ws_align((size_t)planes * (size_t)rows * (size_t)round_up(cols, 8) * 2);
   }
-  // the block's own operands: [cols / 8][rows to 32][8] a plane
-  size_t panel_plane_bytes() const { return (size_t)round_up(M, 32) * (size_t)round_up(F, 8) * 2; }
+  // the block's own operands: [rows / 128][cols / 8][128][8] a plane
+  size_t panel_plane_bytes() const { return (size_t)round_up(M, BM) * (size_t)round_up(F, 8) * 2; }
   size_t panels_bytes() const { return ws_align((size_t)planes * panel_plane_bytes()); }
   Operand operand(const void* base, int64_t rows, int64_t cols) const {
     Operand o;
@@ -142,14 +142,26 @@ struct Carver {
   }
 };
 
+// Few rows and nothing to save: the weights are streamed (dcn_ffn_few.cuh).
+inline bool few_rows(const FfnProblem& p, bool save) {
+  if (save || p.M > 32) return false;
+  return p.dtype == DCN_FLOAT32 || (p.C % 8 == 0 && p.F % 8 == 0);
+}
+
 struct ForwardWs {
   Operand x, wg, wu, wd, h;
-  float* partial;
-  size_t total;
-  bool pack_c, pack_f;
+  void* few = nullptr;  // few rows: the hidden values, row-major
+  float* partial = nullptr;
+  size_t total = 0;
+  bool pack_c = false, pack_f = false;
   ForwardWs(const FfnProblem& p, const FfnTensors& t, void* ws, void* hidden) {
     const Shape s(p);
     Carver c{static_cast<uint8_t*>(ws)};
+    if (few_rows(p, hidden != nullptr)) {
+      few = c.take((size_t)s.M * (size_t)s.F * s.es);
+      total = c.at;
+      return;
+    }
     pack_c = s.pack_rows_c();
     pack_f = s.pack_rows_f();
     x = s.operand(pack_c ? c.take(s.operand_bytes(s.M, s.C)) : t.x, s.M, s.C);

@@ -459,7 +459,7 @@ static bool encode_tmap(CUtensorMap* map, const void* base, bool bf16, int rank,
                         const cuuint64_t* strides, const cuuint32_t* box,
                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   const EncodeFn encode = tmap_encoder();
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return encode &&
          encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
                 const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -485,12 +485,12 @@ bool make_tmap_rows(CUtensorMap* map, const void* base, bool bf16, int64_t plane
                                      : CU_TENSOR_MAP_SWIZZLE_32B);
 }
 
-bool make_tmap_panels(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t panels,
-                      uint32_t box_rows, uint32_t box_panels) {
-  const cuuint64_t dims[4] = {256, (cuuint64_t)rows / 32, (cuuint64_t)panels, (cuuint64_t)planes};
-  const cuuint64_t strides[3] = {512, (cuuint64_t)rows * 16, (cuuint64_t)(rows * panels) * 16};
-  const cuuint32_t box[4] = {256, box_rows / 32, box_panels, 1};
-  return encode_tmap(map, base, bf16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+bool make_tmap_panels(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t row_blocks,
+                      int64_t panels, uint32_t box_rows, uint32_t box_panels) {
+  const cuuint64_t dims[5] = {256, 4, (cuuint64_t)panels, (cuuint64_t)row_blocks, (cuuint64_t)planes};
+  const cuuint64_t strides[4] = {512, 2048, (cuuint64_t)panels * 2048, (cuuint64_t)(row_blocks * panels) * 2048};
+  const cuuint32_t box[5] = {256, box_rows / 32, box_panels, 1, 1};
+  return encode_tmap(map, base, bf16, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // Forward weight image wsw of `w` (weight_images_kernel, or the per-image

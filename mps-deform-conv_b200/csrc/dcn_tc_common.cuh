@@ -660,11 +660,11 @@ bool make_tmap_2d(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, 
 // with the swizzle of the box's rows: 128, 64 or 32 bytes.
 bool make_tmap_rows(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t cols,
                     int64_t ld, int64_t plane, uint32_t box_rows, uint32_t box_cols, int swizzle);
-// Host: a matrix in panels of 8 columns, [planes][panels][rows][8] with rows a
-// multiple of 32: boxes of box_rows (a multiple of 32) x box_panels panels, no
-// swizzle; coordinates (0, row / 32, panel, plane).
-bool make_tmap_panels(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t rows, int64_t panels,
-                      uint32_t box_rows, uint32_t box_panels);
+// Host: a matrix in panels of 8 columns, [planes][row_blocks][panels][128][8]:
+// boxes of box_rows (32 to 128) x box_panels panels, no swizzle; coordinates
+// (0, 32-row piece, panel, 128-row block, plane).
+bool make_tmap_panels(CUtensorMap* map, const void* base, bool bf16, int64_t planes, int64_t row_blocks,
+                      int64_t panels, uint32_t box_rows, uint32_t box_panels);
 
 // Host: device address of the status word on the current device.
 cudaError_t tc_status_ptr(int** out);

@@ -65,18 +65,24 @@ struct FfnArgs {
   dcn_ffn_tensors t;
   FfnArgs(const at::Tensor& input, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
           const OptTensor& bg, const OptTensor& bu, const OptTensor& bd, int64_t activation) {
-    TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
-    TORCH_CHECK(input.dim() >= 1, "input must have a channel dimension");
-    check_cuda(wg, "w_gate", input);
-    check_cuda(wu, "w_up", input);
-    check_cuda(wd, "w_down", input);
+    TORCH_CHECK_VALUE(input.is_cuda(), "Input must be on CUDA device, got ", input.device());
+    TORCH_CHECK_VALUE(input.dim() >= 1, "input must have a channel dimension");
     const int64_t c = input.size(-1);
-    TORCH_CHECK(wg.dim() == 2 && wg.size(1) == c, "w_gate must have shape (hidden, ", c, "), got ", wg.sizes());
+    auto placed = [&](const at::Tensor& t, const char* name) {
+      TORCH_CHECK_VALUE(t.device() == input.device(), name, " must be on same device as input (", input.device(),
+                        "), got ", t.device());
+      check_cuda(t, name, input);
+    };
+    placed(wg, "w_gate");
+    placed(wu, "w_up");
+    placed(wd, "w_down");
+    TORCH_CHECK_VALUE(wg.dim() == 2 && wg.size(1) == c, "w_gate must have shape (hidden, ", c, "), got ", wg.sizes());
     const int64_t f = wg.size(0);
-    TORCH_CHECK(wu.sizes() == wg.sizes(), "w_up must have shape ", wg.sizes(), " as w_gate, got ", wu.sizes());
-    TORCH_CHECK(wd.dim() == 2 && wd.size(0) == c && wd.size(1) == f, "w_down must have shape (", c, ", ", f, "), got ",
-                wd.sizes());
-    TORCH_CHECK(bg.has_value() == bu.has_value(), "b_gate and b_up go together");
+    TORCH_CHECK_VALUE(wu.sizes() == wg.sizes(), "w_up must have shape ", wg.sizes(), " as w_gate, got ", wu.sizes());
+    TORCH_CHECK_VALUE(wd.dim() == 2 && wd.size(0) == c && wd.size(1) == f, "w_down must have shape (", c, ", ", f,
+                      "), got ", wd.sizes());
+    TORCH_CHECK_VALUE(c > 0 && f > 0, "channels and hidden must be positive, got ", c, " and ", f);
+    TORCH_CHECK_VALUE(bg.has_value() == bu.has_value(), "b_gate and b_up go together");
     d.dtype = dtype_code(input);
     d.activation = (int32_t)activation;
     d.channels = c;
@@ -89,8 +95,8 @@ struct FfnArgs {
     w_down = dense16(wd);
     auto bias = [&](const OptTensor& b, const char* name, int64_t n) {
       if (!b.has_value()) return at::Tensor();
-      check_cuda(*b, name, input);
-      TORCH_CHECK(b->dim() == 1 && b->size(0) == n, name, " must have ", n, " elements, got ", b->sizes());
+      placed(*b, name);
+      TORCH_CHECK_VALUE(b->dim() == 1 && b->size(0) == n, name, " must have shape (", n, ",), got ", b->sizes());
       return b->contiguous();
     };
     b_gate = bias(bg, "b_gate", f);

@@ -572,9 +572,16 @@ class _GatedFeedForwardFunction(torch.autograd.Function):
         return (*grads, None)
 
 
+def _activation(name: str) -> int:
+    code = _ACTIVATIONS.get(name)
+    if code is None:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {name!r}")
+    return code
+
+
 def _validate_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation) -> int:
-    if activation not in _ACTIVATIONS:
-        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    """Checks of a traced call (the extension makes them otherwise); returns the activation's code."""
+    act = _activation(activation)
     if input.dim() < 1:
         raise ValueError("input must have a channel dimension")
     channels = input.size(-1)
@@ -596,7 +603,7 @@ def _validate_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, ac
                          (b_down, "b_down")):
         if tensor is not None:
             _check_tensor_device(tensor, name, input.device)
-    return _ACTIVATIONS[activation]
+    return act
 
 
 def gated_feed_forward(
@@ -637,13 +644,16 @@ def gated_feed_forward(
     which then computes gate and up again.  The parameter-gradient hook is
     called once for each of the three weights.
     """
-    traced = input.device.type == "meta" or torch.compiler.is_compiling()
-    if not (input.device.type == "cuda" or traced):
+    if input.is_cuda and not torch.compiler.is_compiling():  # checked by the extension
+        act = _activation(activation)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (
+                input, w_gate, w_up, w_down, b_gate, b_up, b_down)):
+            return _GatedFeedForwardFunction.apply(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+        return _get_lib().gated_feed_forward_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)[0]
+    if not (input.device.type == "meta" or torch.compiler.is_compiling()):
         raise ValueError(f"Input must be on CUDA device, got {input.device}")
     act = _validate_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
-    if traced:
-        return _ops.traced_gated_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
-    return _GatedFeedForwardFunction.apply(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+    return _ops.traced_gated_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
 
 
 class GatedFeedForward2d(nn.Module):
@@ -657,8 +667,7 @@ class GatedFeedForward2d(nn.Module):
         super().__init__()
         if channels <= 0 or hidden <= 0:
             raise ValueError(f"channels and hidden must be positive, got {channels} and {hidden}")
-        if activation not in _ACTIVATIONS:
-            raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+        _activation(activation)
         self.channels = channels
         self.hidden = hidden
         self.activation = activation
