@@ -6,10 +6,12 @@
 // streaming its weights from HBM straight into registers:
 //   few_gate_up   hidden[m][f] = act(x Wg^T + bg) * (x Wu^T + bu)
 //   few_down      y[m][c] = hidden Wd^T + bd
-// A CTA takes 16 weight rows (of gate and of up, or of down); a cluster of up to
-// eight CTAs and their four warps share K in blocks of 64, so that even a
-// product with few weight rows keeps every SM loading.  A lane reads 16-byte
-// pieces, four lanes a 64-byte run of a row.  16-bit data multiplies with the
+// A warp takes 16 weight rows (of gate and of up, or of down) and K in blocks of
+// 64; a lane reads 16-byte pieces, four lanes a 64-byte run of a row.  The four
+// warps of a CTA take different rows (they read the same part of x, which then
+// comes from the L1), or with few weight rows the same ones and share K; a
+// cluster of up to eight CTAs shares K too, so that a product with few weight
+// rows still keeps every SM loading.  16-bit data multiplies with the
 // legacy warp-level matrix instruction (rows of weights as the 16 x 16 operand,
 // up to 8 rows of x as the other): it takes its operands from registers, and at
 // this intensity (2 flops a byte and row) its rate does not matter.  The order
@@ -30,7 +32,7 @@ namespace dcn {
 namespace ffn {
 
 constexpr int kFewRows = 32;     // most rows of x
-constexpr int kFewTile = 16;     // weight rows of a CTA
+constexpr int kFewTile = 16;     // weight rows of a warp
 
 struct FewArgs {
   const void* x;       // [M][K]
@@ -71,18 +73,19 @@ __device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
   return v;
 }
 
-// 16-bit data.  NT: groups of 8 rows of x; GATED: gate and up, else plain.  The
-// CTAs of a cluster share a tile.  K a multiple of 8, all rows on 16-byte boundaries.
+// 16-bit data.  NT: groups of 8 rows of x; GATED: gate and up, else plain; ROWS:
+// the warps take different weight rows, else they share K.  The CTAs of a
+// cluster share a tile.  K a multiple of 8, all rows on 16-byte boundaries.
 constexpr int kFewWarps = 4;
-template <typename T, bool GATED, int NT>
+template <typename T, bool GATED, int NT, bool ROWS>
 __global__ void __launch_bounds__(kFewWarps * 32) ffn_few_kernel(const __grid_constant__ FewArgs a, int ctas) {
   constexpr int SETS = GATED ? 2 : 1, WARPS = kFewWarps;
-  __shared__ float sums[WARPS][SETS][kFewTile][8 * NT + 1];
-  __shared__ float part[SETS][8 * NT][kFewTile];
+  constexpr int TILE = kFewTile * (ROWS ? WARPS : 1), KW = ROWS ? 1 : WARPS;  // weight rows of a tile; warps that share K
+  __shared__ float sums[KW][SETS][TILE][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int rank = ctas > 1 ? (int)cluster_rank() : 0;
-  const int n0 = (blockIdx.x / ctas) * kFewTile;
+  const int tile0 = (blockIdx.x / ctas) * TILE, n0 = tile0 + (ROWS ? warp * kFewTile : 0);
   const T* w[SETS][2];  // this lane's two weight rows; rows past N read row N - 1, their sums are not stored
 #pragma unroll
   for (int s = 0; s < SETS; ++s)
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) ffn_few_kernel(const __grid_co
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[s][n][j] = 0.0f;
 
-  const int blocks = (a.K + 63) / 64, step = WARPS * ctas;
+  const int blocks = (a.K + 63) / 64, step = KW * ctas;
   uint4 r[SETS][2][2];  // [set][row][piece]
   auto fetch = [&](int b) {
 #pragma unroll
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) ffn_few_kernel(const __grid_co
           r[s][i][p] = k + t * 8 < a.K ? load_weights(w[s][i] + k) : make_uint4(0, 0, 0, 0);
         }
   };
-  int b = rank * WARPS + warp;
+  int b = rank * KW + (ROWS ? 0 : warp);
   if (b < blocks) fetch(b);
   if (GATED) pdl_launch();
   else pdl_wait();  // x is the previous kernel's result
@@ -153,10 +156,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) ffn_few_kernel(const __grid_co
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sums[warp][s][g + 8 * (j >> 1)][8 * n + 2 * t + (j & 1)] = acc[s][n][j];
+      for (int j = 0; j < 4; ++j) sums[ROWS ? 0 : warp][s][n0 - tile0 + g + 8 * (j >> 1)][8 * n + 2 * t + (j & 1)] = acc[s][n][j];
   __syncthreads();
   auto finish = [&](int i, auto&& sum) {
-    const int row = i % kFewTile, m = i / kFewTile, c = n0 + row;  // consecutive lanes: consecutive outputs of a row
+    const int row = i % TILE, m = i / TILE, c = tile0 + row;  // consecutive lanes: consecutive outputs of a row
     if (c >= a.N || m >= a.M) return;
     float v[SETS];
 #pragma unroll
@@ -173,25 +176,32 @@ __global__ void __launch_bounds__(kFewWarps * 32) ffn_few_kernel(const __grid_co
     }
     static_cast<T*>(a.out)[(int64_t)m * a.N + c] = from_f<T>(o);
   };
-  auto own = [&](int s, int row, int m) {
-    float v = 0.0f;
-#pragma unroll
-    for (int q = 0; q < WARPS; ++q) v += sums[q][s][row][m];
-    return v;
-  };
   if (ctas == 1) {
-    for (int i = threadIdx.x; i < kFewTile * 8 * NT; i += WARPS * 32) finish(i, own);
+    for (int i = threadIdx.x; i < TILE * 8 * NT; i += WARPS * 32)
+      finish(i, [&](int s, int row, int m) {
+        float v = sums[0][s][row][m];
+#pragma unroll
+        for (int q = 1; q < KW; ++q) v += sums[q][s][row][m];
+        return v;
+      });
     return;
   }
-  for (int i = threadIdx.x; i < kFewTile * 8 * NT; i += WARPS * 32)
+  if (KW > 1) {  // this CTA's part, over its warps
+    for (int i = threadIdx.x; i < TILE * 8 * NT; i += WARPS * 32)
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) part[s][i / kFewTile][i % kFewTile] = own(s, i % kFewTile, i / kFewTile);
+      for (int s = 0; s < SETS; ++s) {
+        float v = sums[0][s][i % TILE][i / TILE];
+#pragma unroll
+        for (int q = 1; q < KW; ++q) v += sums[q][s][i % TILE][i / TILE];
+        sums[0][s][i % TILE][i / TILE] = v;
+      }
+  }
   cluster_sync();
   // each CTA finishes its share of the tile from all parts, in order
-  for (int i = rank * WARPS * 32 + threadIdx.x; i < kFewTile * 8 * NT; i += ctas * WARPS * 32)
+  for (int i = rank * WARPS * 32 + threadIdx.x; i < TILE * 8 * NT; i += ctas * WARPS * 32)
     finish(i, [&](int s, int row, int m) {
       float v = 0.0f;
-      for (int q = 0; q < ctas; ++q) v += load_cluster(&part[s][m][row], (uint32_t)q);
+      for (int q = 0; q < ctas; ++q) v += load_cluster(&sums[0][s][row][m], (uint32_t)q);
       return v;
     });
   cluster_sync();  // the parts are read
@@ -300,16 +310,24 @@ cudaError_t launch_few(const char* name, const FewArgs& a, cudaStream_t st) {
     return launch_few(name, ffn_few_f32_kernel<GATED>, dim3((unsigned)div_up(a.N, 8), (unsigned)div_up(a.M, 8)), 256, 1,
                       !GATED, st, a);
   } else {
-    // CTAs of a tile: doubled while all tiles together are fewer than six CTAs an
-    // SM and every warp keeps a block of K
-    const int64_t tiles = div_up(a.N, kFewTile), blocks = div_up(a.K, 64);
+    // Warps on different rows where that leaves at least four CTAs an SM with K
+    // in eight parts.  CTAs of a tile: doubled while all tiles together are fewer
+    // than six CTAs an SM and every warp keeps a block of K.
+    const int64_t blocks = div_up(a.K, 64);
+    const bool rows = div_up(a.N, kFewTile * kFewWarps) * std::min<int64_t>(8, blocks) >= 4 * kSms;
+    const int64_t tiles = div_up(a.N, kFewTile * (rows ? kFewWarps : 1));
     int ctas = 1;
-    while (ctas < 8 && tiles * ctas < 6 * kSms && 2 * ctas * kFewWarps <= blocks) ctas *= 2;
-    const dim3 grid((unsigned)(tiles * ctas));
-    const int threads = kFewWarps * 32;
-    if (a.M <= 8) return launch_few(name, ffn_few_kernel<T, GATED, 1>, grid, threads, ctas, !GATED, st, a, ctas);
-    if (a.M <= 16) return launch_few(name, ffn_few_kernel<T, GATED, 2>, grid, threads, ctas, !GATED, st, a, ctas);
-    return launch_few(name, ffn_few_kernel<T, GATED, 4>, grid, threads, ctas, !GATED, st, a, ctas);
+    while (ctas < 8 && tiles * ctas < 6 * kSms && 2 * ctas * (rows ? 1 : kFewWarps) <= blocks) ctas *= 2;
+    auto go = [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      const dim3 grid((unsigned)(tiles * ctas));
+      const int threads = kFewWarps * 32;
+      return rows ? launch_few(name, ffn_few_kernel<T, GATED, NT, true>, grid, threads, ctas, !GATED, st, a, ctas)
+                  : launch_few(name, ffn_few_kernel<T, GATED, NT, false>, grid, threads, ctas, !GATED, st, a, ctas);
+    };
+    if (a.M <= 8) return go(std::integral_constant<int, 1>{});
+    if (a.M <= 16) return go(std::integral_constant<int, 2>{});
+    return go(std::integral_constant<int, 4>{});
   }
 }
 

@@ -155,6 +155,7 @@ struct GemmArgs {
   FastDiv per_batch, per_block, last_rows;
   int split;                 // 1: the last tiles are cut along K (Cut), partials to `partial`
   int act;
+  int cols;                  // GATED without pairs: output columns of a tile, a multiple of 16, at most BN / 2
   uint32_t operand_bf16;
   float* partial;
   // outputs: STORE: out[batch] [M][ldo] of T (+ bias); else panels of hidden, or dgate and dup:
@@ -918,6 +919,8 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_rank() : 0;
   constexpr uint32_t TMEM_COLS = 2 * ACC;
+  const int cols = GATED && !PAIR ? a.cols : COLS;
+  const uint32_t tx = GATED && !PAIR ? B_AT + (uint32_t)cols * 256u : (uint32_t)CTAS * STAGE;  // bytes of a stage
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -951,7 +954,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       while (ok && w.next(a)) {
         int z, mt, nt;
         tile_at(a, w.tile, z, mt, nt);
-        const int m0 = (mt * CTAS + rank) * BM, n0 = nt * COLS;
+        const int m0 = (mt * CTAS + rank) * BM, n0 = nt * cols;
         const int nb = PAIR && !GATED ? n0 + rank * (BN / 2) : n0;  // this CTA's part of the column operand
         int sg = w.kb0 / a.nk, kb = w.kb0 - sg * a.nk;
         for (int i = w.kb0; i < w.kb1; ++i) {
@@ -964,7 +967,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
           const uint32_t bar = PAIR ? in_first_cta(full(s)) : full(s);
           const CUtensorMap* ma = &maps.m[seg.a_map + z];
           const CUtensorMap* mb = &maps.m[seg.b_map];
-          if (rank == 0) mbar_arrive_expect_tx(full(s), CTAS * STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(full(s), tx);
           if (A == PANELS_MN) {
             load_panels<PAIR>(dst, ma, k, m0 >> 3, seg.a_plane, bar);
           } else if (A == PANELS_K) {
@@ -979,7 +982,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
             load_g<PAIR>(dst + B_AT, mb + rank, k, n0, seg.b_plane, bar);
           } else if (TWO) {
             tma_load_3d(dst + B_AT, mb, k, n0, seg.b_plane, bar);
-            tma_load_3d(dst + B_AT + COLS * 128, mb + 1, k, n0, seg.b_plane, bar);
+            tma_load_3d(dst + B_AT + cols * 128, mb + 1, k, n0, seg.b_plane, bar);
             if (RECOMP) {  // dy beside x, w_down (MN-major) beside the other two
               tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, bar);
               tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, bar);
@@ -1008,7 +1011,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * COLS : BN, a.operand_bf16 != 0, A_MN, B_MN);
+      const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * cols : BN, a.operand_bf16 != 0, A_MN, B_MN);
       const uint32_t idesc_dh = tcc::idesc_f16_major(BM, COLS, a.operand_bf16 != 0, false, true);
       int used = 0, done = 0;
       bool ok = true;
@@ -1069,7 +1072,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     constexpr int MINE = BLOCKS / STEP > 0 ? BLOCKS / STEP : 1;  // blocks of a warp (BLOCKS = 2: of two warps in four)
     const int first = RUNS ? (warp >> 2) * MINE : warp >> 2;
     constexpr int NEXT = RUNS ? 1 : STEP;
-    const int end = RUNS ? first + MINE : BLOCKS;
+    const int end = RUNS ? first + MINE : cols / CB;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     uint8_t* stage = staging + warp * STAGING;
     float* colf = reinterpret_cast<float*>(staging + EPI_WARPS * STAGING) + warp * 32;
@@ -1102,7 +1105,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     while (ok && w.next(a)) {
       int z, mt, nt;
       tile_at(a, w.tile, z, mt, nt);
-      const int n0 = nt * COLS;
+      const int n0 = nt * cols;
       const int row0 = (mt * CTAS + rank) * BM + q * 32;
       const int64_t row = (int64_t)row0 + lane;
       const bool row_in = row < a.M;
@@ -1210,7 +1213,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       T bias = from_f<T>(0.0f);
       if (use_bias) bias = bias_of(n0 + first * CB);
       SavedRaw<T> raw;
-      if (EPI == EPI_DGATE && first < BLOCKS && n0 + first * CB < a.N) raw.load(saved_block(first), lane);
+      if (EPI == EPI_DGATE && first < end && n0 + first * CB < a.N) raw.load(saved_block(first), lane);
       if constexpr (WIDE) {
         // this thread's sums, added up over the runs: at most two blocks
         constexpr int NB = BLOCKS > 4 ? 2 : 1;
@@ -1230,14 +1233,14 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
 #pragma unroll
           for (int k = 0; k < NB; ++k) {
             const int c = first + STEP * k;
-            if (c >= BLOCKS) break;
+            if (c >= end) break;
             float t[CB];
             tmem_load(acc + c * CB, t);
             tmem_wait(t);
 #pragma unroll
             for (int j = 0; j < CB; ++j) sum[k][j] += t[j];
             if constexpr (TWO) {
-              tmem_load(acc + COLS + c * CB, t);
+              tmem_load(acc + cols + c * CB, t);
               tmem_wait(t);
 #pragma unroll
               for (int j = 0; j < CB; ++j) sum_u[k][j] += t[j];
@@ -1255,7 +1258,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
           const int c = first + STEP * k;
-          if (c >= BLOCKS) break;
+          if (c >= end) break;
           if (k > 0 && use_bias) bias = bias_of(n0 + c * CB);
           if constexpr (EPI == EPI_DGATE) {
             if (k > 0 && n0 + c * CB < a.N) raw.load(saved_block(c), lane);
@@ -1272,7 +1275,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         // v: gate or plain sums or (DGATE) dhidden; u: up; dh: RECOMPUTE's dhidden
         auto read = [&](int c, float (&v)[CB], float (&u)[CB], float (&dh)[CB]) {
           tmem_load(acc + c * CB, v);
-          if (TWO) tmem_load(acc + COLS + c * CB, u);
+          if (TWO) tmem_load(acc + cols + c * CB, u);
           if (RECOMP) tmem_load(acc + 2 * COLS + c * CB, dh);
           tmem_wait(v);
           if (TWO) tmem_wait(u);

@@ -383,10 +383,11 @@ cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* s
   a.nk = (int)div_up(s.C, BK);
   const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, true, false, sizeof(T) == 4);
   if (!make_map(&maps.m[0], w.x, operand_bf16<T>(), ROWS_K, BM) ||
-      !make_map(&maps.m[1], w.wg, operand_bf16<T>(), ROWS_K, (uint32_t)plan.bn / 2) ||
-      !make_map(&maps.m[2], w.wu, operand_bf16<T>(), ROWS_K, (uint32_t)plan.bn / 2))
+      !make_map(&maps.m[1], w.wg, operand_bf16<T>(), ROWS_K, (uint32_t)plan.cols) ||
+      !make_map(&maps.m[2], w.wu, operand_bf16<T>(), ROWS_K, (uint32_t)plan.cols))
     return cudaErrorInvalidValue;
   set_tiles(a, plan.tiles_m, plan.tiles_n, 1);
+  a.cols = plan.cols;
   a.act = p.act;
   a.operand_bf16 = operand_bf16<T>();
   a.out[0] = const_cast<void*>(w.h.base);

@@ -43,6 +43,7 @@ struct GemmPlan {
   bool pair = false, split = false;
   int workers = 0;  // CTAs, or pairs of them
   int tiles_m = 0, tiles_n = 0;
+  int cols = 0;     // output columns of a tile
   size_t partial_bytes() const {
     return split ? ((size_t)workers + (size_t)tiles_m * tiles_n * 2) * BM * (pair ? 2 : 1) * bn * 4 : 0;
   }
@@ -87,7 +88,20 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
       best.workers = (int)(split ? all : std::min<int64_t>(tiles, all));
       best.tiles_m = (int)tm;
       best.tiles_n = (int)tn;
+      best.cols = cols;
     }
+  }
+  if (gated && M <= BM) {
+    // one row tile: its time is that of reading the weights, so the columns are
+    // spread over the SMs in as few waves as the widest tile allows
+    const int most = wide ? 64 : 128;
+    const int64_t waves = div_up(N, (int64_t)most * kSms);
+    best.pair = false;
+    best.bn = 2 * most;
+    best.cols = (int)std::min<int64_t>(most, round_up(div_up(N, kSms * waves), 16));
+    best.tiles_m = 1;
+    best.tiles_n = (int)div_up(N, best.cols);
+    best.workers = std::min(best.tiles_n, kSms);
   }
   return best;
 }
@@ -142,10 +156,16 @@ struct Carver {
   }
 };
 
-// Few rows and nothing to save: the weights are streamed (dcn_ffn_few.cuh).
+// Few rows and nothing to save: the weights are streamed into registers
+// (dcn_ffn_few.cuh).  From 9 rows on the legacy matrix instruction falls behind
+// the weights' arrival (4096 x 14336 in bf16, one call: 1 row 68 us, 8 rows 73,
+// 16 rows 100, 32 rows 153; the tile products 80 at any of these), but on small
+// weights, where launches count, it stays ahead (512 x 2048, 32 rows: 12 us
+// against 21).
 inline bool few_rows(const FfnProblem& p, bool save) {
   if (save || p.M > 32) return false;
-  return p.dtype == DCN_FLOAT32 || (p.C % 8 == 0 && p.F % 8 == 0);
+  if (p.dtype == DCN_FLOAT32) return p.M <= 8 || p.C * p.F <= (int64_t(1) << 22);
+  return p.C % 8 == 0 && p.F % 8 == 0 && (p.M <= 8 || p.C * p.F <= (int64_t(1) << 22));
 }
 
 struct ForwardWs {
