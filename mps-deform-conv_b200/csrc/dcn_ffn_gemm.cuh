@@ -155,7 +155,12 @@ struct GemmArgs {
   FastDiv per_batch, per_block, last_rows;
   int split;                 // 1: the last tiles are cut along K (Cut), partials to `partial`
   int act;
-  int cols;                  // GATED without pairs: output columns of a tile, a multiple of 16, at most BN / 2
+  // GATED, and STORE of ROWS_K columns, without pairs: output columns of a tile (a
+  // multiple of 16, at most the kernel's), bytes of the row operand in a stage and
+  // (panels) between its panels there.  With one row tile only the rows that exist
+  // are loaded; what the others hold is multiplied into results that are not stored.
+  int cols;
+  uint32_t a_bytes, a_lbo;
   uint32_t operand_bf16;
   float* partial;
   // outputs: STORE: out[batch] [M][ldo] of T (+ bias); else panels of hidden, or dgate and dup:
@@ -919,8 +924,9 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_rank() : 0;
   constexpr uint32_t TMEM_COLS = 2 * ACC;
-  const int cols = GATED && !PAIR ? a.cols : COLS;
-  const uint32_t tx = GATED && !PAIR ? B_AT + (uint32_t)cols * 256u : (uint32_t)CTAS * STAGE;  // bytes of a stage
+  constexpr bool FREE = !PAIR && (GATED || (EPI == EPI_STORE && B == ROWS_K));
+  const int cols = FREE ? a.cols : COLS;
+  const uint32_t tx = FREE ? a.a_bytes + (uint32_t)cols * (GATED ? 256u : 128u) : (uint32_t)CTAS * STAGE;  // of a stage
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -1011,7 +1017,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * cols : BN, a.operand_bf16 != 0, A_MN, B_MN);
+      const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * cols : FREE ? cols : BN, a.operand_bf16 != 0, A_MN, B_MN);
       const uint32_t idesc_dh = tcc::idesc_f16_major(BM, COLS, a.operand_bf16 != 0, false, true);
       int used = 0, done = 0;
       bool ok = true;
@@ -1034,7 +1040,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
               // panels in shared memory: K-major [panel][128 rows][16 B] (panels along K by
               // LBO, 8-row groups by SBO); MN-major [panel][64 rows][16 B] (8-row groups along
               // K by LBO, panels by SBO)
-              const uint64_t ad = A == PANELS_K    ? desc_panels(ab + kk * 4096, 2048, 128)
+              const uint64_t ad = A == PANELS_K    ? (FREE ? desc_panels(ab + kk * 2 * a.a_lbo, a.a_lbo, 128) : desc_panels(ab + kk * 4096, 2048, 128))
                                   : A == PANELS_MN ? desc_panels(ab + kk * 256, 128, 1024)
                                   : A == ROWS_MN   ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192)
                                                    : desc_kmajor_sw128(ab + kk * 32);
@@ -1072,7 +1078,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
     constexpr int MINE = BLOCKS / STEP > 0 ? BLOCKS / STEP : 1;  // blocks of a warp (BLOCKS = 2: of two warps in four)
     const int first = RUNS ? (warp >> 2) * MINE : warp >> 2;
     constexpr int NEXT = RUNS ? 1 : STEP;
-    const int end = RUNS ? first + MINE : cols / CB;
+    const int end = RUNS ? min(first + MINE, cols / CB) : cols / CB;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     uint8_t* stage = staging + warp * STAGING;
     float* colf = reinterpret_cast<float*>(staging + EPI_WARPS * STAGING) + warp * 32;
@@ -1120,6 +1126,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
       auto block = [&](int c, float (&v)[CB], float (&u)[CB], float (&dh)[CB], T bias) {
         const int c0 = n0 + c * CB;
         if (!whole) {
+          if (row0 >= a.M) return;
           // an fp32 partial of this tile, 16-byte pieces of 32 rows side by side
           float* slot = a.partial + ((int64_t)w.slot * CTAS + rank) * (BM * BN) + q * (32 * BN);
 #pragma unroll

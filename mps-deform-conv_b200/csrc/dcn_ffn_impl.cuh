@@ -294,6 +294,20 @@ int fill_segments(Seg* seg, const std::vector<std::pair<int, int>>& pairs) {
   return n;
 }
 
+// Rows of the row operand in a stage, and what the kernel is told of them
+// (GemmArgs): a tile's 128, or with one row tile those that exist.
+uint32_t row_box(GemmArgs& a, const GemmPlan& p, Form form, Form columns) {
+  a.cols = p.cols;
+  uint32_t rows = BM;
+  if (!p.pair && p.tiles_m == 1 && columns == ROWS_K) {
+    if (form == PANELS_K) rows = (uint32_t)round_up(a.M, 32);
+    if (form == ROWS_K) rows = (uint32_t)round_up(a.M, 8);
+  }
+  a.a_bytes = rows * 128;
+  a.a_lbo = rows * 16;
+  return rows;
+}
+
 template <typename T>
 constexpr bool operand_bf16() { return !std::is_same<T, __half>::value; }
 
@@ -313,11 +327,11 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   a.nseg = fill_segments<T>(a.seg, pl);
   a.M = (int)M; a.N = (int)N;
   a.nk = (int)div_up(K, BK);
-  const GemmPlan p = plan_gemm(M, N, (int64_t)a.nk * a.nseg, batches, false, true, sizeof(T) == 4);
+  const GemmPlan p = plan_gemm(M, N, (int64_t)a.nk * a.nseg, batches, false, true, sizeof(T) == 4, B == ROWS_K);
   for (int i = 0; i < n_a; ++i)
-    if (!make_map(&maps.m[i], a_ops[i], operand_bf16<T>(), A, BM)) return cudaErrorInvalidValue;
+    if (!make_map(&maps.m[i], a_ops[i], operand_bf16<T>(), A, row_box(a, p, A, B))) return cudaErrorInvalidValue;
   for (int i = 0; i < pairs; ++i)
-    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B, (uint32_t)(p.pair ? p.bn / 2 : p.bn)))
+    if (!make_map(&maps.m[n_a + i], b_ops[i], operand_bf16<T>(), B, (uint32_t)(p.pair ? p.bn / 2 : p.cols)))
       return cudaErrorInvalidValue;
   set_tiles(a, p.tiles_m, p.tiles_n, batches);
   a.split = p.split;
@@ -381,13 +395,12 @@ cudaError_t forward_t(const FfnProblem& p, const FfnTensors& t, void* y, void* s
   a.nseg = fill_segments<T>(a.seg, {{0, 1}});
   a.M = (int)s.M; a.N = (int)s.F;
   a.nk = (int)div_up(s.C, BK);
-  const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, true, false, sizeof(T) == 4);
-  if (!make_map(&maps.m[0], w.x, operand_bf16<T>(), ROWS_K, BM) ||
+  const GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, true, false, sizeof(T) == 4, true);
+  if (!make_map(&maps.m[0], w.x, operand_bf16<T>(), ROWS_K, row_box(a, plan, ROWS_K, ROWS_K)) ||
       !make_map(&maps.m[1], w.wg, operand_bf16<T>(), ROWS_K, (uint32_t)plan.cols) ||
       !make_map(&maps.m[2], w.wu, operand_bf16<T>(), ROWS_K, (uint32_t)plan.cols))
     return cudaErrorInvalidValue;
   set_tiles(a, plan.tiles_m, plan.tiles_n, 1);
-  a.cols = plan.cols;
   a.act = p.act;
   a.operand_bf16 = operand_bf16<T>();
   a.out[0] = const_cast<void*>(w.h.base);
@@ -425,7 +438,7 @@ cudaError_t backward_t(const FfnProblem& p, const FfnTensors& t, const void* dy,
     a.nseg = fill_segments<T>(a.seg, {{0, again ? 2 : 1}});
     a.M = (int)s.M; a.N = (int)s.F;
     a.nk = (int)div_up(s.C, BK);
-    GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, false, false, sizeof(T) == 4);
+    GemmPlan plan = plan_gemm(s.M, s.F, (int64_t)a.nk * a.nseg, 1, false, false, sizeof(T) == 4, false);
     bool ok;
     if (again) {
       plan.pair = false;

@@ -53,9 +53,12 @@ struct GemmPlan {
 // tile's time being its columns over the relative rate of that form (a narrower
 // or unpaired tile reads more operand rows for the same work).  splittable: the
 // product stores plain sums, so the tiles of a last wave that would leave many
-// SMs idle can be cut along K.
+// SMs idle can be cut along K.  weights: the column operand is a weight in rows
+// of the contracted axis; with one row tile 128 columns a stage keep its reads
+// long enough (4096 x 14336 in bf16, 16 rows: 64 columns, cut K 33 us; 32 columns
+// on 128 SMs, K whole 76 us).
 inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool gated, bool splittable,
-                          bool wide) {
+                          bool wide, bool weights) {
   struct Form {
     int bn;
     bool pair;
@@ -66,8 +69,10 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
   GemmPlan best;
   double best_cost = 1e300;
   const Form* forms = wide ? kWide : kNarrow;
+  const bool stream = weights && !gated && M <= BM;
   for (int i = 0; i < (wide ? 3 : 4); ++i) {
     const Form& f = forms[i];
+    if (stream && (f.pair || f.bn == 256)) continue;
     const int cols = gated ? f.bn / 2 : f.bn, rows = f.pair ? 2 * BM : BM, all = f.pair ? kSms / 2 : kSms;
     const int64_t tm = div_up(M, rows), tn = div_up(N, cols), tiles = tm * tn * batches;
     const double tile = f.bn / f.rate * (double)nkb;
@@ -92,11 +97,11 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
     }
   }
   if (gated && M <= BM) {
-    // one row tile: its time is that of reading the weights, so the columns are
+    // one row tile: its time is that of reading the weights, so their rows are
     // spread over the SMs in as few waves as the widest tile allows
     const int most = wide ? 64 : 128;
     const int64_t waves = div_up(N, (int64_t)most * kSms);
-    best.pair = false;
+    best.pair = best.split = false;
     best.bn = 2 * most;
     best.cols = (int)std::min<int64_t>(most, round_up(div_up(N, kSms * waves), 16));
     best.tiles_m = 1;
@@ -106,8 +111,8 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
   return best;
 }
 
-inline size_t store_partial_bytes(int64_t M, int64_t N, int64_t K, int nseg, int batches) {
-  return ws_align(plan_gemm(M, N, div_up(K, BK) * nseg, batches, false, true, nseg >= 6).partial_bytes());
+inline size_t store_partial_bytes(int64_t M, int64_t N, int64_t K, int nseg, int batches, bool weights = false) {
+  return ws_align(plan_gemm(M, N, div_up(K, BK) * nseg, batches, false, true, nseg >= 6, weights).partial_bytes());
 }
 
 // ---------------------------------------------------------------- layouts
@@ -189,7 +194,7 @@ struct ForwardWs {
     wu = s.operand(pack_c ? c.take(s.operand_bytes(s.F, s.C)) : t.w_up, s.F, s.C);
     wd = s.operand(pack_f ? c.take(s.operand_bytes(s.C, s.F)) : t.w_down, s.C, s.F);
     h = s.operand(hidden ? hidden : c.take(s.panels_bytes()), s.M, s.F);
-    partial = static_cast<float*>(c.take(store_partial_bytes(s.M, s.C, s.F, s.pair, 1)));
+    partial = static_cast<float*>(c.take(store_partial_bytes(s.M, s.C, s.F, s.pair, 1, true)));
     total = c.at;
   }
 };
