@@ -43,8 +43,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlockElems = 256;                          // elements of one 8-bit scale, and of one warp pass
-constexpr int kPasses = 4;                                // warp passes of one CTA
-constexpr int kChunk = kWarps * kBlockElems * kPasses;    // elements of one CTA
+constexpr int kRow = kWarps * kBlockElems;                // elements of one pass of a CTA
+// Passes of a CTA, at most: its prologue (the counters, the powers) is paid once
+// and 8-bit passes are fetched ahead; 32-bit states run at the memory's rate and
+// only pay for the longer tail (421 us at 4, 443 at 16 for 96.6 M bf16 parameters
+// with master copies; 8 bits: 454 at 4, 288 at 16).
+constexpr int kMostPasses = 16;
 
 struct AdamwEntry {
   void* param;
@@ -74,7 +78,8 @@ struct AdamwHyper {
 template <int N>
 struct AdamwArgs {
   AdamwHyper h;
-  uint32_t n, chunks;
+  uint32_t n;
+  int passes;  // of a CTA: a chunk is passes x kRow elements
   AdamwEntry e[N];
 };
 
@@ -87,28 +92,75 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-
-// e4m3 code of x in units of 2^(e - 7), |x| < 2^(e + 1): scaled by 2^-120 on
-// top, e4m3's smallest normal 2^-6 becomes fp32's 2^-126, so the top bits of
-// the fp32 pattern (subnormals included) are the code, and adding a word below
-// bit 20 before they are cut off rounds up with the remainder's probability.
-__device__ __forceinline__ uint32_t quantize(float x, float up, uint32_t word16) {
-  const float z = __fmul_rn(__fmul_rn(fabsf(x), up), 7.5231638452626401e-37f);  // 2^-120
-  uint32_t code = (__float_as_uint(z) + (word16 << 4)) >> 20;
-  if (!(fabsf(x) <= 3.402823466e38f)) code = 0x7f;
-  return code | ((__float_as_uint(x) >> 24) & 0x80u);
-}
+// Codes of a block's values, |x| < 2^(e + 1): x / 2^(e - 7) scaled by 2^-120 on
+// top, which puts e4m3's smallest normal 2^-6 at fp32's 2^-126, so that the top
+// bits of the fp32 pattern (subnormals included) are the code, and adding a word
+// below bit 20 before they are cut off rounds up with the remainder's
+// probability.  The two factors are one where 2^(-113 - e) is a normal number.
+struct CodeScale {
+  float first, second;
+  bool two, check;  // of the whole warp; check: the block holds inf or NaN
+  __device__ __forceinline__ CodeScale(int e, bool check_) : check(check_) {
+    two = e > 13;
+    first = __int_as_float((two ? 7 - e + 127 : -113 - e + 127) << 23);
+    second = two ? 7.5231638452626401e-37f : 1.0f;  // 2^-120
+  }
+  __device__ __forceinline__ uint32_t operator()(float x, uint32_t word16) const {
+    float z = __fmul_rn(fabsf(x), first);
+    if (two) z = __fmul_rn(z, second);
+    uint32_t code = (__float_as_uint(z) + (word16 << 4)) >> 20;
+    if (check && !(fabsf(x) <= 3.402823466e38f)) code = 0x7f;
+    return code;
+  }
+};
 
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.0f;
 }
-
-__device__ __forceinline__ int block_exponent(float top) {
+// max that keeps NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+// The block's exponent from the lanes' largest values (NaN kept: patterns of
+// non-negative floats, inf and NaN order as integers do); `bad`: not all finite.
+__device__ __forceinline__ int block_exponent(float top, const float (&x)[8], bool& bad) {
+  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
+  bad = bits >= 0x7f800000u;
+  if (bad) {  // the finite values' exponent
+    float t = 0.0f;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  return max(-100, (int)((__float_as_uint(top) >> 23) & 0xff) - 127);
+    for (int j = 0; j < 8; ++j) t = fmaxf(t, finite_abs(x[j]));
+    bits = __reduce_max_sync(0xffffffffu, __float_as_uint(t));
+  }
+  return max(-100, (int)(bits >> 23) - 127);
+}
+
+// Two fp32 operations an instruction, each rounded on its own as the scalar ones.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 twice(float a) { return make_float2(a, a); }
+// m / d for a positive normal d: the reciprocal is off by at most one unit in
+// the last place.
+__device__ __forceinline__ float rcp_fast(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
 }
 
 __device__ __forceinline__ float2 e4m3_pair(uint32_t two) {
@@ -116,20 +168,26 @@ __device__ __forceinline__ float2 e4m3_pair(uint32_t two) {
   return __half22float2(__half2(h));
 }
 
-// Eight elements of a tensor of element type T as floats.
+// Eight elements of a tensor of element type T, and as floats.
+template <typename T>
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    T t[8];
+    memcpy(t, v, sizeof(t));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = to_f<T>(t[j]);
+  }
+};
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    T t[8];
-    memcpy(t, &a, 16);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f<T>(t[j]);
-  }
+  Raw8<T> r;
+  r.load(p);
+  r.get(v);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
@@ -146,10 +204,36 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   }
 }
 
+// What a lane reads of a whole, aligned pass; fetched a pass ahead.
+template <typename T, bool MASTER, bool BITS8>
+struct AdamwRaw {
+  Raw8<T> g;
+  Raw8<std::conditional_t<MASTER, float, T>> p;
+  Raw8<float> m, v;   // 32-bit states
+  uint2 mc, vc;       // 8-bit states
+  float sm, sv;
+  __device__ __forceinline__ void load(const AdamwEntry& t, long long base, int lane) {
+    const long long i = base + 8 * lane;
+    g.load(static_cast<const T*>(t.grad) + i);
+    if constexpr (MASTER) p.load(t.master + i);
+    else p.load(static_cast<const T*>(t.param) + i);
+    if constexpr (BITS8) {
+      mc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.exp_avg) + i);
+      vc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.exp_avg_sq) + i);
+      sm = t.exp_avg_scale[base / kBlockElems];
+      sv = t.exp_avg_sq_scale[base / kBlockElems];
+    } else {
+      m.load(static_cast<const float*>(t.exp_avg) + i);
+      v.load(static_cast<const float*>(t.exp_avg_sq) + i);
+    }
+  }
+};
+
 // One warp's pass over elements [base, base + 256) of tensor `t`.
 template <typename T, bool MASTER, bool BITS8, bool VEC>
 __device__ __forceinline__ void adamw_pass(const AdamwEntry& t, const AdamwHyper& h, long long base, int lane,
-                                           float gs, float decay, float step_size, float corr, uint32_t key) {
+                                           float gs, float decay, float step_size, float corr, uint32_t key,
+                                           const AdamwRaw<T, MASTER, BITS8>& raw) {
   // lane's element j: VEC base + 8 lane + j, else base + lane + 32 j
   auto at = [&](int j) { return VEC ? base + 8 * lane + j : base + lane + 32 * j; };
   float g[8], p[8], m[8], r[8];   // r: v, then sqrt(v')
@@ -161,24 +245,21 @@ __device__ __forceinline__ void adamw_pass(const AdamwEntry& t, const AdamwHyper
   uint8_t* vc = static_cast<uint8_t*>(t.exp_avg_sq);
   const long long blk = base / kBlockElems;
   if (VEC) {
-    const long long i = base + 8 * lane;
-    load8<T>(grad + i, g);
-    if (MASTER) load8<float>(t.master + i, p);
-    else load8<T>(param + i, p);
-    if (BITS8) {
-      const uint2 a = *reinterpret_cast<const uint2*>(mc + i), b = *reinterpret_cast<const uint2*>(vc + i);
-      const float sm = t.exp_avg_scale[blk], sv = t.exp_avg_sq_scale[blk];
-      const uint32_t aw[4] = {a.x, a.x >> 16, a.y, a.y >> 16}, bw[4] = {b.x, b.x >> 16, b.y, b.y >> 16};
+    raw.g.get(g);
+    raw.p.get(p);
+    if constexpr (BITS8) {
+      const uint32_t aw[4] = {raw.mc.x, raw.mc.x >> 16, raw.mc.y, raw.mc.y >> 16};
+      const uint32_t bw[4] = {raw.vc.x, raw.vc.x >> 16, raw.vc.y, raw.vc.y >> 16};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = e4m3_pair(aw[j]), y = e4m3_pair(bw[j]);
-        m[2 * j] = __fmul_rn(x.x, sm); m[2 * j + 1] = __fmul_rn(x.y, sm);
-        const float y0 = __fmul_rn(y.x, sv), y1 = __fmul_rn(y.y, sv);
-        r[2 * j] = __fmul_rn(y0, y0); r[2 * j + 1] = __fmul_rn(y1, y1);
+        const float2 x = mul2(e4m3_pair(aw[j]), twice(raw.sm)), y = mul2(e4m3_pair(bw[j]), twice(raw.sv));
+        const float2 q = mul2(y, y);
+        m[2 * j] = x.x; m[2 * j + 1] = x.y;
+        r[2 * j] = q.x; r[2 * j + 1] = q.y;
       }
     } else {
-      load8<float>(mf + i, m);
-      load8<float>(vf + i, r);
+      raw.m.get(m);
+      raw.v.get(r);
     }
   } else {
     const float sm = BITS8 ? t.exp_avg_scale[blk] : 1.0f, sv = BITS8 ? t.exp_avg_sq_scale[blk] : 1.0f;
@@ -202,32 +283,38 @@ __device__ __forceinline__ void adamw_pass(const AdamwEntry& t, const AdamwHyper
   float mtop = 0.0f, rtop = 0.0f;
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float gj = __fmul_rn(g[j], gs);
-    m[j] = __fadd_rn(__fmul_rn(m[j], h.b1), __fmul_rn(gj, h.omb1));
-    v[j] = __fadd_rn(__fmul_rn(r[j], h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
-    r[j] = __fsqrt_rn(v[j]);
-    p[j] = p[j] * decay - step_size * __fdividef(m[j], r[j] * corr + h.eps);
-    if (BITS8) {
-      mtop = fmaxf(mtop, finite_abs(m[j]));
-      rtop = fmaxf(rtop, finite_abs(r[j]));
+  for (int j = 0; j < 8; j += 2) {
+    const float2 gj = mul2(make_float2(g[j], g[j + 1]), twice(gs));
+    const float2 mj = add2(mul2(make_float2(m[j], m[j + 1]), twice(h.b1)), mul2(gj, twice(h.omb1)));
+    const float2 vj = add2(mul2(make_float2(r[j], r[j + 1]), twice(h.b2)), mul2(mul2(gj, gj), twice(h.omb2)));
+    m[j] = mj.x; m[j + 1] = mj.y;
+    v[j] = vj.x; v[j + 1] = vj.y;
+#pragma unroll
+    for (int k = j; k < j + 2; ++k) {
+      r[k] = __fsqrt_rn(v[k]);
+      p[k] = p[k] * decay - step_size * (m[k] * rcp_fast(r[k] * corr + h.eps));
+      if (BITS8) {
+        mtop = max_nan(mtop, fabsf(m[k]));
+        rtop = max_nan(rtop, r[k]);
+      }
     }
   }
 
   uint32_t cm[8], cr[8];
   if (BITS8) {
-    const int em = block_exponent(mtop), er = block_exponent(rtop);
-    const float um = pow2i(7 - em), ur = pow2i(7 - er);
+    bool bad_m, bad_r;
+    const int em = block_exponent(mtop, m, bad_m), er = block_exponent(rtop, r, bad_r);
     if (lane == 0) {
       t.exp_avg_scale[blk] = pow2i(em - 7);
       t.exp_avg_sq_scale[blk] = pow2i(er - 7);
     }
+    const CodeScale qm(em, bad_m), qr(er, bad_r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t w = mix32((uint32_t)at(j) ^ key);
-      cm[j] = quantize(m[j], um, w & 0xffffu);
-      cr[j] = quantize(r[j], ur, w >> 16);
-      if (r[j] > 0.0f) cr[j] = max(cr[j], 1u);
+      cm[j] = qm(m[j], w & 0xffffu) | ((__float_as_uint(m[j]) >> 24) & 0x80u);
+      // a positive root keeps at least the smallest code
+      cr[j] = max(qr(r[j], w >> 16), min(__float_as_uint(r[j]), 1u));
     }
   }
 
@@ -262,15 +349,24 @@ __device__ __forceinline__ void adamw_pass(const AdamwEntry& t, const AdamwHyper
   }
 }
 
+// b^n in fp64 by squaring: at most 62 products where pow takes some 2 us; the
+// relative error, below n 2^-52, is far below what an fp32 correction keeps.
+__device__ __forceinline__ double power(double b, uint32_t n) {
+  double r = 1.0;
+#pragma unroll 1
+  for (; n; n >>= 1) {
+    if (n & 1) r *= b;
+    b *= b;
+  }
+  return r;
+}
+
 template <typename T, bool MASTER, bool BITS8, int N>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ AdamwArgs<N> a) {
   __shared__ float s_bias[3];     // decay, step size, 1 / sqrt(1 - b2^t)
   __shared__ uint32_t s_key;
   __shared__ bool s_last;
   const AdamwHyper& h = a.h;
-  const float gs = h.grad_scale ? *h.grad_scale : 1.0f;
-  if (!(fabsf(gs) <= 3.402823466e38f)) return;  // not finite: the whole step is skipped, nothing is written
-
   // the tensor of this CTA's chunk: the last entry that starts at or before it
   uint32_t lo = 0, hi = a.n - 1;
   while (lo < hi) {
@@ -279,27 +375,42 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     else hi = mid - 1;
   }
   const AdamwEntry& t = a.e[lo];
-  if (threadIdx.x == 0) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long start = (long long)(blockIdx.x - t.first_chunk) * a.passes * kRow + warp * kBlockElems;
+  auto whole = [&](int i) { return i < a.passes && t.vec && start + (long long)i * kRow + kBlockElems <= t.numel; };
+  AdamwRaw<T, MASTER, BITS8> raw;
+  // 32-bit states have enough in flight without it, and lose more by the registers
+  if (BITS8 && whole(0)) raw.load(t, start, lane);
+  if (lane == 0 && warp < 2) {  // the two corrections side by side
     const int step = t.step[0] + 1;
     const double lr = h.lr_device ? (double)*h.lr_device : h.lr;
-    s_bias[0] = (float)(1.0 - lr * h.weight_decay);
-    s_bias[1] = (float)(lr / (1.0 - pow(h.beta1, (double)step)));
-    s_bias[2] = (float)rsqrt(1.0 - pow(h.beta2, (double)step));
-    s_key = mix32(h.seed + (uint32_t)step * 0x9e3779b9u);
+    const double left = 1.0 - power(warp == 0 ? h.beta1 : h.beta2, (uint32_t)step);
+    if (warp == 0) {
+      s_bias[0] = (float)(1.0 - lr * h.weight_decay);
+      s_bias[1] = (float)(lr / left);
+      s_key = mix32(h.seed + (uint32_t)step * 0x9e3779b9u);
+    } else {
+      s_bias[2] = (float)rsqrt(left);
+    }
   }
+  // not finite: the whole step is skipped, nothing is written
+  const float gs = h.grad_scale ? *h.grad_scale : 1.0f;
   __syncthreads();
+  if (!(fabsf(gs) <= 3.402823466e38f)) return;
   const float decay = s_bias[0], step_size = s_bias[1], corr = s_bias[2];
   const uint32_t key = s_key;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long start = (long long)(blockIdx.x - t.first_chunk) * kChunk;
 #pragma unroll 1
-  for (int i = 0; i < kPasses; ++i) {
-    const long long base = start + (long long)(i * kWarps + warp) * kBlockElems;
+  for (int i = 0; i < a.passes; ++i) {
+    const long long base = start + (long long)i * kRow;
     if (base >= t.numel) break;
-    if (t.vec && base + kBlockElems <= t.numel)
-      adamw_pass<T, MASTER, BITS8, true>(t, h, base, lane, gs, decay, step_size, corr, key);
-    else
-      adamw_pass<T, MASTER, BITS8, false>(t, h, base, lane, gs, decay, step_size, corr, key);
+    if (whole(i)) {
+      if (!BITS8) raw.load(t, base, lane);
+      const AdamwRaw<T, MASTER, BITS8> now = raw;
+      if (BITS8 && whole(i + 1)) raw.load(t, base + kRow, lane);
+      adamw_pass<T, MASTER, BITS8, true>(t, h, base, lane, gs, decay, step_size, corr, key, now);
+    } else {
+      adamw_pass<T, MASTER, BITS8, false>(t, h, base, lane, gs, decay, step_size, corr, key, raw);
+    }
   }
 
   // every CTA has read its step counter before it takes a ticket, so the last
@@ -320,38 +431,51 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 template <typename T, bool MASTER, bool BITS8, int N>
-cudaError_t adamw_launch(const AdamwHyper& h, const AdamwEntry* e, uint32_t n, uint32_t chunks, cudaStream_t st) {
+cudaError_t adamw_launch(const AdamwHyper& h, const AdamwEntry* e, uint32_t n, uint32_t chunks, int passes,
+                         cudaStream_t st) {
   AdamwArgs<N> a;
   a.h = h;
   a.n = n;
-  a.chunks = chunks;
+  a.passes = passes;
   std::copy(e, e + n, a.e);
   KernelScope ks("adamw", st);
   adamw_kernel<T, MASTER, BITS8, N><<<std::max(1u, chunks), kThreads, 0, st>>>(a);
   return cudaGetLastError();
 }
 
-constexpr int kSmall = 12, kLarge = 384;  // entries of a launch: a layer's tensors, or what 32,764 bytes hold
+// Entries of a launch: a layer's tensors, some, many, or what 32,764 bytes of
+// arguments hold; the arguments of a small call take less time to send.
+constexpr int kLarge = 384;
 static_assert(sizeof(AdamwArgs<kLarge>) <= 32764, "kernel arguments");
 
 template <typename T, bool MASTER, bool BITS8>
 cudaError_t adamw_group(const AdamwHyper& h, const std::vector<AdamwEntry>& all, cudaStream_t st) {
+  // as many passes a CTA as leave eight CTAs an SM
+  unsigned long long total = 0;
+  for (const AdamwEntry& e : all) total += (unsigned long long)e.numel;
+  const int passes = (int)std::min<unsigned long long>(BITS8 ? kMostPasses : kMostPasses / 4, std::max<unsigned long long>(1, total / (kRow * 148ull * 8)));
+  const unsigned long long chunk = (unsigned long long)passes * kRow;
   // launches of at most kLarge tensors and 2^31 - 1 chunks (first_chunk restarts in each)
   size_t i = 0;
   while (i < all.size()) {
     std::vector<AdamwEntry> part;
     unsigned long long chunks = 0;
     while (i < all.size() && part.size() < (size_t)kLarge) {
-      const unsigned long long c = ((unsigned long long)all[i].numel + kChunk - 1) / kChunk;
+      const unsigned long long c = ((unsigned long long)all[i].numel + chunk - 1) / chunk;
       if (!part.empty() && chunks + c > 0x7fffffffull) break;
       part.push_back(all[i]);
       part.back().first_chunk = (uint32_t)chunks;
       chunks += c;
       ++i;
     }
-    const cudaError_t e = part.size() <= (size_t)kSmall
-                              ? adamw_launch<T, MASTER, BITS8, kSmall>(h, part.data(), (uint32_t)part.size(), (uint32_t)chunks, st)
-                              : adamw_launch<T, MASTER, BITS8, kLarge>(h, part.data(), (uint32_t)part.size(), (uint32_t)chunks, st);
+    auto go = [&](auto cap) {
+      return adamw_launch<T, MASTER, BITS8, decltype(cap)::value>(h, part.data(), (uint32_t)part.size(), (uint32_t)chunks,
+                                                                  passes, st);
+    };
+    const cudaError_t e = part.size() <= 12   ? go(std::integral_constant<int, 12>{})
+                          : part.size() <= 48 ? go(std::integral_constant<int, 48>{})
+                          : part.size() <= 144 ? go(std::integral_constant<int, 144>{})
+                                               : go(std::integral_constant<int, kLarge>{});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -439,8 +563,9 @@ struct NormArgs {
   uint32_t n, chunks;
   NormEntry e[N];
 };
-constexpr int kNormChunk = kThreads * 8 * 4;
-constexpr int kNormSmall = 32, kNormLarge = 1300;
+constexpr int kNormLoads = 8;  // of a thread, in flight together
+constexpr int kNormChunk = kThreads * 8 * kNormLoads;
+constexpr int kNormLarge = 1300;
 static_assert(sizeof(NormArgs<kNormLarge>) <= 32764, "kernel arguments");
 constexpr unsigned kNormCtas = 148 * 8;  // one wave of eight 256-thread CTAs per SM
 
@@ -460,15 +585,23 @@ __device__ __forceinline__ double norm_chunk(const NormEntry& t, long long start
   const T* p = static_cast<const T*>(t.data);
   double acc = 0.0;
   if (t.vec && start + kNormChunk <= t.numel) {
-    float v[4][8];
+    constexpr int kHalf = kNormLoads / ((int)sizeof(T) / 2);  // fp32: 16-byte loads twice as many
+    Raw8<T> r[kHalf];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load8<T>(p + start + (i * kThreads + threadIdx.x) * 8, v[i]);
+    for (int k = 0; k < kNormLoads; k += kHalf) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc += sum_squares(v[i]);
+      for (int i = 0; i < kHalf; ++i) r[i].load(p + start + ((k + i) * kThreads + threadIdx.x) * 8);
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) {
+        float v[8];
+        r[i].get(v);
+        acc += sum_squares(v);
+      }
+    }
     return acc;
   }
 #pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kNormLoads; ++i) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -495,6 +628,7 @@ __device__ __forceinline__ double cta_sum(double x) {
 
 template <int N>
 __global__ void __launch_bounds__(kThreads) grad_norm_partial_kernel(const __grid_constant__ NormArgs<N> a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   double acc = 0.0;
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
     uint32_t lo = 0, hi = a.n - 1;
@@ -515,6 +649,8 @@ __global__ void __launch_bounds__(kThreads) grad_norm_partial_kernel(const __gri
 
 __global__ void __launch_bounds__(kThreads) grad_norm_finish_kernel(const double* partial, unsigned n, double max_norm,
                                                                     double loss_scale, float* norm, float* factor) {
+  // launched beside the partial sums; waits for them here
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   double acc = 0.0;
   for (unsigned i = threadIdx.x; i < n; i += kThreads) acc += partial[i];
   const double s = cta_sum(acc);
@@ -585,15 +721,26 @@ cudaError_t grad_norm(const dcn_tensor_ref* t, int64_t n, double max_norm, doubl
       e[k] = {r.data, r.numel, chunk, (uint16_t)r.dtype, (uint16_t)aligned(r.data, 16)};
       chunk += (uint32_t)((r.numel + kNormChunk - 1) / kNormChunk);
     }
-    const cudaError_t err = p.count <= kNormSmall
-                                ? norm_launch<kNormSmall>(e.data(), (uint32_t)p.count, chunk, p.ctas, partial + used, st)
-                                : norm_launch<kNormLarge>(e.data(), (uint32_t)p.count, chunk, p.ctas, partial + used, st);
+    auto go = [&](auto cap) {
+      return norm_launch<decltype(cap)::value>(e.data(), (uint32_t)p.count, chunk, p.ctas, partial + used, st);
+    };
+    const cudaError_t err = p.count <= 32    ? go(std::integral_constant<int, 32>{})
+                            : p.count <= 160 ? go(std::integral_constant<int, 160>{})
+                                             : go(std::integral_constant<int, kNormLarge>{});
     if (err != cudaSuccess) return err;
     used += p.ctas;
   }
   KernelScope ks("grad_norm_finish", st);
-  grad_norm_finish_kernel<<<1, kThreads, 0, st>>>(partial, used, max_norm, loss_scale, norm, factor);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = used ? 1 : 0;  // no partial sums: nothing to overlap with
+  return cudaLaunchKernelEx(&cfg, grad_norm_finish_kernel, (const double*)partial, used, max_norm, loss_scale, norm, factor);
 }
 
 }  // namespace dcn
