@@ -65,7 +65,7 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
     double rate;
   };
   static const Form kNarrow[4] = {{256, true, 1.0}, {256, false, 0.8}, {128, false, 0.65}, {64, false, 0.4}};
-  static const Form kWide[3] = {{128, true, 1.0}, {128, false, 0.8}, {64, false, 0.5}};  // fp32 sums live in registers
+  static const Form kWide[3] = {{128, true, 1.0}, {128, false, 0.85}, {64, false, 0.65}};  // fp32 sums live in registers
   GemmPlan best;
   double best_cost = 1e300;
   const Form* forms = wide ? kWide : kNarrow;
@@ -79,7 +79,8 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
     double cost = (double)div_up(tiles, all) * tile;
     bool split = false;
     if (splittable && tiles < 4 * all && tiles * nkb >= 8 * all) {
-      const double cut = (double)tiles / all * tile + 24.0 * f.bn;  // + writing and adding partials
+      // + writing and adding partials, some 10 us
+      const double cut = (double)tiles / all * tile + (wide ? 48.0 : 40.0) * f.bn;
       if (cut < 0.95 * cost) {
         split = true;
         cost = cut;
