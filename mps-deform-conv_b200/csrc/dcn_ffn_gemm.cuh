@@ -339,7 +339,7 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
-// Two fp32 operations an instruction (each rounded as the scalar one).
+// Two fp32 operations an instruction (a product and a sum may be fused).
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));

@@ -139,18 +139,11 @@ __device__ __forceinline__ int block_exponent(float top, const float (&x)[8], bo
   return max(-100, (int)(bits >> 23) - 127);
 }
 
-// Two fp32 operations an instruction, each rounded on its own as the scalar ones.
+// Two fp32 products an instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
       "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
       : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
@@ -283,20 +276,16 @@ __device__ __forceinline__ void adamw_pass(const AdamwEntry& t, const AdamwHyper
   float mtop = 0.0f, rtop = 0.0f;
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const float2 gj = mul2(make_float2(g[j], g[j + 1]), twice(gs));
-    const float2 mj = add2(mul2(make_float2(m[j], m[j + 1]), twice(h.b1)), mul2(gj, twice(h.omb1)));
-    const float2 vj = add2(mul2(make_float2(r[j], r[j + 1]), twice(h.b2)), mul2(mul2(gj, gj), twice(h.omb2)));
-    m[j] = mj.x; m[j + 1] = mj.y;
-    v[j] = vj.x; v[j + 1] = vj.y;
-#pragma unroll
-    for (int k = j; k < j + 2; ++k) {
-      r[k] = __fsqrt_rn(v[k]);
-      p[k] = p[k] * decay - step_size * (m[k] * rcp_fast(r[k] * corr + h.eps));
-      if (BITS8) {
-        mtop = max_nan(mtop, fabsf(m[k]));
-        rtop = max_nan(rtop, r[k]);
-      }
+  for (int k = 0; k < 8; ++k) {
+    // scalar intrinsics: products and sums in pairs (f32x2) may be fused
+    const float gk = __fmul_rn(g[k], gs);
+    m[k] = __fadd_rn(__fmul_rn(m[k], h.b1), __fmul_rn(gk, h.omb1));
+    v[k] = __fadd_rn(__fmul_rn(r[k], h.b2), __fmul_rn(__fmul_rn(gk, gk), h.omb2));
+    r[k] = __fsqrt_rn(v[k]);
+    p[k] = p[k] * decay - step_size * (m[k] * rcp_fast(r[k] * corr + h.eps));
+    if (BITS8) {
+      mtop = max_nan(mtop, fabsf(m[k]));
+      rtop = max_nan(rtop, r[k]);
     }
   }
 

@@ -366,6 +366,87 @@ def test_graph_capture_and_streams(cuda):
     assert all(torch.equal(a, b) for a, b in zip(got[1:], eager))
 
 
+def test_few_rows_captured_and_on_two_streams(cuda):
+    """The dependent launches of the few-row kernels replay from a graph, and two streams at once keep apart."""
+    calls = []
+    for m, c, f, dt in ((1, 512, 2048, torch.bfloat16), (8, 1024, 264, torch.float16), (5, 96, 200, torch.float32)):
+        args, _ = _inputs(m, c, f, dt, cuda, True, seed=m)
+        calls.append(args)
+    want = [_run(a, None, "gelu")[0] for a in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        outs = [mdc.gated_feed_forward(*a, activation="gelu") for a in calls for _ in range(3)]
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        assert all(torch.equal(o, want[i // 3]) for i, o in enumerate(outs))
+    for k, args in enumerate(calls):  # new data in the captured inputs
+        args[0].mul_(-0.5)
+    graph.replay()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, _run(calls[i // 3], None, "gelu")[0])
+    big, dy = _inputs(3000, 320, 640, torch.bfloat16, cuda, True, seed=30)
+    ref = _run(big, dy, "silu")
+    small = _run(calls[0], None, "silu")[0]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got, few = [], []
+    for _ in range(5):
+        with torch.cuda.stream(streams[0]):
+            got.append(_run(big, dy, "silu"))
+        with torch.cuda.stream(streams[1]):
+            few += [_run(calls[0], None, "silu")[0] for _ in range(10)]
+            got.append(_run(big, dy, "silu"))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, ref))
+    assert all(torch.equal(o, small) for o in few)
+
+
+def test_captured_training_step_of_a_block(cuda):
+    """Deformable layer, gated block, gradient norm and AdamW in one graph: replayed steps leave the parameters
+    of the same steps taken one call at a time (forward and weight gradients are reproducible; the offsets'
+    gradients, summed by atomics, do not reach a parameter here)."""
+    def make():
+        torch.manual_seed(5)
+        layer = mdc.DeformConv2d(64, 64, 3, padding=1).to(cuda, torch.bfloat16)
+        block = mdc.GatedFeedForward2d(64, 160).to(cuda, torch.bfloat16)
+        params = [*layer.parameters(), *block.parameters()]
+        return layer, block, params, mdc.optim.AdamW(params, lr=1e-2, state_bits=8, master_weights=True, seed=9)
+
+    g = torch.Generator(cuda).manual_seed(1)
+    x = torch.randn(2, 64, 9, 8, generator=g, device=cuda).to(torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    off = torch.randn(2, 18, 9, 8, generator=g, device=cuda).to(torch.bfloat16)
+    go = torch.randn(2, 64, 9, 8, generator=g, device=cuda).to(torch.bfloat16)
+
+    def step(layer, block, params, opt):
+        for p in params:
+            p.grad = None
+        block(layer(x, off)).backward(go)
+        _, factor = mdc.optim.grad_norm([p.grad for p in params], max_norm=1.0)
+        opt.step(grad_scale=factor)
+
+    eager = make()
+    for _ in range(6):
+        step(*eager)
+    replayed = make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*replayed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*replayed)
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    for p, q in zip(eager[2], replayed[2]):
+        assert torch.equal(p, q)
+        assert eager[3].state[p]["step"].tolist() == [6, 0] == replayed[3].state[q]["step"].tolist()
+
+
 def test_parameter_gradient_hook(cuda):
     args, dy = _inputs(130, 32, 40, torch.float32, cuda, True, seed=15)
     want = _run(args, dy, "silu")

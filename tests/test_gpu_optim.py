@@ -131,6 +131,22 @@ def test_adamw_32bit_states(dtype, master, misalign, scaled, cuda):
         assert s["steps"][k].tolist() == [taken[k] + 1, 0]
 
 
+@pytest.mark.parametrize("scaled", [False, True])
+def test_adamw_states_round_each_product_and_sum(scaled, cuda):
+    """fp32 states are bit for bit those of separate fp32 products and sums."""
+    s = _inputs([100000, 70001], torch.float32, cuda, seed=21)
+    f = torch.tensor(0.37) if scaled else torch.tensor(1.0)
+    b1, b2 = HYPER["betas"]
+    want = []
+    for g, m, v in zip(s["grads"], s["exp_avgs"], s["exp_avg_sqs"]):
+        g, m, v = g.cpu() * f, m.cpu(), v.cpu()
+        want.append((m * torch.tensor(b1) + g * torch.tensor(1 - b1),
+                     v * torch.tensor(b2) + (g * g) * torch.tensor(1 - b2)))
+    _call(s, grad_scale=f.to(cuda) if scaled else None)
+    for k, (m, v) in enumerate(want):
+        assert torch.equal(s["exp_avgs"][k].cpu(), m) and torch.equal(s["exp_avg_sqs"][k].cpu(), v)
+
+
 # ---------------------------------------------------------------- 8-bit states
 M32 = 0xFFFFFFFF
 
