@@ -459,6 +459,10 @@ static bool encode_tmap(CUtensorMap* map, const void* base, bool bf16, int rank,
                         const cuuint64_t* strides, const cuuint32_t* box,
                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   const EncodeFn encode = tmap_encoder();
+  // the driver's encoder needs a current context, which a thread that has made no
+  // runtime call yet (autograd's, say) lacks; cudaSetDevice makes the device's current
+  int dev = 0;
+  if (!current_context() && (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)) return false;
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return encode &&
          encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,

@@ -366,6 +366,32 @@ def test_graph_capture_and_streams(cuda):
     assert all(torch.equal(a, b) for a, b in zip(got[1:], eager))
 
 
+@pytest.mark.parametrize("size", [(300, 64, 96), (40, 512, 200), (3, 64, 96)], ids=str)
+def test_first_call_of_a_thread(size, cuda):
+    """A thread that has made no CUDA call yet has no current context; forward and backward work all the same."""
+    import threading
+    args, dy = _inputs(*size, torch.bfloat16, cuda, True, seed=33)
+    want = _run(args, dy, "silu")
+    _, saved = mdc._get_lib().gated_feed_forward_forward(*args, 0, True, False)
+    torch.cuda.synchronize()
+    out = {}
+
+    def forward():
+        out["y"] = mdc._get_lib().gated_feed_forward_forward(*args, 0)[0]
+
+    def backward():
+        out["g"] = mdc._get_lib().gated_feed_forward_backward(dy, *args, 0, saved, [True] * 7)
+
+    for f in (forward, backward):
+        t = threading.Thread(target=f)
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    few = _run(args, None, "silu")[0]  # nothing saved: the form of few rows, where it applies
+    assert torch.equal(out["y"], few)
+    assert all(torch.equal(a, b) for a, b in zip(out["g"], want[1:]))
+
+
 def test_few_rows_captured_and_on_two_streams(cuda):
     """The dependent launches of the few-row kernels replay from a graph, and two streams at once keep apart."""
     calls = []
