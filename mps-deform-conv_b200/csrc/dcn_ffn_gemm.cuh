@@ -21,11 +21,12 @@
 // holds columns 8 p .. 8 p + 7, 16 bytes a row, and the panels of the 128 rows
 // follow one another (a tile is one run of memory).  The lanes of an epilogue
 // warp are rows, so they store 512 contiguous bytes an instruction from their
-// registers, where a row-major matrix needs staging and a TMA store whose rows
-// are 32 bytes (these row requests, beside the operands', held the TMA up: the
-// dhidden pass of 92416 x 2048 in bf16 took 440 us).  Eight rows
-// of a panel are 128 contiguous bytes, the matrix unit's 8 x 16-byte core
-// matrix without swizzle, read K-major or MN-major as a product needs it.
+// registers, where a row-major matrix needs staging in shared memory, a proxy
+// fence and TMA stores with short rows (measured: gate and up of 92416 x 512 ->
+// 2048 in bf16 437 -> 402 us, dhidden of 921600 x 64 -> 170 in fp16 249 -> 217,
+// of 8192 x 128 -> 512 in fp32 66 -> 46).  Eight rows of a panel are 128
+// contiguous bytes, the matrix unit's 8 x 16-byte core matrix without swizzle,
+// read K-major or MN-major as a product needs it.
 //
 // Warp roles (640 threads): warps 0-15 epilogue, warp 16 issues the MMAs, warp
 // 17 the TMA loads.  A CTA works through its share of the output tiles; the
@@ -33,10 +34,15 @@
 // next tile's MMAs.  Epilogue warp w reads TMEM lanes 32 (w % 4) .. +31: lane i
 // owns one row, 16 columns at a time, and takes blocks w / 4, w / 4 + 4, ... of
 // the tile.  A block's sums are read while the one before is worked on, and the
-// buffer goes back to the MMAs once the last has been read: held to the end of
-// the epilogue, a buffer's products and its epilogue exclude each other, and a
-// tile takes half of their sum (8460 cycles where the products take 4100 and
-// the gated epilogue 5500, 23104 x 512 -> 2048 rows in bf16).
+// buffer goes back to the MMAs once the last has been read; held to the end of
+// the epilogue, a buffer's products and its epilogue would exclude each other.
+//
+// What bounds it: products with a long K the tensor cores, at 1.3 to 1.45
+// PFLOP/s in bf16 until the power cap is reached.  The gated epilogues have some
+// 30 instructions a value pair and two special functions, 16 warps issue about
+// half of the cycles, and a tile of 128 x 128 pairs takes them some 5500 cycles:
+// as long as the products at K = 700, so below that they set the pace
+// (27200 x 256 -> 1024: 45 us with relu, 55 with gelu; the products alone 18).
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along
@@ -52,10 +58,8 @@
 // (tcgen05 cta_group::2).  Each holds its own 128 rows of the row operand, half
 // of the column operand (GATED: one gate, the other up) and the accumulator of
 // its rows; the first issues the MMAs for both.  A CTA alone reads 384 operand
-// rows for 128 x 256 results, a pair 512 for 256 x 256: the single-CTA products
-// were bound by their operand reads from the L2 (about 15 TB/s; everything an
-// epilogue wrote came on top of the products' time), and a pair reads a third
-// less.  Loads go to the CTA's own shared memory and report to the first CTA's
+// rows for 128 x 256 results, a pair 512 for 256 x 256, a third less (92416 x 512
+// -> 2048 in bf16: dx 284 -> 266 us, weight gradients 446 -> 413).  Loads go to the CTA's own shared memory and report to the first CTA's
 // barrier; commits arrive at both.
 //
 // Every mbarrier wait is bounded (dcn_sm100.cuh).
@@ -339,33 +343,6 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
-// Two fp32 operations an instruction (a product and a sum may be fused).
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 parts(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t twice(float a) { return pair_of(a, a); }
 template <bool ACCURATE>
 __device__ __forceinline__ float sigmoid(float x) {
   // far below zero the exponential overflows to inf and the quotient is 0, as it should be
@@ -414,99 +391,20 @@ __device__ __forceinline__ float2 act_both(float x) {
     return make_float2(s, s * (1.0f - s));
   }
 }
-// The fast forms on two values.
-__device__ __forceinline__ uint64_t sigmoid2(uint64_t x) {
-  const float2 e = parts(mul2(x, twice(-kLog2e)));
-  const float2 d = parts(add2(pair_of(exp2_fast(e.x), exp2_fast(e.y)), twice(1.0f)));
-  return pair_of(rcp_fast(d.x), rcp_fast(d.y));
-}
-struct Cdf2 {
-  uint64_t cdf, e;
-};
-__device__ __forceinline__ Cdf2 normal_cdf2(uint64_t x) {
-  const float2 xs = parts(x);
-  const uint64_t z = pair_of(fabsf(xs.x), fabsf(xs.y));
-  const float2 d = parts(fma2(twice(0.308f), z, twice(1.0f)));
-  const uint64_t t = pair_of(rcp_fast(d.x), rcp_fast(d.y));
-  const float2 q = parts(mul2(mul2(x, x), twice(-0.5f * kLog2e)));
-  const uint64_t e = pair_of(exp2_fast(q.x), exp2_fast(q.y));
-  uint64_t r = fma2(t, twice(-0.0754310913f), twice(0.189621131f));
-  r = fma2(t, r, twice(0.00726954421f));
-  r = fma2(t, r, twice(0.136535319f));
-  r = fma2(t, r, twice(0.118880802f));
-  r = fma2(t, r, twice(0.123122739f));
-  const uint64_t low2 = mul2(e, mul2(t, r));
-  const float2 low = parts(low2), high = parts(fma2(low2, twice(-1.0f), twice(1.0f)));
-  return {pair_of(xs.x > 0.0f ? high.x : low.x, xs.y > 0.0f ? high.y : low.y), e};
-}
-template <int ACT>
-__device__ __forceinline__ uint64_t act_value2(uint64_t x) {
-  if constexpr (ACT == kActSilu) return mul2(x, sigmoid2(x));
-  else if constexpr (ACT == kActGelu) return mul2(x, normal_cdf2(x).cdf);
-  else if constexpr (ACT == kActSigmoid) return sigmoid2(x);
-  else {
-    const float2 f = parts(x);
-    return pair_of(act_value<false, kActRelu>(f.x), act_value<false, kActRelu>(f.y));
-  }
-}
-template <int ACT>
-__device__ __forceinline__ void act_both2(uint64_t x, uint64_t& a, uint64_t& da) {
-  if constexpr (ACT == kActSilu) {
-    const uint64_t s = sigmoid2(x);
-    a = mul2(x, s);
-    da = fma2(a, fma2(s, twice(-1.0f), twice(1.0f)), s);
-  } else if constexpr (ACT == kActGelu) {
-    const Cdf2 c = normal_cdf2(x);
-    a = mul2(x, c.cdf);
-    da = fma2(x, mul2(twice(0.39894228040143268f), c.e), c.cdf);
-  } else if constexpr (ACT == kActSigmoid) {
-    a = sigmoid2(x);
-    da = mul2(a, fma2(a, twice(-1.0f), twice(1.0f)));
-  } else {
-    const float2 f = parts(x);
-    const float2 p = act_both<false, kActRelu>(f.x), q = act_both<false, kActRelu>(f.y);
-    a = pair_of(p.x, q.x);
-    da = pair_of(p.y, q.y);
-  }
-}
-
 // A row's block at a time; the activation is picked once for all of it.
 template <bool ACCURATE, int ACT>
 __device__ __forceinline__ void gate_block(const float (&g)[CB], const float (&u)[CB], float (&h)[CB]) {
 #pragma unroll
-  for (int j = 0; j < CB; j += 2) {
-    if constexpr (ACCURATE) {
-      h[j] = act_value<true, ACT>(g[j]) * u[j];
-      h[j + 1] = act_value<true, ACT>(g[j + 1]) * u[j + 1];
-    } else {
-      const float2 r = parts(mul2(act_value2<ACT>(pair_of(g[j], g[j + 1])), pair_of(u[j], u[j + 1])));
-      h[j] = r.x;
-      h[j + 1] = r.y;
-    }
-  }
+  for (int j = 0; j < CB; ++j) h[j] = act_value<ACCURATE, ACT>(g[j]) * u[j];
 }
 // (gate, up) to (dgate, dup)
 template <bool ACCURATE, int ACT>
 __device__ __forceinline__ void dgate_block(const float (&dh)[CB], float (&g)[CB], float (&u)[CB]) {
 #pragma unroll
-  for (int j = 0; j < CB; j += 2) {
-    if constexpr (ACCURATE) {
-#pragma unroll
-      for (int k = j; k < j + 2; ++k) {
-        const float2 s = act_both<true, ACT>(g[k]);
-        g[k] = dh[k] * u[k] * s.y;
-        u[k] = dh[k] * s.x;
-      }
-    } else {
-      uint64_t a, da;
-      act_both2<ACT>(pair_of(g[j], g[j + 1]), a, da);
-      const uint64_t d = pair_of(dh[j], dh[j + 1]);
-      const float2 x = parts(mul2(mul2(d, pair_of(u[j], u[j + 1])), da)), y = parts(mul2(d, a));
-      g[j] = x.x;
-      g[j + 1] = x.y;
-      u[j] = y.x;
-      u[j + 1] = y.y;
-    }
+  for (int j = 0; j < CB; ++j) {
+    const float2 s = act_both<ACCURATE, ACT>(g[j]);
+    g[j] = dh[j] * u[j] * s.y;
+    u[j] = dh[j] * s.x;
   }
 }
 template <bool ACCURATE>
@@ -746,17 +644,15 @@ __device__ __forceinline__ void stage_sums(uint8_t* rows, int lane, int at, cons
 template <typename T>
 __device__ __forceinline__ void staged_column_sums(const uint8_t* rows, int lane, float (&sum)[4]) {
   const int piece = lane & 7;
-  uint64_t lo = twice(0.0f), hi = twice(0.0f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = (lane >> 3) + 4 * i;
     const uint2 p = *reinterpret_cast<const uint2*>(rows + r * 64 + (((piece + r) & 7) << 3));
     const float2 x = tcc::Vec<T>::unpack(p.x), y = tcc::Vec<T>::unpack(p.y);
-    lo = add2(lo, pair_of(x.x, x.y));
-    hi = add2(hi, pair_of(y.x, y.y));
+    sum[0] += x.x; sum[1] += x.y; sum[2] += y.x; sum[3] += y.y;
   }
-  const float2 x = parts(lo), y = parts(hi);
-  sum[0] = x.x; sum[1] = x.y; sum[2] = y.x; sum[3] = y.y;
 #pragma unroll
   for (int o = 8; o <= 16; o <<= 1)
 #pragma unroll
@@ -1143,13 +1039,11 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
 #pragma unroll
           for (int j = 0; j < CB / 4; ++j) {
             const float4 f = reinterpret_cast<const float4*>(colf)[j];
-            auto add4 = [&](float (&t)[CB], const float4& b) {
-              const float2 lo = parts(add2(pair_of(t[4 * j], t[4 * j + 1]), pair_of(b.x, b.y)));
-              const float2 hi = parts(add2(pair_of(t[4 * j + 2], t[4 * j + 3]), pair_of(b.z, b.w)));
-              t[4 * j] = lo.x; t[4 * j + 1] = lo.y; t[4 * j + 2] = hi.x; t[4 * j + 3] = hi.y;
-            };
-            add4(v, f);
-            if (TWO) add4(u, reinterpret_cast<const float4*>(colf + CB)[j]);
+            v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+            if (TWO) {
+              const float4 h = reinterpret_cast<const float4*>(colf + CB)[j];
+              u[4 * j] += h.x; u[4 * j + 1] += h.y; u[4 * j + 2] += h.z; u[4 * j + 3] += h.w;
+            }
           }
         }
         // this row in the panels of the block's columns; rows past M are zero

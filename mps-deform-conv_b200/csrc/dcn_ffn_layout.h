@@ -165,7 +165,7 @@ struct Carver {
 // Few rows and nothing to save: the weights are streamed into registers
 // (dcn_ffn_few.cuh).  From 9 rows on the legacy matrix instruction falls behind
 // the weights' arrival (4096 x 14336 in bf16, one call: 1 row 68 us, 8 rows 73,
-// 16 rows 100, 32 rows 153; the tile products 80 at any of these), but on small
+// 16 rows 100, 32 rows 153; the tile products 77 at any of these), but on small
 // weights, where launches count, it stays ahead (512 x 2048, 32 rows: 12 us
 // against 21).
 inline bool few_rows(const FfnProblem& p, bool save) {
