@@ -410,6 +410,8 @@ DCN_API int dcn_ffn_backward(const dcn_ffn_desc *desc, const dcn_ffn_tensors *t,
  * that is 0 between calls; tensors may share one.  The call advances each
  * counter by one.  All tensors of one call are stepped together; calls that
  * share tensors or counters must not overlap on the GPU.
+ * Refused: written memory (parameters, master copies, states, counters) that
+ * overlaps other written memory, a gradient, grad_scale or lr_device.
  * grad_scale (one fp32 on the device, or NULL for 1) multiplies the
  * gradients; when it is not finite the whole step is skipped and nothing is
  * written, counters included.  lr_device (one fp32 on the device), when not

@@ -71,12 +71,39 @@ static int check_adamw(const dcn_adamw_options* o, const dcn_adamw_tensor* t, in
       add(e.exp_avg_sq_scale, (e.numel + 255) / 256 * 4);
     }
   }
-  // two CTAs must not update the same memory
+  // two CTAs must not update the same memory, nor one read what another updates
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i].first < written[i - 1].second)
       return fail(DCN_ERR_INVALID_ARGUMENT,
                   "parameters, master copies and states must not overlap one another (the same tensor twice?)");
+  auto meets = [&](const void* p, int64_t bytes) {
+    const uintptr_t a = (uintptr_t)p;
+    // the first range that starts at or past the end; the one before it reaches furthest
+    auto it = std::lower_bound(written.begin(), written.end(), std::make_pair(a + (uintptr_t)bytes, uintptr_t(0)));
+    return p && it != written.begin() && (it - 1)->second > a;
+  };
+  std::vector<uintptr_t> counters;
+  counters.reserve((size_t)n);
+  for (int64_t i = 0; i < n; ++i) {
+    const char* what = t[i].numel && meets(t[i].grad, t[i].numel * elem_bytes(t[i].dtype)) ? "grad"
+                       : meets(t[i].step, 8)                                               ? "step"
+                                                                                           : nullptr;
+    if (what)
+      return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: %s must not overlap a parameter, master copy or state",
+                  (long long)i, what);
+    counters.push_back((uintptr_t)t[i].step);
+  }
+  std::sort(counters.begin(), counters.end());
+  counters.erase(std::unique(counters.begin(), counters.end()), counters.end());
+  for (size_t i = 1; i < counters.size(); ++i)
+    if (counters[i] - counters[i - 1] < 8)
+      return fail(DCN_ERR_INVALID_ARGUMENT, "step counters must be the same or not overlap");
+  for (uintptr_t c : counters) written.emplace_back(c, c + 8);
+  std::sort(written.begin(), written.end());
+  if (meets(o->grad_scale, 4) || meets(o->lr_device, 4))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "%s must not overlap a parameter, master copy, state or step counter",
+                meets(o->grad_scale, 4) ? "grad_scale" : "lr_device");
   return DCN_OK;
 }
 

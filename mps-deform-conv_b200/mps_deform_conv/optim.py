@@ -86,8 +86,9 @@ def adamw_step(
 
     Raises:
         ValueError: If a tensor is not on a CUDA device.
-        RuntimeError: If shapes, dtypes, layouts or hyperparameters do not fit, or two
-            of the written tensors overlap.
+        RuntimeError: If shapes, dtypes, layouts or hyperparameters do not fit, or a
+            written tensor overlaps another one of the call (counters may be shared,
+            gradients the same).
     """
     from mps_deform_conv import _get_lib
     _require_cuda(params, "params")

@@ -64,6 +64,28 @@ def test_adamw_refuses_the_same_parameter_twice():
     assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "twice" in msg
 
 
+@pytest.mark.parametrize("kw,options,needle", [
+    (dict(grad=0x100000), {}, "tensor 0: grad"),                      # the gradient is the parameter
+    (dict(grad=0x120000 + 255), {}, "tensor 0: grad"),                # and by one byte a state
+    (dict(grad=0x120000 - 255), {}, "tensor 0: grad"),
+    (dict(step=0x120000 + 8), {}, "tensor 0: step"),                  # the counter lies in a state
+    (dict(step=0x120000 - 4), {}, "tensor 0: step"),
+    (dict(), dict(grad_scale=0x100000 + 4), "grad_scale"),
+    (dict(), dict(lr_device=0x120000 + 252), "lr_device"),
+    (dict(), dict(grad_scale=0x150004), "grad_scale"),                # the counter's ticket
+])
+def test_adamw_refuses_inputs_in_written_memory(kw, options, needle):
+    rc, msg = _call(_options(**options), _tensors(**kw), 1)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and needle in msg and "overlap" in msg
+
+
+def test_adamw_refuses_counters_that_overlap():
+    t = _tensors(2)
+    t[1].step = t[0].step + 4
+    rc, msg = _call(_options(), t, 2)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "counters" in msg
+
+
 def test_adamw_empty_lists():
     assert _call(_options(), None, 0)[0] == _abi.DCN_OK
     assert _call(None, None, 0)[0] == _abi.DCN_ERR_INVALID_ARGUMENT
