@@ -99,11 +99,14 @@ static int check_adamw(const dcn_adamw_options* o, const dcn_adamw_tensor* t, in
   for (size_t i = 1; i < counters.size(); ++i)
     if (counters[i] - counters[i - 1] < 8)
       return fail(DCN_ERR_INVALID_ARGUMENT, "step counters must be the same or not overlap");
-  for (uintptr_t c : counters) written.emplace_back(c, c + 8);
-  std::sort(written.begin(), written.end());
-  if (meets(o->grad_scale, 4) || meets(o->lr_device, 4))
-    return fail(DCN_ERR_INVALID_ARGUMENT, "%s must not overlap a parameter, master copy, state or step counter",
-                meets(o->grad_scale, 4) ? "grad_scale" : "lr_device");
+  auto meets_any = [&](const float* p) {
+    const uintptr_t a = (uintptr_t)p;
+    auto it = std::lower_bound(counters.begin(), counters.end(), a + 4);
+    return p && (meets(p, 4) || (it != counters.begin() && *(it - 1) + 8 > a));
+  };
+  const char* scalar = meets_any(o->grad_scale) ? "grad_scale" : meets_any(o->lr_device) ? "lr_device" : nullptr;
+  if (scalar)
+    return fail(DCN_ERR_INVALID_ARGUMENT, "%s must not overlap a parameter, master copy, state or step counter", scalar);
   return DCN_OK;
 }
 

@@ -25,7 +25,7 @@ dcn_conv_desc make_desc(const at::Tensor& input, int64_t out_channels, int64_t k
                         int64_t groups, int64_t offset_groups, bool use_mask) {
   TORCH_CHECK(input.dim() == 4, "input must be 4-D (N, C, H, W), got ", input.dim(), "-D");
   dcn_conv_desc d;
-  d.dtype = dtype_code(input);
+  d.dtype = dtype_code(input, "deform_conv2d");
   d.use_mask = use_mask ? 1 : 0;
   d.batch = input.size(0);
   d.in_channels = input.size(1);

@@ -9,13 +9,13 @@
 
 #include "dcn_b200.h"
 
-inline int32_t dtype_code(const at::Tensor& t) {
+inline int32_t dtype_code(const at::Tensor& t, const char* op) {
   switch (t.scalar_type()) {
     case at::kFloat: return DCN_FLOAT32;
     case at::kHalf: return DCN_FLOAT16;
     case at::kBFloat16: return DCN_BFLOAT16;
     default:
-      TORCH_CHECK(false, "unsupported dtype ", t.scalar_type(),
+      TORCH_CHECK(false, op, ": unsupported dtype ", t.scalar_type(),
                   " (expected float32, float16 or bfloat16)");
   }
   return 0;

@@ -83,7 +83,7 @@ struct FfnArgs {
                       "), got ", wd.sizes());
     TORCH_CHECK_VALUE(c > 0 && f > 0, "channels and hidden must be positive, got ", c, " and ", f);
     TORCH_CHECK_VALUE(bg.has_value() == bu.has_value(), "b_gate and b_up go together");
-    d.dtype = dtype_code(input);
+    d.dtype = dtype_code(input, "gated_feed_forward");
     d.activation = (int32_t)activation;
     d.channels = c;
     d.hidden = f;
@@ -259,7 +259,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     }
     t.step = s.data_ptr<int32_t>();
     t.numel = p.numel();
-    t.dtype = dtype_code(p);
+    t.dtype = dtype_code(p, "adamw_step");
     t.reserved = 0;
   }
   check_status(dcn_adamw_step(&o, e.data(), (int64_t)n, stream_of(params[0])));
@@ -292,7 +292,7 @@ std::tuple<at::Tensor, at::Tensor> grad_norm(const Tensors& grads, double max_no
       dense.push_back(g.contiguous());
       g = dense.back();
     }
-    refs[i] = {g.data_ptr(), g.numel(), dtype_code(g), 0};
+    refs[i] = {g.data_ptr(), g.numel(), dtype_code(g, "grad_norm"), 0};
   }
   auto opt = grads[0].options().dtype(at::kFloat);
   auto out = at::empty({2}, opt);

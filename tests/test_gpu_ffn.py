@@ -541,6 +541,21 @@ def test_refusals_on_the_device(cuda):
         mdc.gated_feed_forward(args[0], args[1], args[2], args[3].t(), *args[4:])
 
 
+def test_dtype_refusals_name_their_operator(cuda):
+    """The helper is shared; each operator keeps its own prefix."""
+    x, w = torch.zeros(1, 4, 5, 5, device=cuda).double(), torch.zeros(4, 4, 3, 3, device=cuda).double()
+    offset = torch.zeros(1, 18, 5, 5, device=cuda).double()
+    with pytest.raises(RuntimeError, match="^deform_conv2d: unsupported dtype"):
+        mdc.deform_conv2d(x, offset, w, padding=1)
+    v, u = torch.zeros(3, 8, device=cuda).double(), torch.zeros(16, 8, device=cuda).double()
+    with pytest.raises(RuntimeError, match="^gated_feed_forward: unsupported dtype"):
+        mdc.gated_feed_forward(v, u, u, u.t().contiguous())
+    with pytest.raises(RuntimeError, match="^grad_norm: unsupported dtype"):
+        mdc.optim.grad_norm([v])
+    with pytest.raises(RuntimeError, match="^adamw_step: unsupported dtype"):
+        mdc.optim.adamw_step([v], [v.clone()], [v.float()], [v.float()], [mdc.optim.new_step(cuda)], lr=1e-3)
+
+
 def test_registered_operators(cuda):
     ops = torch.ops.mps_deform_conv
     for bias in (True, False):
