@@ -38,11 +38,16 @@
 // the epilogue, a buffer's products and its epilogue would exclude each other.
 //
 // What bounds it: products with a long K the tensor cores, at 1.3 to 1.45
-// PFLOP/s in bf16 until the power cap is reached.  The gated epilogues have some
-// 30 instructions a value pair and two special functions, 16 warps issue about
-// half of the cycles, and a tile of 128 x 128 pairs takes them some 5500 cycles:
-// as long as the products at K = 700, so below that they set the pace
-// (27200 x 256 -> 1024: 45 us with relu, 55 with gelu; the products alone 18).
+// PFLOP/s in bf16 until the power cap is reached.  The gated epilogues take some
+// 26 instructions and two special functions a value pair; the counters show 47 %
+// (gate and up) and 55 % (dhidden) of the issue slots busy and the tensor cores
+// 43 and 22 % (23104 x 512 -> 2048).  Clock stamps in a build for that put a
+// 128 x 128 pair tile's epilogue near 5500 cycles, what its products take at
+// K = 700 and the peak rate, so below that the epilogues set the pace: gate and
+// up of 27200 x 256 -> 1024 take 45 us with relu and 57 with gelu, 18 us of
+// operations at the measured matrix rate.  Arithmetic in packed pairs (f32x2)
+// takes the same time (backbone-sized case 81.2 us both ways; 92416 x 512 ->
+// 2048, forward and backward, 1742 against 1752).
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along
@@ -59,8 +64,9 @@
 // of the column operand (GATED: one gate, the other up) and the accumulator of
 // its rows; the first issues the MMAs for both.  A CTA alone reads 384 operand
 // rows for 128 x 256 results, a pair 512 for 256 x 256, a third less (92416 x 512
-// -> 2048 in bf16: dx 284 -> 266 us, weight gradients 446 -> 413).  Loads go to the CTA's own shared memory and report to the first CTA's
-// barrier; commits arrive at both.
+// -> 2048 in bf16: dx 284 -> 266 us, weight gradients 446 -> 413).  Loads go to
+// the CTA's own shared memory and report to the first CTA's barrier; commits
+// arrive at both.
 //
 // Every mbarrier wait is bounded (dcn_sm100.cuh).
 #pragma once
@@ -97,10 +103,10 @@ enum Epi { EPI_GATED, EPI_DGATE, EPI_RECOMPUTE, EPI_STORE };
 // two row operands (x, dy).
 constexpr int kRecomputeCols = 64, kRecomputeBn = 3 * kRecomputeCols;
 // Output staging of an epilogue warp: STORE (16-bit) its columns of a tile for
-// one TMA store, DGATE and RECOMPUTE two blocks whose columns are summed.
-constexpr uint32_t kSumBlock = 32 * CB * 2;
+// one TMA store, DGATE and RECOMPUTE an fp32 block whose columns are summed.
+constexpr uint32_t kSumBlock = 32 * CB * 4;
 __host__ __device__ constexpr uint32_t staging_bytes(int epi, int bn, bool wide) {
-  return wide || epi == EPI_GATED ? 0u : epi == EPI_STORE ? 32u * (uint32_t)(bn / 4) * 2u : 2u * kSumBlock;
+  return wide || epi == EPI_GATED ? 0u : epi == EPI_STORE ? 32u * (uint32_t)(bn / 4) * 2u : kSumBlock;
 }
 __host__ __device__ constexpr uint32_t stage_bytes(int bn, bool pair) {
   return (bn == kRecomputeBn ? 2 : 1) * A_STAGE + (uint32_t)bn * 128u / (pair ? 2u : 1u);
@@ -497,8 +503,8 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
 
 // A block's columns of one row, as an operand of a following product: two
 // panels' pieces (fp32 data: in each of three bf16 planes).  `at`: this row in
-// the first panel, 2048 bytes before the next; columns at and past `left` are not in the matrix, their
-// panel is skipped (values inside a last panel are zero).
+// the first panel, 2048 bytes before the next; a panel at or past column `left`
+// is not in the matrix and is skipped (a last panel's other columns are zero).
 template <typename T>
 __device__ __forceinline__ void store_panels(uint8_t* at, int64_t plane, int left, const float (&v)[CB]) {
   constexpr int kPanel = BM * 16;
@@ -625,38 +631,46 @@ struct SavedRaw {
 };
 
 // ---------------------------------------------------------------- column sums of a block
-// 16-bit: of the rounded values, staged by their lanes as [32 rows][dgate 16,
-// dup 16] (64-byte rows, their 8-byte pieces rotated by the row): lane l adds
-// four columns, piece l % 8, of rows l / 8, l / 8 + 4, ..., then the four row
-// groups meet in two shuffles.  Lanes 0-7 hold the sums of columns 4 l .. 4 l + 3
-// of the 32.  (By mma.sync with a row operand of ones: 150 us more in the
-// 92416 x 2048 pass; the legacy instruction takes the tensor cores' time.)
-template <typename T>
-__device__ __forceinline__ void stage_sums(uint8_t* rows, int lane, int at, const float (&v)[CB]) {
+// 16-bit data: a block of fp32 values, before their rounding (rounded ones
+// would put as much error into a sum of mixed signs as the result's own
+// rounding does), staged as [32 rows][16] with the 16-byte pieces of row r at
+// j ^ (r / 2 % 4), so eight lanes cover all banks; lane l then adds piece l % 4
+// of rows l / 4, l / 4 + 8, ...  (By mma.sync with a row operand of ones: 150
+// us more in the 92416 x 2048 pass; the legacy instruction takes the tensor
+// cores' time.)
+__device__ __forceinline__ void staged_column_sums(uint8_t* rows, int lane, const float (&v)[CB], float (&sum)[4]) {
+  __syncwarp();
 #pragma unroll
-  for (int j = 0; j < CB / 4; ++j) {
-    uint2 p;
-    p.x = pack2(v[4 * j], v[4 * j + 1], (T*)nullptr);
-    p.y = pack2(v[4 * j + 2], v[4 * j + 3], (T*)nullptr);
-    *reinterpret_cast<uint2*>(rows + lane * 64 + (((at + j + lane) & 7) << 3)) = p;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void staged_column_sums(const uint8_t* rows, int lane, float (&sum)[4]) {
-  const int piece = lane & 7;
+  for (int j = 0; j < CB / 4; ++j)
+    *reinterpret_cast<float4*>(rows + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
 #pragma unroll
   for (int j = 0; j < 4; ++j) sum[j] = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = (lane >> 3) + 4 * i;
-    const uint2 p = *reinterpret_cast<const uint2*>(rows + r * 64 + (((piece + r) & 7) << 3));
-    const float2 x = tcc::Vec<T>::unpack(p.x), y = tcc::Vec<T>::unpack(p.y);
-    sum[0] += x.x; sum[1] += x.y; sum[2] += y.x; sum[3] += y.y;
+  for (int i = 0; i < 4; ++i) {
+    const int r = (lane >> 2) + 8 * i;
+    const float4 f = *reinterpret_cast<const float4*>(rows + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+    sum[0] += f.x; sum[1] += f.y; sum[2] += f.z; sum[3] += f.w;
+  }
+}
+// The eight row groups (lane / 4) of two such blocks meet, each step halving
+// what a lane holds: lane l returns block l / 16's column 4 (l % 4) + 2 (l / 8 %
+// 2) + l / 4 % 2.
+__device__ __forceinline__ float meet_row_groups(int lane, const float (&a)[4], const float (&b)[4]) {
+  float s[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float other = __shfl_xor_sync(0xffffffffu, lane & 16 ? a[j] : b[j], 16);
+    s[j] = (lane & 16 ? b[j] : a[j]) + other;
   }
 #pragma unroll
-  for (int o = 8; o <= 16; o <<= 1)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+  for (int j = 0; j < 2; ++j) {
+    const float other = __shfl_xor_sync(0xffffffffu, lane & 8 ? s[j] : s[j + 2], 8);
+    s[j] = (lane & 8 ? s[j + 2] : s[j]) + other;
+  }
+  const float other = __shfl_xor_sync(0xffffffffu, lane & 4 ? s[0] : s[1], 4);
+  return (lane & 4 ? s[1] : s[0]) + other;
 }
 // fp32: lanes 0-15 return the sums of columns 0-15 over the warp's lanes, in an
 // order fixed by the lanes.
@@ -847,123 +861,123 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   Work w(a, blockIdx.x / CTAS, gridDim.x / CTAS);
 
   if (warp >= EPI_WARPS) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == LOAD_WARP) {
-    // ------------------------------------------------ TMA loads
-    if (lane == 0) {
-      int issued = 0;
-      bool ok = true;
-      while (ok && w.next(a)) {
-        int z, mt, nt;
-        tile_at(a, w.tile, z, mt, nt);
-        const int m0 = (mt * CTAS + rank) * BM, n0 = nt * cols;
-        const int nb = PAIR && !GATED ? n0 + rank * (BN / 2) : n0;  // this CTA's part of the column operand
-        int sg = w.kb0 / a.nk, kb = w.kb0 - sg * a.nk;
-        for (int i = w.kb0; i < w.kb1; ++i) {
-          const int s = issued % S;
-          ok = mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag, a.status, ST_FFN_LOAD);
-          if (!ok) break;
-          const Seg seg = a.seg[sg];
-          const int k = kb * BK;
-          const uint32_t dst = sbase + s * STAGE;
-          const uint32_t bar = PAIR ? in_first_cta(full(s)) : full(s);
-          const CUtensorMap* ma = &maps.m[seg.a_map + z];
-          const CUtensorMap* mb = &maps.m[seg.b_map];
-          if (rank == 0) mbar_arrive_expect_tx(full(s), tx);
-          if (A == PANELS_MN) {
-            load_panels<PAIR>(dst, ma, k, m0 >> 3, seg.a_plane, bar);
-          } else if (A == PANELS_K) {
-            load_panels<PAIR>(dst, ma, m0, k >> 3, seg.a_plane, bar);
-          } else if (A == ROWS_MN) {
-            load_g<PAIR>(dst, ma, m0, k, seg.a_plane, bar);
-            load_g<PAIR>(dst + 8192, ma, m0 + 64, k, seg.a_plane, bar);
-          } else {
-            load_g<PAIR>(dst, ma, k, m0, seg.a_plane, bar);
-          }
-          if (GATED && PAIR) {
-            load_g<PAIR>(dst + B_AT, mb + rank, k, n0, seg.b_plane, bar);
-          } else if (TWO) {
-            tma_load_3d(dst + B_AT, mb, k, n0, seg.b_plane, bar);
-            tma_load_3d(dst + B_AT + cols * 128, mb + 1, k, n0, seg.b_plane, bar);
-            if (RECOMP) {  // dy beside x, w_down (MN-major) beside the other two
-              tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, bar);
-              tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, bar);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == LOAD_WARP) {
+      // ------------------------------------------------ TMA loads
+      if (lane == 0) {
+        int issued = 0;
+        bool ok = true;
+        while (ok && w.next(a)) {
+          int z, mt, nt;
+          tile_at(a, w.tile, z, mt, nt);
+          const int m0 = (mt * CTAS + rank) * BM, n0 = nt * cols;
+          const int nb = PAIR && !GATED ? n0 + rank * (BN / 2) : n0;  // this CTA's part of the column operand
+          int sg = w.kb0 / a.nk, kb = w.kb0 - sg * a.nk;
+          for (int i = w.kb0; i < w.kb1; ++i) {
+            const int s = issued % S;
+            ok = mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag, a.status, ST_FFN_LOAD);
+            if (!ok) break;
+            const Seg seg = a.seg[sg];
+            const int k = kb * BK;
+            const uint32_t dst = sbase + s * STAGE;
+            const uint32_t bar = PAIR ? in_first_cta(full(s)) : full(s);
+            const CUtensorMap* ma = &maps.m[seg.a_map + z];
+            const CUtensorMap* mb = &maps.m[seg.b_map];
+            if (rank == 0) mbar_arrive_expect_tx(full(s), tx);
+            if (A == PANELS_MN) {
+              load_panels<PAIR>(dst, ma, k, m0 >> 3, seg.a_plane, bar);
+            } else if (A == PANELS_K) {
+              load_panels<PAIR>(dst, ma, m0, k >> 3, seg.a_plane, bar);
+            } else if (A == ROWS_MN) {
+              load_g<PAIR>(dst, ma, m0, k, seg.a_plane, bar);
+              load_g<PAIR>(dst + 8192, ma, m0 + 64, k, seg.a_plane, bar);
+            } else {
+              load_g<PAIR>(dst, ma, k, m0, seg.a_plane, bar);
             }
-          } else if (B == PANELS_MN) {
-            load_panels<PAIR>(dst + A_STAGE, mb, k, nb >> 3, seg.b_plane, bar);
-          } else if (B == ROWS_MN) {
+            if (GATED && PAIR) {
+              load_g<PAIR>(dst + B_AT, mb + rank, k, n0, seg.b_plane, bar);
+            } else if (TWO) {
+              tma_load_3d(dst + B_AT, mb, k, n0, seg.b_plane, bar);
+              tma_load_3d(dst + B_AT + cols * 128, mb + 1, k, n0, seg.b_plane, bar);
+              if (RECOMP) {  // dy beside x, w_down (MN-major) beside the other two
+                tma_load_3d(dst + A_STAGE, ma + 1, k, m0, seg.a_plane, bar);
+                tma_load_3d(dst + B_AT + 2 * COLS * 128, mb + 2, n0, k, seg.b_plane, bar);
+              }
+            } else if (B == PANELS_MN) {
+              load_panels<PAIR>(dst + A_STAGE, mb, k, nb >> 3, seg.b_plane, bar);
+            } else if (B == ROWS_MN) {
 #pragma unroll
-            for (int q = 0; q < BN / 64 / CTAS; ++q)
-              load_g<PAIR>(dst + A_STAGE + q * 8192, mb, nb + 64 * q, k, seg.b_plane, bar);
-          } else {
-            load_g<PAIR>(dst + A_STAGE, mb, k, nb, seg.b_plane, bar);
-          }
-          ++issued;
-          if (++kb == a.nk) {
-            kb = 0;
-            ++sg;
+              for (int q = 0; q < BN / 64 / CTAS; ++q)
+                load_g<PAIR>(dst + A_STAGE + q * 8192, mb, nb + 64 * q, k, seg.b_plane, bar);
+            } else {
+              load_g<PAIR>(dst + A_STAGE, mb, k, nb, seg.b_plane, bar);
+            }
+            ++issued;
+            if (++kb == a.nk) {
+              kb = 0;
+              ++sg;
+            }
           }
         }
+        // copies in flight land before the CTA may go (a pair's report to the first CTA)
+        if (rank == 0)
+          for (int i = issued > S ? issued - S : 0; i < issued; ++i)
+            mbar_wait(full(i % S), (i / S) & 1, abort_flag, a.status, ST_FFN_DRAIN);
       }
-      // copies in flight land before the CTA may go (a pair's report to the first CTA)
-      if (rank == 0)
-        for (int i = issued > S ? issued - S : 0; i < issued; ++i)
-          mbar_wait(full(i % S), (i / S) & 1, abort_flag, a.status, ST_FFN_DRAIN);
-    }
-  } else if (warp == MMA_WARP) {
-    // ------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * cols : FREE ? cols : BN, a.operand_bf16 != 0, A_MN, B_MN);
-      const uint32_t idesc_dh = tcc::idesc_f16_major(BM, COLS, a.operand_bf16 != 0, false, true);
-      int used = 0, done = 0;
-      bool ok = true;
-      while (ok && w.next(a)) {
-        for (int k0 = w.kb0; ok && k0 < w.kb1; k0 += RUN) {
-          const int k1 = w.kb1 - k0 > RUN ? k0 + RUN : w.kb1;
-          const int b = done & 1;
-          ok = mbar_wait(acc_empty(b), ((done >> 1) & 1) ^ 1, abort_flag, a.status, ST_FFN_MMA);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(b * ACC);
-          for (int i = k0; i < k1; ++i) {
-            const int s = used % S;
-            ok = mbar_wait(full(s), (used / S) & 1, abort_flag, a.status, ST_FFN_MMA);
+    } else if (warp == MMA_WARP) {
+      // ------------------------------------------------ MMA issuer
+      if (lane == 0 && rank == 0) {
+        const uint32_t idesc = tcc::idesc_f16_major(BM * CTAS, TWO ? 2 * cols : FREE ? cols : BN, a.operand_bf16 != 0, A_MN, B_MN);
+        const uint32_t idesc_dh = tcc::idesc_f16_major(BM, COLS, a.operand_bf16 != 0, false, true);
+        int used = 0, done = 0;
+        bool ok = true;
+        while (ok && w.next(a)) {
+          for (int k0 = w.kb0; ok && k0 < w.kb1; k0 += RUN) {
+            const int k1 = w.kb1 - k0 > RUN ? k0 + RUN : w.kb1;
+            const int b = done & 1;
+            ok = mbar_wait(acc_empty(b), ((done >> 1) & 1) ^ 1, abort_flag, a.status, ST_FFN_MMA);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t ab = sbase + s * STAGE, bb = ab + B_AT;
+            const uint32_t d = tmem + (uint32_t)(b * ACC);
+            for (int i = k0; i < k1; ++i) {
+              const int s = used % S;
+              ok = mbar_wait(full(s), (used / S) & 1, abort_flag, a.status, ST_FFN_MMA);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t ab = sbase + s * STAGE, bb = ab + B_AT;
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-              // panels in shared memory: K-major [panel][128 rows][16 B] (panels along K by
-              // LBO, 8-row groups by SBO); MN-major [panel][64 rows][16 B] (8-row groups along
-              // K by LBO, panels by SBO)
-              const uint64_t ad = A == PANELS_K    ? (FREE ? desc_panels(ab + kk * 2 * a.a_lbo, a.a_lbo, 128) : desc_panels(ab + kk * 4096, 2048, 128))
-                                  : A == PANELS_MN ? desc_panels(ab + kk * 256, 128, 1024)
-                                  : A == ROWS_MN   ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192)
-                                                   : desc_kmajor_sw128(ab + kk * 32);
-              const uint64_t bd = B == PANELS_MN ? desc_panels(bb + kk * 256, 128, 1024)
-                                  : B == ROWS_MN ? tcc::desc_mnmajor_sw128(bb + kk * 2048, 8192)
-                                                 : desc_kmajor_sw128(bb + kk * 32);
-              mma_g<PAIR>(d, ad, bd, idesc, (i > k0 || kk > 0) ? 1u : 0u);
-              if (RECOMP)
-                mma_f16(d + 2 * COLS, desc_kmajor_sw128(ab + A_STAGE + kk * 32),
-                        tcc::desc_mnmajor_sw128(bb + 2 * COLS * 128 + kk * 2048, 8192), idesc_dh,
-                        (i > k0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < BK / 16; ++kk) {
+                // panels in shared memory: K-major [panel][128 rows][16 B] (panels along K by
+                // LBO, 8-row groups by SBO); MN-major [panel][64 rows][16 B] (8-row groups along
+                // K by LBO, panels by SBO)
+                const uint64_t ad = A == PANELS_K    ? (FREE ? desc_panels(ab + kk * 2 * a.a_lbo, a.a_lbo, 128) : desc_panels(ab + kk * 4096, 2048, 128))
+                                    : A == PANELS_MN ? desc_panels(ab + kk * 256, 128, 1024)
+                                    : A == ROWS_MN   ? tcc::desc_mnmajor_sw128(ab + kk * 2048, 8192)
+                                                     : desc_kmajor_sw128(ab + kk * 32);
+                const uint64_t bd = B == PANELS_MN ? desc_panels(bb + kk * 256, 128, 1024)
+                                    : B == ROWS_MN ? tcc::desc_mnmajor_sw128(bb + kk * 2048, 8192)
+                                                   : desc_kmajor_sw128(bb + kk * 32);
+                mma_g<PAIR>(d, ad, bd, idesc, (i > k0 || kk > 0) ? 1u : 0u);
+                if (RECOMP)
+                  mma_f16(d + 2 * COLS, desc_kmajor_sw128(ab + A_STAGE + kk * 32),
+                          tcc::desc_mnmajor_sw128(bb + 2 * COLS * 128 + kk * 2048, 8192), idesc_dh,
+                          (i > k0 || kk > 0) ? 1u : 0u);
+              }
+              commit_g<PAIR>(empty(s), true);
+              ++used;
             }
-            commit_g<PAIR>(empty(s), true);
-            ++used;
+            if (!ok) break;
+            commit_g<PAIR>(acc_full(b), true);
+            ++done;
           }
-          if (!ok) break;
-          commit_g<PAIR>(acc_full(b), true);
-          ++done;
+        }
+        // MMAs still running finish before TMEM and shared memory are released
+        if (used > 0) {
+          commit_g<PAIR>(drain, false);
+          mbar_wait(drain, 0, abort_flag, a.status, ST_FFN_DRAIN);
         }
       }
-      // MMAs still running finish before TMEM and shared memory are released
-      if (used > 0) {
-        commit_g<PAIR>(drain, false);
-        mbar_wait(drain, 0, abort_flag, a.status, ST_FFN_DRAIN);
-      }
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     // ------------------------------------------------ epilogue
@@ -1077,19 +1091,12 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
                 sums[a.N + c0 + lane] = su;
               }
             } else {
-              __syncwarp();
-              stage_sums<T>(stage, lane, 0, v);
-              stage_sums<T>(stage, lane, 4, u);
-              __syncwarp();
-              float sum[4];
-              staged_column_sums<T>(stage, lane, sum);
-              if (lane < 8) {  // dgate's columns, then dup's
-                const int c = c0 + 4 * (lane & 3);
-                float* out = sums + (lane >= 4 ? a.N : 0) + c;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (c + j < a.N) out[j] = sum[j];
-              }
+              float sg[4], su[4];
+              staged_column_sums(stage, lane, v, sg);
+              staged_column_sums(stage, lane, u, su);
+              const float sum = meet_row_groups(lane, sg, su);
+              const int c = c0 + 4 * (lane & 3) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1);
+              if (c < a.N) sums[(lane >> 4) * a.N + c] = sum;
             }
           }
         } else {

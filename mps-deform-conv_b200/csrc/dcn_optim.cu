@@ -486,7 +486,6 @@ cudaError_t adamw_step(const dcn_adamw_options& o, const dcn_adamw_tensor* t, in
   h.seed = o.seed;
   // one launch group per (dtype, master copies or not): entries in call order
   std::vector<AdamwEntry> group[3][2];
-  std::vector<std::pair<int32_t*, std::pair<AdamwEntry*, int>>> unused;
   for (int64_t i = 0; i < n; ++i) {
     AdamwEntry e;
     e.param = t[i].param; e.grad = t[i].grad; e.exp_avg = t[i].exp_avg; e.exp_avg_sq = t[i].exp_avg_sq;
@@ -538,9 +537,10 @@ cudaError_t adamw_step(const dcn_adamw_options& o, const dcn_adamw_tensor* t, in
 // norm = sqrt(sum of all squares) / loss_scale.  Each CTA sums its share of the
 // chunks in a fixed order and writes one fp64 partial; a second one-CTA kernel
 // adds the partials in order, so the result does not depend on timing.  HBM
-// bound: the gradients are read once (96.6 M bf16 values: 39 us, 5.0 TB/s).  Sums are fp64 per 8 elements: the fp32
-// sum of 8 squares is converted, and recomputed in fp64 when it left fp32's
-// range (overflow past 3e38 or below 1e-30), which only extreme gradients do.
+// bound: the gradients are read once (96.6 M bf16 values: 39 us, 5.0 TB/s).
+// Sums are fp64 per 8 elements: the fp32 sum of 8 squares is converted, and
+// recomputed in fp64 when it left fp32's range (overflow past 3e38 or below
+// 1e-30), which only extreme gradients do.
 namespace {
 
 struct NormEntry {

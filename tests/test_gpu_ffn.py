@@ -6,8 +6,8 @@ Bounds are elementwise and count roundings:
     products' absolute values.  fp32 data runs six such passes, and drops terms below
     3 * 2^-24 of a product;
   * the hidden values and their gradients are rounded to the type (half of its eps) as
-    operands and as summands of the bias gradients; saved gate and up values of 16-bit data
-    (more than 256 channels) to 11 bits;
+    operands (the bounds count it for the bias gradients' summands too); saved gate and up
+    values of 16-bit data (more than 256 channels) to 11 bits;
   * errors of gate and up enter the activation by its largest slope, those of its derivative
     by the largest curvature (relu: a sign may change where gate is within its own error);
   * 16-bit data: the fast exponential and quotient leave 2^-19 of an activation's value, the
@@ -169,6 +169,24 @@ def test_few_rows(m, dtype, cuda):
     for c, f in ((256, 1000), (520, 88), (64, 4096), (1000, 72), (2048, 512), (33, 31)):
         args, _ = _inputs(m, c, f, dt, cuda, f % 16 == 8, seed=m + c)
         _check(_run(args, None, "silu"), _reference(args, None, "silu", dt), f"{(m, c, f)}")
+
+
+@pytest.mark.parametrize("channels,dtype", [(512, "bf16"), (64, "bf16"), (64, "fp16")])
+def test_bias_gradients_sum_unrounded_values(channels, dtype, cuda):
+    """Sums of mixed signs over many rows.  Their error is the result's own rounding, 1 in its units, beside
+    values that keep at least three bits more than the type (saved gate and up: 2 x (1/8)^2 in squares); the
+    norm over 1536 columns scatters by 1 / sqrt(2 x 1536) = 2 %, six of which are allowed for.  Summands
+    rounded to the type would add as much as the result's rounding: 1.41."""
+    dt = {"bf16": torch.bfloat16, "fp16": torch.float16}[dtype]
+    args, dy = _inputs(20000, channels, 1536, dt, cuda, True, seed=21)
+    got = _run(args, dy, "silu")
+    ref = _reference(args, dy, "silu", dt)
+    for name in ("db_gate", "db_up"):
+        k = NAMES.index(name)
+        exact = ref[k][0]
+        own = float((got[k].double() - exact).norm())
+        rounded = float((exact.to(dt).double() - exact).norm())
+        assert own <= rounded * (1 + 2 / 64) ** 0.5 * 1.12, (name, own / rounded)
 
 
 def test_strides_views_and_alignment(cuda):
