@@ -38,16 +38,15 @@
 // the epilogue, a buffer's products and its epilogue would exclude each other.
 //
 // What bounds it: products with a long K the tensor cores, at 1.3 to 1.45
-// PFLOP/s in bf16 until the power cap is reached.  The gated epilogues take some
-// 26 instructions and two special functions a value pair; the counters show 47 %
-// (gate and up) and 55 % (dhidden) of the issue slots busy and the tensor cores
-// 43 and 22 % (23104 x 512 -> 2048).  Clock stamps in a build for that put a
-// 128 x 128 pair tile's epilogue near 5500 cycles, what its products take at
-// K = 700 and the peak rate, so below that the epilogues set the pace: gate and
-// up of 27200 x 256 -> 1024 take 45 us with relu and 57 with gelu, 18 us of
-// operations at the measured matrix rate.  Arithmetic in packed pairs (f32x2)
-// takes the same time (backbone-sized case 81.2 us both ways; 92416 x 512 ->
-// 2048, forward and backward, 1742 against 1752).
+// PFLOP/s in bf16 until the power cap is reached.  Gated passes the epilogue: 35
+// instructions a value pair, issued by four warps a scheduler that wait for
+// TMEM and for one another's results in between.  23104 x 512 -> 2048 in bf16:
+// a pair of tiles every 8700 cycles, in 4100 of which the tensor cores work;
+// issue slots 50 % (gate and up) and 56 % (dhidden) busy, tensor cores 46 and
+// 23 %.  27200 x 256 -> 1024: 45 us with relu, 57 with gelu, 18 us of operations
+// at the measured matrix rate.  Arithmetic in packed pairs (f32x2) takes the
+// same time (that case, both products: 81.2 us both ways; 92416 x 512 -> 2048,
+// forward and backward, 1742 us against 1752).
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along

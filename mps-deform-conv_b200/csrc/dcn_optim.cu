@@ -27,7 +27,7 @@
 // per lane, as 16-byte loads where every pointer of the tensor allows them and
 // as single elements, 32 lanes side by side, where not and at tails.
 // Measured on 96.6 M bf16 parameters: fp32 states with master copies 415 us, the
-// measured copy rate; 8-bit states without 295 us, 3.3 TB/s: some 80
+// measured copy rate; 8-bit states without 293 us, 3.3 TB/s: some 80
 // instructions an element (exact root, two codes, hash) hold it there.
 #include <stdint.h>
 
