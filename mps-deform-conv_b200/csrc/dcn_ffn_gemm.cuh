@@ -50,11 +50,11 @@
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along
-// K instead (struct Cut): S = W / R workers a tile walk S equal slices of K,
-// tile by tile side by side, so that at any time all tiles read the same rows
-// of both operands and these come from the L2 (dealt tile after tile, a
-// product with a long K reads them from memory once per tile); the W - S R
-// workers left over share the end of K in equal runs.  Each piece is an fp32
+// K instead (struct Cut): up to W / R workers a tile walk slices of K of one
+// length, tile by tile side by side, so that at any time all tiles read the same
+// rows of both operands and these come from the L2 (dealt tile after tile, a
+// product with a long K reads them from memory once per tile); workers left
+// over share the end of K in runs no longer than a slice.  Each piece is an fp32
 // partial in a slot of its own, and a second kernel adds a tile's slots in a
 // fixed order: the result does not depend on timing.
 //
@@ -162,7 +162,8 @@ struct GemmArgs {
   int tiles_m, tiles_n, batches;  // a batch adds its index to a_map (and picks the output)
   // tiles are dealt in blocks of kGroupM row tiles x all column tiles; divisors of tile_at
   FastDiv per_batch, per_block, last_rows;
-  int split;                 // 1: the last tiles are cut along K (Cut), partials to `partial`
+  int split;                 // 1: the last cut.R tiles are cut along K, partials to `partial`
+  Cut cut;
   int act;
   // GATED, and STORE of ROWS_K columns, without pairs: output columns of a tile (a
   // multiple of 16, at most the kernel's), bytes of the row operand in a stage and
@@ -690,46 +691,28 @@ __device__ __forceinline__ float column_sum(float (&v)[CB], int lane) {
 }
 
 // ---------------------------------------------------------------- work
-// How the last R tiles of a product are cut along their nkb K blocks among W
-// workers.  Worker s R + t, s < S: slice s of tile t, K blocks [s a, s a + a).
-// The E = W - S R others: equal runs of the units (tile, K block >= S a), tile
-// after tile.  Slots: the worker's index in the first case; S R + e + t in the
-// second (unique, since along the runs either e or t grows by one).
-struct Cut {
-  int R, S, E, a, nkb;
-  __host__ __device__ Cut(int R_, int W, int nkb_) : R(R_), nkb(nkb_) {
-    S = W / R;
-    E = W - S * R;
-    a = E ? (int)((int64_t)nkb * R / W) : (nkb + S - 1) / S;
-  }
-  __host__ __device__ int rest() const { return E ? nkb - S * a : 0; }  // K blocks of the runs
-  __host__ __device__ int slots() const { return S * R + (E ? E + R : 0); }
-};
-
+// The pieces of a worker: whole tiles worker, worker + workers, ..., then its
+// share of the cut ones (struct Cut).
 struct Work {
   int worker, workers, nkb;
   int at, whole_end;            // whole tiles: at, at + workers, ... below whole_end
-  int base;                     // first of the cut tiles; -1: none
   int64_t unit, unit_end;       // units still to do of a run
   bool slice;                   // the slice is still to do
   int tile, kb0, kb1, slot;     // the current piece; slot < 0: a whole tile
-  __device__ __forceinline__ Work(const GemmArgs& a, int worker_, int workers_)
-      : worker(worker_), workers(workers_), nkb(a.nk * a.nseg), at(worker_), base(-1), unit(0), unit_end(0), slice(false) {
-    const int tiles = a.tiles_m * a.tiles_n * a.batches;
-    whole_end = tiles;
+  DCN_HOST_DEVICE Work(const GemmArgs& a, int worker_, int workers_)
+      : worker(worker_), workers(workers_), nkb(a.nk * a.nseg), at(worker_), unit(0), unit_end(0), slice(false) {
+    whole_end = a.tiles_m * a.tiles_n * a.batches;
     if (a.split) {
-      base = whole_end = tiles / workers * workers;
-      const Cut c(tiles - base, workers, nkb);
-      slice = worker < c.S * c.R;
-      if (!slice) {
-        const int e = worker - c.S * c.R;
-        const int64_t units = (int64_t)c.R * c.rest();
-        unit = units * e / c.E;
-        unit_end = units * (e + 1) / c.E;
+      whole_end -= a.cut.R;
+      const int e = worker - a.cut.S * a.cut.R;
+      slice = e < 0;
+      if (!slice && e < a.cut.E) {
+        unit = a.cut.units() * e / a.cut.E;
+        unit_end = a.cut.units() * (e + 1) / a.cut.E;
       }
     }
   }
-  __device__ __forceinline__ bool next(const GemmArgs& a) {
+  DCN_HOST_DEVICE bool next(const GemmArgs& a) {
     if (at < whole_end) {
       tile = at;
       at += workers;
@@ -738,26 +721,24 @@ struct Work {
       slot = -1;
       return true;
     }
-    if (base < 0) return false;
-    const Cut c(a.tiles_m * a.tiles_n * a.batches - base, workers, nkb);
+    const Cut& c = a.cut;
     if (slice) {
       slice = false;
       const int s = worker / c.R;
-      tile = base + worker - s * c.R;
+      tile = whole_end + worker - s * c.R;
       kb0 = s * c.a;
       kb1 = min(nkb, kb0 + c.a);
       slot = worker;
-      return kb0 < kb1;
+      return true;
     }
     if (unit >= unit_end) return false;
-    const int rest = c.rest();
-    const int t = (int)(unit / rest);
-    const int k = (int)(unit - (int64_t)t * rest);
-    const int len = (int)min((int64_t)(rest - k), unit_end - unit);
-    tile = base + t;
+    const int t = (int)(unit / c.rest);
+    const int k = (int)(unit - (int64_t)t * c.rest);
+    const int len = (int)min((int64_t)(c.rest - k), unit_end - unit);
+    tile = whole_end + t;
     kb0 = c.S * c.a + k;
     kb1 = kb0 + len;
-    slot = c.S * c.R + (worker - c.S * c.R) + t;
+    slot = worker + t;
     unit += len;
     return true;
   }

@@ -121,8 +121,8 @@ struct ReduceArgs {
   void* out[2];
   const void* bias;
   int64_t ldo;
-  int M, N, nkb, workers, base, tiles, ctas, vec;
-  GemmArgs g;  // for tile_at
+  int M, N, base, ctas, vec;  // base: the first cut tile
+  GemmArgs g;  // for tile_at, and the cut
 };
 
 template <typename T, int BN>
@@ -137,20 +137,14 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__
   const int64_t row = (int64_t)mt * BM * a.ctas + q * 32 + lane;
   const int c0 = nt * BN + c * 32;
   if (row - lane >= a.M || c0 >= a.N) return;
-  const Cut cut(a.tiles, a.workers, a.nkb);
-  int e0 = 0, e1 = -1;  // the runs that touch this tile
-  if (cut.rest() > 0) {
-    const int64_t rest = cut.rest(), units = rest * cut.R;
-    e0 = (int)(((t * rest + 1) * cut.E - 1) / units);
-    e1 = (int)(((t + 1) * rest * cut.E - 1) / units);
-  }
+  const Cut& cut = a.g.cut;
+  int run;
+  const int n = cut.pieces(t, run);
   float4 v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int slices = min(cut.S, (a.nkb + cut.a - 1) / cut.a);
-  const int n = slices + (e1 - e0 + 1);
   for (int i = warp; i < n; i += 8) {
-    const int slot = i < slices ? i * cut.R + t : cut.S * cut.R + e0 + (i - slices) + t;
+    const int slot = cut.slot(t, i, run);
     const float4* p = reinterpret_cast<const float4*>(a.partial + (int64_t)slot * a.ctas * (BM * BN) + q * (32 * BN) + c * 1024) + lane;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -338,6 +332,7 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
       return cudaErrorInvalidValue;
   set_tiles(a, p.tiles_m, p.tiles_n, batches);
   a.split = p.split;
+  a.cut = p.cut;
   a.operand_bf16 = operand_bf16<T>();
   a.partial = partial;
   a.out[0] = out[0];
@@ -359,13 +354,11 @@ cudaError_t store_product(const char* name, const std::vector<Operand>& a_ops, c
   r.bias = bias;
   r.ldo = ldo;
   r.M = a.M; r.N = a.N; r.g = a;
-  r.nkb = a.nk * a.nseg; r.workers = p.workers; r.vec = a.vec;
-  const int tiles = p.tiles_m * p.tiles_n * batches;
-  r.base = tiles / p.workers * p.workers;
-  r.tiles = tiles - r.base;
+  r.vec = a.vec;
+  r.base = p.tiles_m * p.tiles_n * batches - p.cut.R;
   KernelScope ks("ffn_reduce", st);
   r.ctas = p.pair ? 2 : 1;
-  const unsigned grid = (unsigned)(r.tiles * (p.bn / 32 * 4 * r.ctas));
+  const unsigned grid = (unsigned)(p.cut.R * (p.bn / 32 * 4 * r.ctas));
   if (p.bn == 256) ffn_reduce_kernel<T, 256><<<grid, 256, 0, st>>>(r);
   else if (p.bn == 128) ffn_reduce_kernel<T, 128><<<grid, 256, 0, st>>>(r);
   else ffn_reduce_kernel<T, 64><<<grid, 256, 0, st>>>(r);

@@ -6,6 +6,8 @@
 
 #include "dcn_ffn.h"
 
+#define DCN_HOST_DEVICE __host__ __device__ __forceinline__
+
 namespace dcn {
 namespace ffn {
 
@@ -38,12 +40,45 @@ struct Operand {
 };
 
 // ---------------------------------------------------------------- plans
+// How the last R tiles of a product are cut along their nkb K blocks among W >
+// R workers.  a is the even share R nkb / W rounded up, so it is at least 1.
+// Worker s R + t, s < S: slice s of tile t, K blocks [s a, s a + a).  The K blocks
+// `rest` past S a of each tile go to E workers more, in runs of the units (tile, K
+// block >= S a), tile after tile, whose lengths differ by at most one.  No run is
+// longer than a slice: R rest <= R nkb - R S a <= (W - R S) a, and where W - R S
+// is more than R rest, E is R rest.  So the longest piece is the even share to a
+// K block, no piece is empty, and the workers left over are those of the rounding.
+// Slots: the worker's index for a slice, S R + e + t for a run (unique, since
+// along the runs either e or t grows by one).
+struct Cut {
+  int R = 0, S = 0, E = 0, a = 0, rest = 0;
+  Cut() = default;
+  Cut(int R_, int W, int nkb) : R(R_) {
+    a = (int)(((int64_t)nkb * R + W - 1) / W);
+    S = std::min(W / R, (nkb + a - 1) / a);
+    rest = std::max(0, nkb - S * a);
+    E = (int)std::min<int64_t>(W - S * R, (int64_t)R * rest);
+  }
+  DCN_HOST_DEVICE int64_t units() const { return (int64_t)R * rest; }
+  // Pieces of tile t: its S slices, then the runs that touch it, from `run` on.
+  DCN_HOST_DEVICE int pieces(int t, int& run) const {
+    run = 0;
+    if (rest == 0) return S;
+    run = (int)((((int64_t)t * rest + 1) * E - 1) / units());
+    return S + (int)(((int64_t)(t + 1) * rest * E - 1) / units()) - run + 1;
+  }
+  DCN_HOST_DEVICE int slot(int t, int piece, int run) const {
+    return piece < S ? piece * R + t : S * R + run + (piece - S) + t;
+  }
+};
+
 struct GemmPlan {
   int bn = 256;
   bool pair = false, split = false;
   int workers = 0;  // CTAs, or pairs of them
   int tiles_m = 0, tiles_n = 0;
   int cols = 0;     // output columns of a tile
+  Cut cut;          // split: of the tiles past whole rounds of the workers
   size_t partial_bytes() const {
     return split ? ((size_t)workers + (size_t)tiles_m * tiles_n * 2) * BM * (pair ? 2 : 1) * bn * 4 : 0;
   }
@@ -78,7 +113,7 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
     const double tile = f.bn / f.rate * (double)nkb;
     double cost = (double)div_up(tiles, all) * tile;
     bool split = false;
-    if (splittable && tiles < 4 * all && tiles * nkb >= 8 * all) {
+    if (splittable && tiles % all && tiles < 4 * all && tiles * nkb >= 8 * all) {
       // + writing and adding partials, some 10 us
       const double cut = (double)tiles / all * tile + (wide ? 48.0 : 40.0) * f.bn;
       if (cut < 0.95 * cost) {
@@ -95,6 +130,7 @@ inline GemmPlan plan_gemm(int64_t M, int64_t N, int64_t nkb, int batches, bool g
       best.tiles_m = (int)tm;
       best.tiles_n = (int)tn;
       best.cols = cols;
+      best.cut = split ? Cut((int)(tiles % all), all, (int)nkb) : Cut();
     }
   }
   if (gated && M <= BM) {

@@ -604,3 +604,17 @@ def test_compiled_module_matches_eager(backend, cuda):
     got = run(torch.compile(mod, fullgraph=True, backend=backend))
     assert all(torch.equal(a, b) for a, b in zip(got, eager))
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("m,c,f,dtype,train", [
+    (19000, 384, 1536, "bfloat16", True), (4 * 69 * 69, 320, 1280, "bfloat16", True), (19300, 64, 1024, "float16", True),
+    (19201, 128, 2048, "bfloat16", False), (19300, 64, 1600, "bfloat16", False), (19300, 64, 256, "float32", True),
+    (19201, 64, 170, "float32", True), (19300, 64, 512, "float32", False), (18945, 192, 512, "float32", False),
+    (57200, 64, 256, "float32", True), (817, 408, 1096, "float16", True), (870, 424, 1696, "bfloat16", False)])
+def test_products_cut_among_few_tiles(m, c, f, dtype, train, cuda):
+    """A last wave of few tiles, cut along K among all SMs: an even share of less than one K block a slice
+    (three tiles for 148 SMs), and shares that leave runs beside the slices."""
+    dt = DTYPES[dtype]
+    args, dy = _inputs(m, c, f, dt, cuda, train, seed=m % 1000 + c)
+    dy = dy if train else None
+    _check(_run(args, dy, "silu"), _reference(args, dy, "silu", dt), f"{(m, c, f)} {dtype}")
