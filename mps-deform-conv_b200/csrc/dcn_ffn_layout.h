@@ -60,6 +60,7 @@ struct Cut {
     E = (int)std::min<int64_t>(W - S * R, (int64_t)R * rest);
   }
   DCN_HOST_DEVICE int64_t units() const { return (int64_t)R * rest; }
+  size_t slots() const { return (size_t)S * R + (E ? E + R - 1 : 0); }
   // Pieces of tile t: its S slices, then the runs that touch it, from `run` on.
   DCN_HOST_DEVICE int pieces(int t, int& run) const {
     run = 0;
@@ -79,9 +80,7 @@ struct GemmPlan {
   int tiles_m = 0, tiles_n = 0;
   int cols = 0;     // output columns of a tile
   Cut cut;          // split: of the tiles past whole rounds of the workers
-  size_t partial_bytes() const {
-    return split ? ((size_t)workers + (size_t)tiles_m * tiles_n * 2) * BM * (pair ? 2 : 1) * bn * 4 : 0;
-  }
+  size_t partial_bytes() const { return cut.slots() * BM * (pair ? 2 : 1) * bn * 4; }
 };
 
 // Column tile and CTA pairing: the choice whose waves of tiles cost least, a

@@ -1,6 +1,7 @@
 // Host-side enumeration of the gated feed-forward block's cut products: what the
 // workers of a launch write (Work) against what the reduction adds (Cut).  Prints
 // one line per fault and ends with their number; nothing runs on a GPU.
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -71,7 +72,70 @@ static void check_cut(int tiles, int W, int nkb) {
   EXPECT(busiest <= even, "W %d R %d nkb %d: a worker has %lld K blocks, an even share is %lld", W, R, nkb, busiest, even);
 }
 
-int main() {
+// The plan of a product M x N over nkb K blocks: what its pieces take of the
+// partial buffer, and the longest work of a worker against that without the cut.
+static bool check_plan(int64_t M, int64_t N, int64_t nkb, int batches, bool wide, bool weights) {
+  const GemmPlan p = plan_gemm(M, N, nkb, batches, false, true, wide, weights);
+  if (!p.split) {
+    EXPECT(p.partial_bytes() == 0, "%lld x %lld x %lld: a buffer without a cut", (long long)M, (long long)N, (long long)nkb);
+    return false;
+  }
+  GemmArgs a{};
+  a.tiles_m = p.tiles_m;
+  a.tiles_n = p.tiles_n;
+  a.batches = batches;
+  a.nseg = 1;
+  a.nk = (int)nkb;
+  a.split = 1;
+  a.cut = p.cut;
+  const int tiles = p.tiles_m * p.tiles_n * batches;
+  EXPECT(p.cut.R == tiles % p.workers, "%lld x %lld x %lld: %d tiles cut", (long long)M, (long long)N, (long long)nkb, p.cut.R);
+  int64_t top = -1, longest = 0;
+  for (int w = 0; w < p.workers; ++w) {
+    Work work(a, w, p.workers);
+    int64_t mine = 0;
+    for (; work.next(a); mine += work.kb1 - work.kb0)
+      if (work.slot > top) top = work.slot;
+    if (mine > longest) longest = mine;
+  }
+  const int64_t bytes = (top + 1) * BM * (p.pair ? 2 : 1) * p.bn * 4, uncut = div_up(tiles, p.workers) * nkb;
+  EXPECT((int64_t)p.partial_bytes() == bytes, "%lld x %lld x %lld: partial sums of %lld bytes in a buffer of %lld",
+         (long long)M, (long long)N, (long long)nkb, (long long)bytes, (long long)p.partial_bytes());
+  EXPECT(longest < uncut, "%lld x %lld x %lld: the cut takes %lld K blocks, no cut %lld", (long long)M, (long long)N,
+         (long long)nkb, (long long)longest, (long long)uncut);
+  return true;
+}
+
+// Sizes spread over the logarithm; the same every time.
+static uint64_t state = 1;
+static uint64_t next_random() {
+  state = state * 6364136223846793005ull + 1442695040888963407ull;
+  return state >> 33;
+}
+static int64_t size(double lo, double hi) {
+  return (int64_t)(lo * exp(log(hi / lo) * (double)(next_random() % 100001) / 1e5) + 0.5);
+}
+static int check_plans() {
+  int cuts = 0;
+  for (int i = 0; i < 60000; ++i) {
+    const bool wide = next_random() % 4 == 0;
+    const int seg = wide ? 6 : 1;
+    const int64_t M = size(1, 1e6), C = size(16, 4096), F = C * (1 + (int64_t)(next_random() % 5)) + (int64_t)(next_random() % 3);
+    if ((double)M * F > 5e8) continue;
+    cuts += check_plan(M, C, div_up(F, BK) * seg, 1, wide, true);        // y
+    cuts += check_plan(M, C, div_up(F, BK) * seg * 2, 1, wide, false);   // dx
+    cuts += check_plan(C, F, div_up(M, BK) * seg, 1, wide, false);       // dw_down
+    cuts += check_plan(F, C, div_up(M, BK) * seg, 2, wide, false);       // dw_gate, dw_up
+  }
+  return cuts;
+}
+
+int main(int argc, char** argv) {
+  if (argc > 1 && !strcmp(argv[1], "plans")) {
+    const int cuts = check_plans();
+    printf("%d cut products, %d faults\n", cuts, faults);
+    return faults != 0 || cuts < 1000;
+  }
   int combinations = 0;
   for (int W : {kSms / 2, kSms}) {
     for (int R = 1; R < W; ++R) {

@@ -25,3 +25,9 @@ def test_cut_products_add_every_k_block_once(program):
     wrote and no others, and no worker has more than an even share (to a K block)."""
     r = subprocess.run([program], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout
+
+
+def test_partial_buffers_hold_the_cut_products_sums_and_no_more(program):
+    """At sizes of the block's products; and no cut gives a worker as much as it has without one."""
+    r = subprocess.run([program, "plans"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
