@@ -551,7 +551,7 @@ __device__ __forceinline__ int scale_exponent(const float (&v)[CB], float top) {
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
 
 template <typename T>
-__device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, const float (&g)[CB], const float (&u)[CB]) {
+__device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, bool row_in, const float (&g)[CB], const float (&u)[CB]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -561,7 +561,8 @@ __device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, const flo
     }
   } else {
     const float tg = largest(g), tu = largest(u);
-    const bool fits = fminf(tg, tu) >= 0.0625f && fmaxf(tg, tu) < 32768.0f;
+    // a row past the matrix holds anything and has no say in how the others are kept
+    const bool fits = !row_in || (fminf(tg, tu) >= 0.0625f && fmaxf(tg, tu) < 32768.0f);
     int eg = 14, eu = 14;
     if (__all_sync(0xffffffffu, fits)) {
 #pragma unroll
@@ -1045,7 +1046,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
         const bool rows_in = row0 - q * 32 < a.M;
         const int64_t at = ((int64_t)(row0 >> 7) * a.ldo + (c0 >> 3)) * (BM * 16) + (q * 32 + lane) * 16;
         if constexpr (GATED) {
-          if (a.saved) save_gate_up<T>(saved_block(c), lane, v, u);
+          if (a.saved) save_gate_up<T>(saved_block(c), lane, row_in, v, u);
           gate_block<WIDE>(a.act, v, u, v);
           if (row0 + 32 > a.M && !row_in) {
 #pragma unroll

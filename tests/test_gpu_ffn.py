@@ -618,3 +618,25 @@ def test_products_cut_among_few_tiles(m, c, f, dtype, train, cuda):
     args, dy = _inputs(m, c, f, dt, cuda, train, seed=m % 1000 + c)
     dy = dy if train else None
     _check(_run(args, dy, "silu"), _reference(args, dy, "silu", dt), f"{(m, c, f)} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_few_training_rows_do_not_depend_on_earlier_calls(dtype, cuda):
+    """One tile with fewer rows than 128: what an earlier call left in shared memory where rows are missing
+    does not reach a gradient's bits.  Weight rows many decades apart, so that the two ways of keeping gate
+    and up for the backward (more than 256 channels) differ in the small ones."""
+    dt = DTYPES[dtype]
+    args, dy = _inputs(40, 512, 2048, dt, cuda, False, seed=41)
+    decades = torch.exp2(torch.arange(2048, device=cuda) % 16 * -2.0).to(dt)
+    args[1], args[2] = args[1] * decades[:, None], args[2] * decades.flip(0)[:, None]
+    fill, _ = _inputs(128, 512, 2048, dt, cuda, False, seed=42)
+    results = []
+    for scale in (1.0, 1e4, 1.0, 1e-6, 0.0):
+        other = [fill[0] * scale, *args[1:]]
+        leaves = [t if t is None else t.detach().requires_grad_(True) for t in args]
+        mdc._get_lib().gated_feed_forward_forward(*other, 0, True)
+        y = mdc.gated_feed_forward(*leaves)
+        results.append([y.detach(), *torch.autograd.grad(y, leaves[:4], dy)])
+    for got in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
+    _check(results[0], _reference(args, dy, "silu", dt))
