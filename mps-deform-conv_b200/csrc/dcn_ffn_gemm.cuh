@@ -334,7 +334,7 @@ __device__ __forceinline__ void load_panels(uint32_t dst, const CUtensorMap* map
 }
 
 // ---------------------------------------------------------------- activations
-// ACCURATE (fp32 data): CUDA's expf, erff and IEEE division.  Else the matching
+// ACCURATE (fp32 data): CUDA's expf, normcdff and IEEE division.  Else the matching
 // hardware approximations, whose few ulp are far below a 16-bit result's
 // rounding, with subnormals flushed (an exponential below 2^-126 is 0 here;
 // the forms that keep them cost four instructions more each).
@@ -354,7 +354,9 @@ __device__ __forceinline__ float sigmoid(float x) {
   // far below zero the exponential overflows to inf and the quotient is 0, as it should be
   return ACCURATE ? 1.0f / (1.0f + expf(-x)) : rcp_fast(1.0f + exp2_fast(-kLog2e * x));
 }
-// The normal distribution function and exp(-x^2 / 2).  Fast form: with z = |x|,
+// The normal distribution function and exp(-x^2 / 2).  fp32: not 1 + erf(x / sqrt 2),
+// which cancels in the lower tail (at -5 a tenth of the value, below -5.5 all of it;
+// normcdff is within 5 ulp).  Fast form: with z = |x|,
 // Phi(-z) = exp(-z^2 / 2) R(z), where R(z) = erfcx(z / sqrt 2) / 2 is smooth and
 // R ~ t (c0 + c1 t + ... + c5 t^5), t = 1 / (1 + 0.308 z): coefficients fitted
 // here for the least largest relative error, 4e-6 over z in [0, 14] (past that
@@ -362,7 +364,7 @@ __device__ __forceinline__ float sigmoid(float x) {
 // derivative needs the same exponential.
 template <bool ACCURATE>
 __device__ __forceinline__ float2 normal_cdf(float x) {
-  if (ACCURATE) return make_float2(0.5f * (1.0f + erff(x * 0.70710678118654752f)), expf(-0.5f * x * x));
+  if (ACCURATE) return make_float2(normcdff(x), expf(-0.5f * x * x));
   const float z = fabsf(x);
   const float t = rcp_fast(fmaf(0.308f, z, 1.0f));
   const float e = exp2_fast((-0.5f * kLog2e) * (z * z));

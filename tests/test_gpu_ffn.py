@@ -640,3 +640,22 @@ def test_few_training_rows_do_not_depend_on_earlier_calls(dtype, cuda):
     for got in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
     _check(results[0], _reference(args, dy, "silu", dt))
+
+
+@pytest.mark.parametrize("m", [8, 449])
+def test_gelu_keeps_its_lower_tail(m, cuda):
+    """fp32, one channel with weights of 1 and up = 1 (its bias), so that y is gelu(x) and dx its derivative
+    with no other rounding.  normcdff and expf are documented within 5 and 2 units in the last place (2^-23
+    each at most); the product x Phi adds one rounding.  In the derivative Phi + x phi: x^2 / 2 carries two
+    roundings into the exponent, phi's constant, two products and the sum four more."""
+    x = torch.linspace(-10, -3, m, device=cuda).mul(64).round().div(64).view(m, 1)
+    one, zero = torch.ones(1, 1, device=cuda), torch.zeros(1, 1, device=cuda)
+    args = [x, one, zero, one, torch.zeros(1, device=cuda), torch.ones(1, device=cuda), None]
+    v = x.double()  # torch's ndtr cancels there, in 64 bits too
+    cdf, density = 0.5 * torch.special.erfc(v * -math.sqrt(0.5)), torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+    y, dx = _run(args, None, "gelu")[0], _run(args, one.expand(m, 1), "gelu")[1]
+    exact = v * cdf
+    assert ((y.double() - exact).abs() <= (5 + 1) * 2.0 ** -23 * exact.abs()).all()
+    assert ((_run(args, one.expand(m, 1), "gelu")[0].double() - exact).abs() <= (5 + 1) * 2.0 ** -23 * exact.abs()).all()
+    err = 5 * 2.0 ** -23 * cdf + (v * density).abs() * (v * v * 2.0 ** -24 + 2 * 2.0 ** -23 + 4 * 2.0 ** -24)
+    assert ((dx.double() - (cdf + v * density)).abs() <= err + 2.0 ** -24 * err).all()
