@@ -17,6 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 
 from . import ops as _ops
 from . import optim
@@ -579,6 +580,13 @@ def _activation(name: str) -> int:
     return code
 
 
+def _refuse_forward_mode(tensors) -> None:
+    """A tangent would be dropped without a word where no input requires grad."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("gated_feed_forward has no forward-mode derivative")
+
+
 def _validate_feed_forward(input, w_gate, w_up, w_down, b_gate, b_up, b_down, activation) -> int:
     """Checks of a traced call (the extension makes them otherwise); returns the activation's code."""
     act = _activation(activation)
@@ -637,6 +645,7 @@ def gated_feed_forward(
 
     Raises:
         ValueError: If input is not on a CUDA device or shapes do not fit.
+        NotImplementedError: If an input carries a forward-mode tangent.
 
     float32, float16 or bfloat16, all tensors alike.  Sums are fp32; the hidden
     values are rounded to the dtype between the two products.  With
@@ -644,6 +653,8 @@ def gated_feed_forward(
     which then computes gate and up again.  The parameter-gradient hook is
     called once for each of the three weights.
     """
+    if not torch.compiler.is_compiling():
+        _refuse_forward_mode((input, w_gate, w_up, w_down, b_gate, b_up, b_down))
     if input.is_cuda and not torch.compiler.is_compiling():  # checked by the extension
         act = _activation(activation)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (

@@ -163,3 +163,14 @@ def test_module_compiles_to_one_graph_on_meta():
     assert y.shape == x.shape
     assert any("gated_feed_forward" in t for t in graphs[0])
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("k", range(7))
+def test_forward_mode_is_refused(k):
+    """No input requires grad, so autograd sees no call: the tangent must not vanish silently."""
+    a = _args(device="meta")
+    with torch.autograd.forward_ad.dual_level():
+        assert mdc.gated_feed_forward(*a).shape == (6, 8)  # nothing carries a tangent
+        a[k] = torch.autograd.forward_ad.make_dual(a[k], torch.zeros_like(a[k]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            mdc.gated_feed_forward(*a)

@@ -659,3 +659,13 @@ def test_gelu_keeps_its_lower_tail(m, cuda):
     assert ((_run(args, one.expand(m, 1), "gelu")[0].double() - exact).abs() <= (5 + 1) * 2.0 ** -23 * exact.abs()).all()
     err = 5 * 2.0 ** -23 * cdf + (v * density).abs() * (v * v * 2.0 ** -24 + 2 * 2.0 ** -23 + 4 * 2.0 ** -24)
     assert ((dx.double() - (cdf + v * density)).abs() <= err + 2.0 ** -24 * err).all()
+
+
+def test_forward_mode_is_refused(cuda):
+    args, _ = _inputs(6, 16, 24, torch.float32, cuda, True)
+    for k, t in enumerate(args):
+        def call(x):
+            return mdc.gated_feed_forward(*args[:k], x, *args[k + 1:])  # noqa: B023
+
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
