@@ -27,6 +27,9 @@ static int guarded(F&& f) {
   }
 }
 
+// A kernel reads and writes whole elements: elsewhere it would fault.
+static bool on(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
 constexpr int64_t kMaxNumel = int64_t(1) << 40;  // keeps every chunk count and byte offset in range
 
 static int check_adamw(const dcn_adamw_options* o, const dcn_adamw_tensor* t, int64_t n) {
@@ -107,6 +110,16 @@ static int check_adamw(const dcn_adamw_options* o, const dcn_adamw_tensor* t, in
   const char* scalar = meets_any(o->grad_scale) ? "grad_scale" : meets_any(o->lr_device) ? "lr_device" : nullptr;
   if (scalar)
     return fail(DCN_ERR_INVALID_ARGUMENT, "%s must not overlap a parameter, master copy, state or step counter", scalar);
+  for (int64_t i = 0; i < n; ++i) {
+    const dcn_adamw_tensor& e = t[i];
+    const int64_t es = elem_bytes(e.dtype), state = o->state_bits == 8 ? 1 : 4;
+    const bool scales = o->state_bits != 8 || (on(e.exp_avg_scale, 4) && on(e.exp_avg_sq_scale, 4));
+    if (!on(e.step, 4) || (e.numel && !(on(e.param, es) && on(e.grad, es) && on(e.exp_avg, state) &&
+                                        on(e.exp_avg_sq, state) && on(e.master, 4) && scales)))
+      return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: a pointer is not aligned to its elements", (long long)i);
+  }
+  if (!on(o->grad_scale, 4) || !on(o->lr_device, 4))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "grad_scale or lr_device is not aligned to 4 bytes");
   return DCN_OK;
 }
 
@@ -147,15 +160,17 @@ static FfnProblem problem(const dcn_ffn_desc* d) {
   return {d->dtype, d->activation, d->tokens, d->channels, d->hidden};
 }
 
-static bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool on16(const void* p) { return on(p, 16); }
 
-static int check_ffn_tensors(const dcn_ffn_tensors* t) {
+static int check_ffn_tensors(const dcn_ffn_tensors* t, int64_t es) {
   if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down)
     return fail(DCN_ERR_INVALID_ARGUMENT, "NULL tensor pointer (x, w_gate, w_up, w_down)");
   if ((t->b_gate != nullptr) != (t->b_up != nullptr))
     return fail(DCN_ERR_INVALID_ARGUMENT, "b_gate and b_up go together");
   if (!on16(t->x) || !on16(t->w_gate) || !on16(t->w_up) || !on16(t->w_down))
     return fail(DCN_ERR_INVALID_ARGUMENT, "x and the weights must be 16-byte aligned");
+  if (!on(t->b_gate, es) || !on(t->b_up, es) || !on(t->b_down, es))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "a bias is not aligned to its elements");
   return DCN_OK;
 }
 
@@ -194,18 +209,20 @@ size_t dcn_grad_norm_workspace_size(const dcn_tensor_ref* grads, int64_t n) {
 int dcn_grad_norm(const dcn_tensor_ref* grads, int64_t n, double max_norm, double loss_scale, float* norm,
                   float* factor, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&] {
-    const int r = check_refs(grads, n);
+    int r = check_refs(grads, n);
     if (r != DCN_OK) return r;
     if (!(loss_scale > 0.0 && isfinite(loss_scale)))
       return fail(DCN_ERR_INVALID_ARGUMENT, "loss_scale must be positive and finite, got %g", loss_scale);
     if (isnan(max_norm)) return fail(DCN_ERR_INVALID_ARGUMENT, "max_norm is NaN");
     if (!norm || !factor) return fail(DCN_ERR_INVALID_ARGUMENT, "NULL output (norm, factor)");
-    for (int64_t i = 0; i < n; ++i)
+    if (!on(norm, 4) || !on(factor, 4)) return fail(DCN_ERR_INVALID_ARGUMENT, "norm or factor is not aligned to 4 bytes");
+    for (int64_t i = 0; i < n; ++i) {
       if (grads[i].numel && !grads[i].data)
         return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: NULL pointer", (long long)i);
-    const size_t need = grad_norm_workspace(grads, n);
-    if (workspace_bytes < need || !workspace)
-      return fail(DCN_ERR_WORKSPACE, "grad_norm workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+      if (grads[i].numel && !on(grads[i].data, elem_bytes(grads[i].dtype)))
+        return fail(DCN_ERR_INVALID_ARGUMENT, "tensor %lld: the pointer is not aligned to its elements", (long long)i);
+    }
+    if ((r = check_buffer(workspace, workspace_bytes, grad_norm_workspace(grads, n), "grad_norm workspace")) != DCN_OK) return r;
     const cudaError_t e = grad_norm(grads, n, max_norm, loss_scale, norm, factor, workspace, (cudaStream_t)stream);
     return e == cudaSuccess ? ok() : cuda_fail(e, "grad_norm");
   });
@@ -234,7 +251,7 @@ int dcn_ffn_forward(const dcn_ffn_desc* desc, const dcn_ffn_tensors* t, void* y,
     int r = check_ffn(desc);
     if (r != DCN_OK) return r;
     if (desc->tokens == 0) return ok();
-    if ((r = check_ffn_tensors(t)) != DCN_OK) return r;
+    if ((r = check_ffn_tensors(t, elem_bytes(desc->dtype))) != DCN_OK) return r;
     if (!y && !saved) return fail(DCN_ERR_INVALID_ARGUMENT, "y and saved are both NULL");
     if (y && !on16(y)) return fail(DCN_ERR_INVALID_ARGUMENT, "y must be 16-byte aligned");
     const FfnProblem p = problem(desc);
@@ -257,9 +274,12 @@ int dcn_ffn_backward(const dcn_ffn_desc* desc, const dcn_ffn_tensors* t, const v
     const FfnGrads g{grads->x, grads->w_gate, grads->w_up, grads->w_down, grads->b_gate, grads->b_up, grads->b_down};
     if (!on16(g.x) || !on16(g.w_gate) || !on16(g.w_up) || !on16(g.w_down))
       return fail(DCN_ERR_INVALID_ARGUMENT, "gradients of x and of the weights must be 16-byte aligned");
+    const int64_t size = elem_bytes(desc->dtype);
+    if (!on(g.b_gate, size) || !on(g.b_up, size) || !on(g.b_down, size))
+      return fail(DCN_ERR_INVALID_ARGUMENT, "a bias gradient is not aligned to its elements");
     cudaStream_t st = (cudaStream_t)stream;
     if (desc->tokens == 0) {  // sums over no rows
-      const size_t es = (size_t)elem_bytes(desc->dtype), c = (size_t)desc->channels, f = (size_t)desc->hidden;
+      const size_t es = (size_t)size, c = (size_t)desc->channels, f = (size_t)desc->hidden;
       const std::pair<void*, size_t> zero[6] = {{g.w_gate, c * f}, {g.w_up, c * f}, {g.w_down, c * f},
                                                 {g.b_gate, f},     {g.b_up, f},     {g.b_down, c}};
       for (auto& z : zero)
@@ -270,7 +290,7 @@ int dcn_ffn_backward(const dcn_ffn_desc* desc, const dcn_ffn_tensors* t, const v
       if (params_ready) params_ready(user_data);
       return ok();
     }
-    if ((r = check_ffn_tensors(t)) != DCN_OK) return r;
+    if ((r = check_ffn_tensors(t, elem_bytes(desc->dtype))) != DCN_OK) return r;
     if (!grad_y || !on16(grad_y))
       return fail(DCN_ERR_INVALID_ARGUMENT, "grad_y is NULL or not 16-byte aligned");
     const FfnProblem p = problem(desc);

@@ -174,3 +174,18 @@ def test_forward_mode_is_refused(k):
         a[k] = torch.autograd.forward_ad.make_dual(a[k], torch.zeros_like(a[k]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             mdc.gated_feed_forward(*a)
+
+
+@pytest.mark.parametrize("name", ["b_gate", "b_up", "b_down"])
+@pytest.mark.parametrize("dtype,off", [(_abi.DCN_BFLOAT16, 1), (_abi.DCN_FLOAT32, 2)])
+def test_biases_off_their_elements_are_refused(name, dtype, off):
+    """A kernel's access there would fault the GPU."""
+    lib = _abi.load()
+    d = _desc(dtype)
+    bad = _tensors(**{name: 0x70000 + off})
+    rc = lib.dcn_ffn_forward(ctypes.byref(d), ctypes.byref(bad), 0x1000000, None, 0, 0x2000000, 1 << 40, None)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "aligned" in lib.dcn_last_error().decode()
+    for tensors, grads in ((bad, _tensors()), (_tensors(), bad)):
+        rc = lib.dcn_ffn_backward(ctypes.byref(d), ctypes.byref(tensors), 0x9000000, 0x4000000, 1 << 40,
+                                  ctypes.byref(grads), 0x2000000, 1 << 40, None, _abi.PARAMS_READY_FN(), None)
+        assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "aligned" in lib.dcn_last_error().decode()

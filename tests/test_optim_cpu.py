@@ -144,3 +144,36 @@ def test_state_layouts():
     assert not c.float().any()
     with pytest.raises(ValueError, match="state_bits"):
         optim.new_state(w, 4)
+
+
+@pytest.mark.parametrize("kw,bits,needle", [
+    (dict(param=0x100002), 32, "aligned"), (dict(param=0x100001, dtype=_abi.DCN_BFLOAT16), 32, "aligned"),
+    (dict(grad=0x110002), 32, "aligned"), (dict(exp_avg=0x120002), 32, "aligned"),
+    (dict(exp_avg_sq=0x130001), 32, "aligned"), (dict(master=0x140002), 32, "aligned"), (dict(step=0x150002), 32, "aligned"),
+    (dict(exp_avg_scale=0x160002, exp_avg_sq_scale=0x170000), 8, "aligned"),
+    (dict(exp_avg_scale=0x160000, exp_avg_sq_scale=0x170001), 8, "aligned"),
+])
+def test_adamw_refuses_pointers_off_their_elements(kw, bits, needle):
+    """A kernel's access there would fault the GPU."""
+    rc, msg = _call(_options(state_bits=bits), _tensors(**kw), 1)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and needle in msg
+
+
+@pytest.mark.parametrize("options", [dict(grad_scale=0x900002), dict(lr_device=0x900001)])
+def test_adamw_refuses_scalars_off_their_elements(options):
+    rc, msg = _call(_options(**options), _tensors(), 1)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "aligned" in msg
+
+
+def test_grad_norm_refuses_pointers_off_their_elements():
+    lib = _abi.load()
+
+    def call(data=0x1000, dtype=_abi.DCN_FLOAT32, norm=0x2000, factor=0x2004, ws=0x4000):
+        ref = (_abi.DcnTensorRef * 1)(_abi.DcnTensorRef(data, 100, dtype, 0))
+        rc = lib.dcn_grad_norm(ref, 1, 1.0, 1.0, norm, factor, ws, 1 << 16, None)
+        return rc, lib.dcn_last_error().decode()
+
+    for kw in (dict(data=0x1002), dict(data=0x1001, dtype=_abi.DCN_FLOAT16), dict(norm=0x2002), dict(factor=0x2005),
+               dict(ws=0x4004), dict(ws=0x4010)):
+        rc, msg = call(**kw)
+        assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "aligned" in msg, kw
