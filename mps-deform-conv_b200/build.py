@@ -10,12 +10,14 @@
    reference's pybind11 module ``_C`` and calls the C ABI.
 
 Usage:  python mps-deform-conv_b200/build.py [--force] [--no-bounds]
-Every step is incremental (skipped when outputs are newer than sources).
+Every step is incremental (skipped when outputs are newer than sources and this
+file; an object also keeps the command that made it).
 """
 from __future__ import annotations
 
 import glob
 import os
+import shlex
 import shutil
 import subprocess
 import sys
@@ -52,6 +54,14 @@ def _stale(out: str, deps) -> bool:
     return any(not os.path.exists(d) or os.path.getmtime(d) > t for d in deps)
 
 
+def _read(path: str) -> str:
+    """The file's text; empty when there is none."""
+    if not os.path.exists(path):
+        return ""
+    with open(path) as f:
+        return f.read()
+
+
 def _read_deps(path: str):
     """Files named in a make dependency file; a missing file when it is absent (so the object is stale)."""
     if not os.path.exists(path):
@@ -67,7 +77,7 @@ def build_lib(force: bool = False, verbose: bool = False, bounds: bool = False) 
     bdir = os.path.join(BUILD, "bounds") if bounds else BUILD
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     deps = srcs + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh")) + \
-        glob.glob(os.path.join(INCLUDE, "*.h"))
+        glob.glob(os.path.join(INCLUDE, "*.h")) + [os.path.abspath(__file__)]
     if not force and not _stale(out, deps):
         return out
     os.makedirs(bdir, exist_ok=True)
@@ -75,18 +85,23 @@ def build_lib(force: bool = False, verbose: bool = False, bounds: bool = False) 
     nvcc = [_nvcc(), *NVCC_FLAGS, *(["-DDCN_DEBUG_BOUNDS"] if bounds else []), "-I", INCLUDE, "-I", CSRC]
 
     def compile_one(src: str):
-        """Compile one file when it or a header it read last time is newer; returns (object, log)."""
+        """Compile one file when it or a header it read last time is newer, or the command another one;
+        returns (object, log)."""
         obj = os.path.join(bdir, os.path.basename(src) + ".o")
-        if not force and not _stale(obj, [src, *_read_deps(obj + ".d")]) and os.path.exists(obj + ".log"):
-            with open(obj + ".log") as f:
-                return obj, f.read()
-        r = subprocess.run([*nvcc, "-MMD", "-MF", obj + ".d", "-c", src, "-o", obj], capture_output=True, text=True)
+        cmd = [*nvcc, "-MMD", "-MF", obj + ".d", "-c", src, "-o", obj]
+        if not force and not _stale(obj, [src, *_read_deps(obj + ".d")]) and os.path.exists(obj + ".log") and \
+                _read(obj + ".cmd") == shlex.join(cmd):
+            return obj, _read(obj + ".log")
+        if os.path.exists(obj + ".cmd"):
+            os.remove(obj + ".cmd")
+        r = subprocess.run(cmd, capture_output=True, text=True)
         log = r.stdout + r.stderr
         if r.returncode != 0:
             sys.stderr.write(log)
             raise RuntimeError(f"nvcc failed on {src}")
-        with open(obj + ".log", "w") as f:
-            f.write(log)
+        for suffix, text in ((".log", log), (".cmd", shlex.join(cmd))):
+            with open(obj + suffix, "w") as f:
+                f.write(text)
         return obj, log
 
     with ThreadPoolExecutor(max_workers=max(1, min(len(srcs), os.cpu_count() or 1))) as pool:
