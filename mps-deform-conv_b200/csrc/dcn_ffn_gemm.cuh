@@ -189,10 +189,10 @@ struct GemmArgs {
 // lanes of one warp) lies together, each 16-byte piece of the 32 lanes side by
 // side, so both passes move whole lines:
 //   16-bit data: gate, up as fp16: 11 bits, not bf16's 8, of values that the
-//     derivative multiplies, at the same size.  Where a warp has a row whose
-//     largest value is outside [2^-4, 2^15), its values are multiplied by powers
-//     of two per (row, 16 columns) that bring the largest below 2^15.  One int16
-//     per lane holds the two exponents (14: as they are);
+//     derivative multiplies, at the same size.  A row whose largest value of the
+//     16 columns is outside [2^-4, 2^15) is multiplied by powers of two that bring
+//     the largest below 2^15.  One int16 per lane holds the two exponents (14: as
+//     they are); a warp without such a row skips the scaling;
 //   fp32 data: gate, up as fp32.
 template <typename T>
 __host__ __device__ inline size_t saved_block_offset(int64_t m_block, int64_t col_block, int64_t col_blocks) {
@@ -563,7 +563,7 @@ __device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, bool row_
     }
   } else {
     const float tg = largest(g), tu = largest(u);
-    // a row past the matrix holds anything and has no say in how the others are kept
+    // a row past the matrix holds anything
     const bool fits = !row_in || (fminf(tg, tu) >= 0.0625f && fmaxf(tg, tu) < 32768.0f);
     int eg = 14, eu = 14;
     if (__all_sync(0xffffffffu, fits)) {
@@ -573,8 +573,9 @@ __device__ __forceinline__ void save_gate_up(uint8_t* block, int lane, bool row_
         *reinterpret_cast<uint4*>(block + 1024 + j * 512 + lane * 16) = pack8<__half>(u, j);
       }
     } else {
-      eg = scale_exponent(g, tg);
-      eu = scale_exponent(u, tu);
+      // per row: what a row keeps does not depend on its neighbours
+      eg = fits ? 14 : scale_exponent(g, tg);
+      eu = fits ? 14 : scale_exponent(u, tu);
       const float sg = exp2_int(14 - eg), su = exp2_int(14 - eu);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {

@@ -669,3 +669,85 @@ def test_forward_mode_is_refused(cuda):
 
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(call, (t,), (torch.ones_like(t),))
+
+
+# The backward reads gate and up back above these many channels, and computes them again up to them.
+SAVED_CHANNELS = [("float16", 264), ("bfloat16", 264), ("bfloat16", 512), ("float32", 136)]
+
+
+def _reads_saved_values(args):
+    """The state that the forward leaves is more than the hidden values in their panels."""
+    (m, c), f = args[0].shape, args[1].shape[0]
+    saved = mdc._get_lib().gated_feed_forward_forward(*args, 0, True)[1].numel()
+    panels = (3 if args[0].dtype == torch.float32 else 1) * (-(-m // 128) * 128) * (-(-f // 8) * 8) * 2
+    return saved >= panels + 2 * 2 * m * f
+
+
+@pytest.mark.parametrize("dtype,c", SAVED_CHANNELS)
+def test_saved_state_rows_keep_to_themselves(dtype, c, cuda):
+    """Rows that are not finite, or far outside fp16's range, leave the others' results as they are, bit for
+    bit, those of their own 32-row block too.  Hidden units many decades apart, so that the ways of keeping
+    a block differ in the small ones."""
+    dt = DTYPES[dtype]
+    args, dy = _inputs(300, c, 96, dt, cuda, True, seed=51)
+    decades = torch.exp2(torch.arange(96, device=cuda) % 16 * -2.0).to(dt)
+    for k in (1, 2, 4, 5):
+        args[k] = args[k] * (decades[:, None] if args[k].dim() == 2 else decades)
+    assert _reads_saved_values(args)
+    dy[5] = dy[299] = 0.0  # with finite values these rows then add nothing to the weights' gradients
+    clean = _run(args, dy, "silu")
+    _check(clean, _reference(args, dy, "silu", dt))
+    keep = torch.ones(300, dtype=torch.bool, device=cuda)
+    keep[5] = keep[299] = False
+    big = 20.0 if dtype == "float16" else 3e4  # the hidden values of these rows stay finite
+    for a, b in ((float("nan"), float("inf")), (big, -big), (0.0, 2.0 ** -14)):
+        x = args[0].clone()
+        x[5], x[299] = a, b
+        got = _run([x, *args[1:]], dy, "silu")
+        assert torch.equal(got[0][keep], clean[0][keep]) and torch.equal(got[1][keep], clean[1][keep])
+        if not math.isfinite(a):
+            assert got[0][5].isnan().all() and got[1][5].isnan().all() and not got[0][299].isfinite().any()
+        else:
+            assert all(torch.equal(p, q) for p, q in zip(got[2:], clean[2:])), (a, b)
+
+
+@pytest.mark.parametrize("dtype,c", SAVED_CHANNELS)
+def test_saved_state_far_tails_and_small_values(dtype, c, cuda):
+    """Gate and up many decades apart in one row and between rows, beyond fp16's range where the type has it."""
+    dt = DTYPES[dtype]
+    reach = 6 if dtype == "float16" else 20
+    args, dy = _inputs(96, c, 64, dt, cuda, False, seed=52)
+    scale = torch.exp2(torch.linspace(-reach, reach, 64, device=cuda)).to(dt)
+    args[2] = args[2] * scale[:, None]
+    args[1] = args[1] * scale.flip(0)[:, None]
+    for rows in (torch.zeros(96, device=cuda), torch.linspace(-4, 4, 96, device=cuda).round()):
+        case = [(args[0].float() * torch.exp2(rows)[:, None]).to(dt), *args[1:]]
+        assert _reads_saved_values(case)
+        for act in ("silu", "relu"):
+            got, ref = _run(case, dy, act), _reference(case, dy, act, dt)
+            if dtype == "float16":  # rounds 65520 and above to inf
+                for t, (v, e) in zip(got, ref):
+                    assert (t[v.abs() - e >= 65520].double() == math.inf * v.sign()[v.abs() - e >= 65520]).all()
+                    past = v.abs() + e >= 65504
+                    assert past.float().mean() < 0.05  # the check says something
+                    t[past], v[past] = 0.0, 0.0
+            _check(got, ref, "decades")
+
+
+@pytest.mark.parametrize("dtype,c", [("bfloat16", 264), ("bfloat16", 512), ("float32", 136)])
+@pytest.mark.parametrize("power", [-30, 30])
+def test_saved_state_outside_fp16(dtype, c, power, cuda):
+    """All of gate and up near 2^30 or 2^-30 (relu, whose products scale with them exactly): the gradients are
+    those of the same rows near 1, scaled.  Per factor and sum half a step of the type, and half a step of 11 bits of
+    what was saved; the sums' own error is below another half step."""
+    dt = DTYPES[dtype]
+    args, dy = _inputs(96, c, 64, dt, cuda, False, seed=53)
+    assert _reads_saved_values(args)
+    scaled = [args[0] * 2.0 ** power, *args[1:]]
+    ref = _reference(args, dy, "relu", dt)
+    got = _run(scaled, dy, "relu")
+    u = max(torch.finfo(dt).eps / 2, 0 if dt == torch.float32 else 2.0 ** -11)
+    # y ~ s^2; dgate and dup ~ s, so dx ~ s and the gate and up gradients ~ s^2; dw_down ~ s^2
+    for name, t, (v, _), order in zip(NAMES, got, ref, (2, 1, 2, 2, 2)):
+        err = float((t.double() * 2.0 ** (-power * order) - v).norm() / v.norm())
+        assert err <= 4 * u + (2.0 ** -20 if dt == torch.float32 else 2.0 ** -11), (name, err)
