@@ -201,8 +201,20 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the states keep their own dtypes (torch casts floating
-        point states to the parameter's)."""
+        point states to the parameter's), and a learning rate held as a tensor
+        stays that tensor and takes the loaded value, since a schedule writes it.
+        The states are new tensors: a step captured before is captured again."""
+        held = [g["lr"] for g in self.param_groups]
         super().load_state_dict(state_dict)
+        taken = {}
+        for group, lr in zip(self.param_groups, held):
+            value = float(group["lr"])
+            if isinstance(lr, Tensor):
+                if taken.setdefault(id(lr), value) != value:  # groups that shared it and are loaded with different ones
+                    lr = lr.detach().clone()
+                group["lr"] = lr.fill_(value)
+            elif isinstance(group["lr"], Tensor) and group["params"]:
+                group["lr"] = group["lr"].detach().to(group["params"][0].device)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, params):

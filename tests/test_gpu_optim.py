@@ -532,3 +532,27 @@ def test_training_step_norm_then_adamw_on_a_side_stream(cuda):
         # the factor's own error (7 roundings) enters the gradient once and its square's root once
         err = 3 * U * p.abs() + 30 * U * (rate * m_new).abs() + rate * 12 * U * terms
         assert ((s["masters"][k].cpu().double() - ref).abs() <= err).all()
+
+
+def test_loading_a_checkpoint_mapped_to_the_cpu(cuda, tmp_path):
+    """States and the learning rate come back to the device, the latter into the optimizer's own tensor."""
+    def make():
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 3000, device=cuda).bfloat16())
+        p.grad = torch.linspace(1, -1, 3000, device=cuda).bfloat16()
+        return p, optim.AdamW([p], lr=torch.tensor(1e-2, device=cuda), state_bits=8, master_weights=True)
+
+    p, opt = make()
+    opt.step()
+    opt.param_groups[0]["lr"].fill_(3e-2)
+    torch.save([p.detach(), opt.state_dict()], tmp_path / "checkpoint")
+    opt.step()
+    q, other = make()
+    lr = other.param_groups[0]["lr"]
+    value, state = torch.load(tmp_path / "checkpoint", map_location="cpu")
+    other.load_state_dict(state)
+    with torch.no_grad():
+        q.copy_(value)
+    assert other.param_groups[0]["lr"] is lr
+    other.step()
+    assert torch.equal(p, q)
+    assert all(torch.equal(a.view(torch.uint8), other.state[q][k].view(torch.uint8)) for k, a in opt.state[p].items())

@@ -177,3 +177,24 @@ def test_grad_norm_refuses_pointers_off_their_elements():
                dict(ws=0x4004), dict(ws=0x4010)):
         rc, msg = call(**kw)
         assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "aligned" in msg, kw
+
+
+def test_loading_keeps_the_learning_rate_tensor():
+    """A schedule writes the tensor that the optimizer was made with."""
+    def make(lr, lr2=None):
+        p = [torch.nn.Parameter(torch.zeros(4)) for _ in range(2)]
+        groups = [dict(params=[p[0]]), dict(params=[p[1]], **({} if lr2 is None else dict(lr=lr2)))]
+        return optim.AdamW(groups, lr=lr)
+
+    lr = torch.tensor(0.5)
+    opt = make(lr)
+    opt.load_state_dict(make(torch.tensor(0.25)).state_dict())
+    assert all(g["lr"] is lr for g in opt.param_groups) and float(lr) == 0.25
+    opt.load_state_dict(make(0.125).state_dict())  # saved by an optimizer with a plain number
+    assert all(g["lr"] is lr for g in opt.param_groups) and float(lr) == 0.125
+    opt.load_state_dict(make(0.75, 0.5).state_dict())  # one tensor cannot hold two values
+    assert opt.param_groups[0]["lr"] is lr and [float(g["lr"]) for g in opt.param_groups] == [0.75, 0.5]
+    plain, source = make(0.5), torch.tensor(0.25)
+    plain.load_state_dict(make(source).state_dict())
+    assert all(isinstance(g["lr"], torch.Tensor) and g["lr"] is not source and float(g["lr"]) == 0.25
+               for g in plain.param_groups)
