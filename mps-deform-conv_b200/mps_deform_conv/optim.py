@@ -31,6 +31,11 @@ def _require_cuda(tensors: Sequence[Tensor], name: str) -> None:
         raise ValueError(f"{name} must be on CUDA device, got {tensors[0].device}")
 
 
+def _same_order(a: Tensor, b: Tensor) -> bool:
+    """The two tensors' elements lie in the same order in memory."""
+    return a.shape == b.shape and ((a.is_contiguous() and b.is_contiguous()) or a.stride() == b.stride())
+
+
 def new_step(device, taken: int = 0) -> Tensor:
     """A step counter of ``adamw_step``: two int32, the steps taken and a ticket
     that the kernel uses and leaves at 0."""
@@ -203,7 +208,20 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but the states keep their own dtypes (torch casts floating
         point states to the parameter's), and a learning rate held as a tensor
         stays that tensor and takes the loaded value, since a schedule writes it.
-        The states are new tensors: a step captured before is captured again."""
+        The states are new tensors: a step captured before is captured again.
+        32-bit states saved from a parameter in another memory format are brought
+        to this one's.
+
+        Raises:
+            ValueError: If 8-bit states are of another memory format; their scales
+                belong to 256 elements in memory order.
+        """
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, params):
+            for key, value in state_dict["state"].get(i, {}).items():
+                if isinstance(value, Tensor) and value.dtype == torch.float8_e4m3fn and not _same_order(value, p):
+                    raise ValueError(f"{key} of parameter {i} holds 8-bit codes in another memory format than the parameter")
         held = [g["lr"] for g in self.param_groups]
         super().load_state_dict(state_dict)
         taken = {}
@@ -215,9 +233,9 @@ class AdamW(torch.optim.Optimizer):
                 group["lr"] = lr.fill_(value)
             elif isinstance(group["lr"], Tensor) and group["params"]:
                 group["lr"] = group["lr"].detach().to(group["params"][0].device)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, params):
             for key, value in state_dict["state"].get(i, {}).items():
                 if isinstance(value, Tensor):
+                    if value.dtype == torch.float32 and value.shape == p.shape and not _same_order(value, p):
+                        value = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(value)
                     self.state[p][key] = value.detach().to(p.device, copy=True)

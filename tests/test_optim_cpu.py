@@ -198,3 +198,40 @@ def test_loading_keeps_the_learning_rate_tensor():
     plain.load_state_dict(make(source).state_dict())
     assert all(isinstance(g["lr"], torch.Tensor) and g["lr"] is not source and float(g["lr"]) == 0.25
                for g in plain.param_groups)
+
+
+def test_loading_states_of_another_memory_format():
+    """32-bit states come to the parameter's format with their values; codes cannot, as their scales go by
+    memory order.  Scales and counters have shapes of their own and are taken as they are."""
+    w = torch.randn(6, 5, 3, 3)
+
+    def make(fmt, bits):
+        p = torch.nn.Parameter(w.clone().contiguous(memory_format=fmt))
+        opt = optim.AdamW([p], state_bits=bits)
+        m, s = optim.new_state(p, bits)
+        v, t = optim.new_state(p, bits)
+        opt.state[p] = dict(step=optim.new_step("cpu", 3), exp_avg=m, exp_avg_sq=v)
+        if bits == 8:
+            opt.state[p].update(exp_avg_scale=s, exp_avg_sq_scale=t)
+        else:
+            m.copy_(w)
+            v.copy_(w * w)
+        return p, opt
+
+    for a, b in ((torch.contiguous_format, torch.channels_last), (torch.channels_last, torch.contiguous_format)):
+        _, source = make(a, 32)
+        p, opt = make(b, 32)
+        opt.load_state_dict(source.state_dict())
+        state = opt.state[p]
+        assert torch.equal(state["exp_avg"], w) and torch.equal(state["exp_avg_sq"], w * w)
+        assert state["exp_avg"].stride() == state["exp_avg_sq"].stride() == p.stride()
+        assert state["step"].tolist() == [3, 0]
+        _, source = make(a, 8)
+        p, opt = make(b, 8)
+        before = dict(opt.state[p])
+        with pytest.raises(ValueError, match="memory format"):
+            opt.load_state_dict(source.state_dict())
+        assert all(opt.state[p][k] is t for k, t in before.items())  # nothing was loaded
+        _, same = make(b, 8)
+        opt.load_state_dict(same.state_dict())
+        assert opt.state[p]["exp_avg"].stride() == p.stride() and opt.state[p]["exp_avg_scale"].shape == (2,)
