@@ -1,5 +1,6 @@
 // dcn_abi_train.cu -- the extern "C" entry points of the training-block
 // operators of include/dcn_b200.h: argument checks and dispatch.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -43,6 +44,9 @@ static int check_adamw(const dcn_adamw_options* o, const dcn_adamw_tensor* t, in
     return fail(DCN_ERR_INVALID_ARGUMENT, "betas must be in [0, 1), got (%g, %g)", o->beta1, o->beta2);
   if (!(o->eps >= 0.0 && isfinite(o->eps)))
     return fail(DCN_ERR_INVALID_ARGUMENT, "eps must be non-negative and finite, got %g", o->eps);
+  // the kernel's reciprocal takes a subnormal for 0: 0 / eps would be NaN
+  if (o->eps > 0.0 && !((float)o->eps >= FLT_MIN))
+    return fail(DCN_ERR_INVALID_ARGUMENT, "eps must be 0 or at least 2^-126, got %g", o->eps);
   if (!(o->weight_decay >= 0.0 && isfinite(o->weight_decay)))
     return fail(DCN_ERR_INVALID_ARGUMENT, "weight_decay must be non-negative and finite, got %g", o->weight_decay);
   std::vector<std::pair<uintptr_t, uintptr_t>> written;

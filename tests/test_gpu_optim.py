@@ -556,3 +556,10 @@ def test_loading_a_checkpoint_mapped_to_the_cpu(cuda, tmp_path):
     other.step()
     assert torch.equal(p, q)
     assert all(torch.equal(a.view(torch.uint8), other.state[q][k].view(torch.uint8)) for k, a in opt.state[p].items())
+
+
+def test_smallest_eps_divides_zero_by_it(cuda):
+    p = torch.ones(300, device=cuda)
+    zero = lambda: torch.zeros(300, device=cuda)  # noqa: E731
+    optim.adamw_step([p], [zero()], [zero()], [zero()], [optim.new_step(cuda)], lr=1e-3, eps=2.0 ** -126, weight_decay=0.0)
+    assert torch.equal(p, torch.ones_like(p))

@@ -235,3 +235,10 @@ def test_loading_states_of_another_memory_format():
         _, same = make(b, 8)
         opt.load_state_dict(same.state_dict())
         assert opt.state[p]["exp_avg"].stride() == p.stride() and opt.state[p]["exp_avg_scale"].shape == (2,)
+
+
+@pytest.mark.parametrize("eps", [1e-40, 2.0 ** -127, 1e-60])
+def test_adamw_refuses_an_eps_that_fp32_flushes(eps):
+    """A zero gradient on a zero state would become 0 / 0 where the formula says 0 / eps."""
+    rc, msg = _call(_options(eps=eps), _tensors(), 1)
+    assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "eps must be 0 or" in msg
