@@ -349,8 +349,8 @@ DCN_API int dcn_deform_conv2d_backward_overlap(const dcn_conv_desc *desc, const 
  *   w_gate, w_up  [hidden][channels]   b_gate, b_up  [hidden]    (NULL = none)
  *   w_down        [channels][hidden]   b_down        [channels]  (NULL = none)
  * b_gate and b_up go together.  All tensors are dense, of desc->dtype; x, y,
- * the weights and their gradients start on 16-byte boundaries, workspace and
- * saved state on 256-byte ones.  Any sizes (tokens may be 0).  Accumulation
+ * the weights and their gradients start on 16-byte boundaries, biases and their
+ * gradients on their elements', workspace and saved state on 256-byte ones.  Any sizes (tokens may be 0).  Accumulation
  * and elementwise work are fp32; the hidden values, and in the backward their
  * two gradients, are rounded to the dtype as operands of the products that
  * follow.  Activations: silu x / (1 + exp(-x)); gelu x Phi(x) (the exact
@@ -411,7 +411,9 @@ DCN_API int dcn_ffn_backward(const dcn_ffn_desc *desc, const dcn_ffn_tensors *t,
  * counter by one.  All tensors of one call are stepped together; calls that
  * share tensors or counters must not overlap on the GPU.
  * Refused: written memory (parameters, master copies, states, counters) that
- * overlaps other written memory, a gradient, grad_scale or lr_device.
+ * overlaps other written memory, a gradient, grad_scale or lr_device; pointers
+ * that are not aligned to their elements; an eps above 0 and below 2^-126, which
+ * the fp32 arithmetic would take for 0.
  * grad_scale (one fp32 on the device, or NULL for 1) multiplies the
  * gradients; when it is not finite the whole step is skipped and nothing is
  * written, counters included.  lr_device (one fp32 on the device), when not
@@ -447,7 +449,8 @@ DCN_API int dcn_adamw_step(const dcn_adamw_options *opt, const dcn_adamw_tensor 
  * two fp32 on the device.  A negative max_norm clips nothing.  When the norm
  * is not finite the factor is NaN, which makes dcn_adamw_step skip its step:
  * `factor` is meant as its grad_scale.  Sums are fp64 in a fixed order (the
- * result is reproducible bit for bit).
+ * result is reproducible bit for bit).  The workspace starts on a 256-byte
+ * boundary, gradients and outputs on their elements'.
  */
 typedef struct dcn_tensor_ref {
   const void *data;

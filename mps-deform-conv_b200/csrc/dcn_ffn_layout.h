@@ -202,7 +202,13 @@ struct Carver {
 // the weights' arrival (4096 x 14336 in bf16, one call: 1 row 68 us, 8 rows 73,
 // 16 rows 100, 32 rows 153; the tile products 77 at any of these), but on small
 // weights, where launches count, it stays ahead (512 x 2048, 32 rows: 12 us
-// against 21).
+// against 21).  The bound of 2^22 weights a matrix is near where the two meet: in
+// graphs, weights from memory, this form at 1024 x 4096 and 2048 x 2048 against the
+// tile products at 8 hidden units more takes, in bf16, 19 : 34 and 23 : 29 us on 16
+// rows, 30 : 34 and 37 : 29 on 32; in fp32 109 : 85 and 87 : 118 on 16 rows, 135 :
+// 85 and 141 : 118 on 32, where the meeting point lies lower.  fp32 up to 8 rows
+// always comes here (4096 x 14336: 1 row 161 us, 8 rows 417); not measured against
+// the tile products.
 inline bool few_rows(const FfnProblem& p, bool save) {
   if (save || p.M > 32) return false;
   if (p.dtype == DCN_FLOAT32) return p.M <= 8 || p.C * p.F <= (int64_t(1) << 22);

@@ -651,7 +651,7 @@ def gated_feed_forward(
     values are rounded to the dtype between the two products.  With
     ``set_training_cache(False)`` the forward keeps nothing for the backward,
     which then computes gate and up again.  The parameter-gradient hook is
-    called once for each of the three weights.
+    called once for each of the three weights (not by a compiled call).
     """
     if not torch.compiler.is_compiling():
         _refuse_forward_mode((input, w_gate, w_up, w_down, b_gate, b_up, b_down))
@@ -671,7 +671,8 @@ class GatedFeedForward2d(nn.Module):
     """Gated feed-forward block over the channels of a feature map (N, C, H, W).
 
     Stands after a deformable layer in a backbone block: a channels_last map is
-    read and returned as it is; other maps are brought to that order and back.
+    read and returned as it is; a contiguous map is brought to that order and
+    back; a map with other strides is copied and returned as channels_last.
     """
 
     def __init__(self, channels: int, hidden: int, bias: bool = True, activation: str = "silu"):

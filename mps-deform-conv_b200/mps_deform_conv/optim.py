@@ -83,6 +83,7 @@ def adamw_step(
         steps: One counter per tensor (``new_step``); several may be the same tensor.
             Each is advanced by one
         lr: Learning rate, or one float32 element on the device
+        eps: 0, or at least 2^-126
         masters: float32 copies that hold the parameters' values between steps
         exp_avg_scales, exp_avg_sq_scales: Scales of 8-bit states
         grad_scale: One float32 element on the device that multiplies the gradients
