@@ -697,7 +697,9 @@ __device__ __forceinline__ float column_sum(float (&v)[CB], int lane) {
 
 // ---------------------------------------------------------------- work
 // The pieces of a worker: whole tiles worker, worker + workers, ..., then its
-// share of the cut ones (struct Cut).
+// share of the cut ones (struct Cut).  CUT: the product may have cut tiles (the
+// gated passes never do, and keep the registers that this takes).
+template <bool CUT>
 struct Work {
   int worker, workers, nkb;
   int at, whole_end;            // whole tiles: at, at + workers, ... below whole_end
@@ -707,7 +709,7 @@ struct Work {
   DCN_HOST_DEVICE Work(const GemmArgs& a, int worker_, int workers_)
       : worker(worker_), workers(workers_), nkb(a.nk * a.nseg), at(worker_), unit(0), unit_end(0), slice(false) {
     whole_end = a.tiles_m * a.tiles_n * a.batches;
-    if (a.split) {
+    if (CUT && a.split) {
       whole_end -= a.cut.R;
       const int e = worker - a.cut.S * a.cut.R;
       slice = e < 0;
@@ -726,6 +728,7 @@ struct Work {
       slot = -1;
       return true;
     }
+    if (!CUT) return false;
     const Cut& c = a.cut;
     if (slice) {
       slice = false;
@@ -843,7 +846,7 @@ ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmA
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  Work w(a, blockIdx.x / CTAS, gridDim.x / CTAS);
+  Work<EPI == EPI_STORE> w(a, blockIdx.x / CTAS, gridDim.x / CTAS);
 
   if (warp >= EPI_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));

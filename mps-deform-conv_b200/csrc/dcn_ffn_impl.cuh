@@ -137,15 +137,16 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__
   const int64_t row = (int64_t)mt * BM * a.ctas + q * 32 + lane;
   const int c0 = nt * BN + c * 32;
   if (row - lane >= a.M || c0 >= a.N) return;
-  const Cut& cut = a.g.cut;
+  const Cut cut = a.g.cut;
   int run;
   const int n = cut.pieces(t, run);
   float4 v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* first = reinterpret_cast<const float4*>(a.partial + q * (32 * BN) + c * 1024) + lane;
+#pragma unroll 2
   for (int i = warp; i < n; i += 8) {
-    const int slot = cut.slot(t, i, run);
-    const float4* p = reinterpret_cast<const float4*>(a.partial + (int64_t)slot * a.ctas * (BM * BN) + q * (32 * BN) + c * 1024) + lane;
+    const float4* p = first + (int64_t)cut.slot(t, i, run) * a.ctas * (BM * BN / 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float4 f = p[j * 32];

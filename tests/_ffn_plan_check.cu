@@ -35,7 +35,7 @@ static void check_cut(int tiles, int W, int nkb) {
   std::vector<int> whole(tiles, 0), owner(2 * W, -1), covered((size_t)R * nkb, 0);
   long long busiest = 0;
   for (int w = 0; w < W; ++w) {
-    Work work(a, w, W);
+    Work<true> work(a, w, W);
     long long mine = 0;
     while (work.next(a)) {
       if (work.slot < 0) {
@@ -92,7 +92,7 @@ static bool check_plan(int64_t M, int64_t N, int64_t nkb, int batches, bool wide
   EXPECT(p.cut.R == tiles % p.workers, "%lld x %lld x %lld: %d tiles cut", (long long)M, (long long)N, (long long)nkb, p.cut.R);
   int64_t top = -1, longest = 0;
   for (int w = 0; w < p.workers; ++w) {
-    Work work(a, w, p.workers);
+    Work<true> work(a, w, p.workers);
     int64_t mine = 0;
     for (; work.next(a); mine += work.kb1 - work.kb0)
       if (work.slot > top) top = work.slot;
