@@ -196,7 +196,8 @@ class AdamW(torch.optim.Optimizer):
                     return [s[key] for s in states]
 
                 bits8 = group["state_bits"] == 8
-                lr, scale = group["lr"], grad_scale
+                # one tensor serves parameters on several devices
+                lr, scale = (t.to(device) if isinstance(t, Tensor) else t for t in (group["lr"], grad_scale))
                 adamw_step([p for p, _ in items], [p.grad for p, _ in items], column("exp_avg"),
                            column("exp_avg_sq"), column("step"), lr=lr, betas=group["betas"], eps=group["eps"],
                            weight_decay=group["weight_decay"], masters=column("master") if master else None,

@@ -242,3 +242,24 @@ def test_adamw_refuses_an_eps_that_fp32_flushes(eps):
     """A zero gradient on a zero state would become 0 / 0 where the formula says 0 / eps."""
     rc, msg = _call(_options(eps=eps), _tensors(), 1)
     assert rc == _abi.DCN_ERR_INVALID_ARGUMENT and "eps must be 0 or" in msg
+
+
+def test_scalars_reach_parameters_on_every_device(monkeypatch):
+    """Parameters on two devices and one factor and learning rate: each call gets them on its own device (else
+    the second would be refused after the first had been stepped).  Two devices without a GPU stand in."""
+    calls = []
+    monkeypatch.setattr(optim, "_require_cuda", lambda tensors, name: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(optim, "adamw_step", lambda params, *a, **kw: calls.append((params[0], kw["lr"], kw["grad_scale"])))
+    params = [torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4, device="meta"))]
+    for p in params:
+        p.grad = torch.zeros_like(p)
+    lr, factor = torch.tensor(1e-3), torch.tensor(0.5)
+    opt = optim.AdamW(params, lr=lr)
+    opt.step(grad_scale=factor)
+    assert [c[0].device.type for c in calls] == ["cpu", "meta"]
+    assert all(c[1].device == c[2].device == c[0].device for c in calls)
+    assert calls[0][1] is lr and calls[0][2] is factor  # no copy where they are
+    calls.clear()
+    optim.AdamW(params, lr=1e-3).step()
+    assert all(c[1] == 1e-3 and c[2] is None for c in calls)
