@@ -19,8 +19,7 @@
 // share of two instructions' operands, x read the same way.  fp32 data
 // multiplies on the CUDA cores.  The warps' sums meet in shared memory, the
 // CTAs' in each other's, both in a fixed order.  The hidden values are rounded to
-// the data's type between the two kernels, as they are in the tile products, so
-// that the number of rows in a call does not change how a row is rounded.
+// the data's type between the two kernels, where the tile products round them too.
 //
 // Measured (back-to-back calls in a graph): one row through 512 -> 2048 in bf16
 // 6.9 us, of it 1 us of weights at the memory's rate: two launches and their

@@ -41,13 +41,13 @@
 // PFLOP/s in bf16 until the power cap is reached.  Gated passes the epilogue: 35
 // instructions a value pair, issued by four warps a scheduler that wait for
 // TMEM and for one another's results in between.  23104 x 512 -> 2048 in bf16:
-// a pair of tiles every 8700 cycles, in 4100 of which the tensor cores work;
-// issue slots 50 % (gate and up) and 56 % (dhidden) busy, tensor cores 46 and
-// 23 %.  27200 x 256 -> 1024: 45 us with relu, 57 with gelu, 18 us of operations
+// a pair of tiles every 8000 cycles, in 4100 of which the tensor cores work;
+// issue slots 55 % (gate and up) and 56 % (dhidden) busy, tensor cores 51 and
+// 23 %.  27200 x 256 -> 1024: 42 us with relu, 53 with gelu, 18 us of operations
 // at the measured matrix rate.  Arithmetic in packed pairs (f32x2), not used
 // here, gained 2 % where gate and up are 92416 x 512 -> 2048 (419 us against 428;
 // forward and backward 1742 against 1752) and nothing in that case (both products
-// 81.2 us both ways).
+// 81.2 us both ways), timed while the cut's state still took registers here.
 //
 // Work is dealt in whole tiles: worker w takes tiles w, w + W, ...  Where the
 // last wave would leave many of the W workers idle, its R tiles are cut along

@@ -8,8 +8,8 @@
 //
 // Work: 6 M C F flops forward, 12 M C F backward (M rows, C channels, F hidden).
 // Measured, forward and backward: 92416 x 512 -> 2048 in bf16 1.75 ms of kernels
-// (1.0 PFLOP/s; 2.05 to 2.08 ms once steady calls reach the power cap), 921600 x
-// 64 -> 170 in fp16 0.98 ms, 8192 x 128 -> 512 in fp32 0.24 ms.
+// (1.0 PFLOP/s; 2.06 to 2.08 ms once steady calls reach the power cap), 921600 x
+// 64 -> 170 in fp16 0.88 ms, 8192 x 128 -> 512 in fp32 0.26 ms.
 // The hidden values and the two hidden gradients are rounded to the data's
 // type, as operands of the following products; everything else stays in 32
 // bits to the final rounding.
