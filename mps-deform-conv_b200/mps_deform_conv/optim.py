@@ -197,7 +197,7 @@ class AdamW(torch.optim.Optimizer):
 
                 bits8 = group["state_bits"] == 8
                 # one tensor serves parameters on several devices
-                lr, scale = (t.to(device) if isinstance(t, Tensor) else t for t in (group["lr"], grad_scale))
+                lr, scale = (t.to(device) if isinstance(t, Tensor) and t.is_cuda else t for t in (group["lr"], grad_scale))
                 adamw_step([p for p, _ in items], [p.grad for p, _ in items], column("exp_avg"),
                            column("exp_avg_sq"), column("step"), lr=lr, betas=group["betas"], eps=group["eps"],
                            weight_decay=group["weight_decay"], masters=column("master") if master else None,

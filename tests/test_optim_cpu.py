@@ -246,20 +246,23 @@ def test_adamw_refuses_an_eps_that_fp32_flushes(eps):
 
 def test_scalars_reach_parameters_on_every_device(monkeypatch):
     """Parameters on two devices and one factor and learning rate: each call gets them on its own device (else
-    the second would be refused after the first had been stepped).  Two devices without a GPU stand in."""
+    the second would be refused after the first had been stepped).  Fake tensors stand in for two GPUs.  A host
+    tensor is left to the refusal of adamw_step: it would make every step wait."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
     calls = []
-    monkeypatch.setattr(optim, "_require_cuda", lambda tensors, name: None)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(optim, "adamw_step", lambda params, *a, **kw: calls.append((params[0], kw["lr"], kw["grad_scale"])))
-    params = [torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4, device="meta"))]
-    for p in params:
-        p.grad = torch.zeros_like(p)
-    lr, factor = torch.tensor(1e-3), torch.tensor(0.5)
-    opt = optim.AdamW(params, lr=lr)
-    opt.step(grad_scale=factor)
-    assert [c[0].device.type for c in calls] == ["cpu", "meta"]
-    assert all(c[1].device == c[2].device == c[0].device for c in calls)
-    assert calls[0][1] is lr and calls[0][2] is factor  # no copy where they are
-    calls.clear()
-    optim.AdamW(params, lr=1e-3).step()
-    assert all(c[1] == 1e-3 and c[2] is None for c in calls)
+    monkeypatch.setattr(optim.AdamW, "_init_state", lambda self, p, group: dict(step=p, exp_avg=p, exp_avg_sq=p))
+    with FakeTensorMode():
+        params = [torch.nn.Parameter(torch.zeros(4, device=f"cuda:{k}")) for k in range(2)]
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        lr, factor = torch.ones((), device="cuda:0"), torch.ones((), device="cuda:1")
+        optim.AdamW(params, lr=lr).step(grad_scale=factor)
+        assert [c[0].device.index for c in calls] == [0, 1]
+        assert all(c[1].device == c[2].device == c[0].device for c in calls)
+        assert calls[0][1] is lr and calls[1][2] is factor  # no copy where they are
+        calls.clear()
+        host = torch.ones(())
+        optim.AdamW(params, lr=host).step()
+        assert all(c[1] is host and c[2] is None for c in calls)
